@@ -18,6 +18,8 @@ ABI_VERSION = 3
 EXPORTS = (
     "ga_init", "ga_attn_workspace_bytes", "ga_attn_decode", "ga_attn_extend", "ga_attn_decode_noalloc", "ga_attn_merge",
     "ga_attn_exchange_merge",
+    "ga_paged_workspace_bytes", "ga_paged_attend",
+    "ga_pages_scratch_bytes", "ga_pages_copy", "ga_pages_fork", "ga_pages_free", "ga_pages_evict", "ga_pages_grow", "ga_pages_compact",
     "ga_gdn_recurrent", "ga_gdn_verify", "ga_fp8_tensor_peak", "ga_last_launch_count", "ga_attn_workspace_status", "ga_attn_workspace_clear_status", "ga_last_error",
     "ga_abi_version", "ga_sm_count",
 )
@@ -100,6 +102,34 @@ class GaGdnVerifyParams(ctypes.Structure):
     ]
 
 
+class GaPagedParams(ctypes.Structure):
+    _fields_ = [
+        ("kv_type", c_int32), ("q", c_void_p), ("q_is_bf16", c_int32), ("q_stride_tok", c_int64), ("q_stride_head", c_int64),
+        ("k_cache", c_void_p), ("v_cache", c_void_p),
+        ("k_stride_page", c_int64), ("k_stride_tok", c_int64), ("k_stride_head", c_int64),
+        ("v_stride_page", c_int64), ("v_stride_tok", c_int64), ("v_stride_head", c_int64),
+        ("num_pages", c_int32), ("page_size", c_int32),
+        ("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32),
+        ("page_table", c_void_p), ("pt_stride_row", c_int64), ("pt_stride_col", c_int64), ("pt_cols", c_int32),
+        ("cache_seqlens", c_void_p), ("cu_seqlens_q", c_void_p),
+        ("k_descale", c_void_p), ("kd_stride_b", c_int64), ("kd_stride_h", c_int64),
+        ("v_descale", c_void_p), ("vd_stride_b", c_int64), ("vd_stride_h", c_int64),
+        ("out", c_void_p), ("o_stride_tok", c_int64), ("o_stride_head", c_int64),
+        ("lse", c_void_p), ("total_q", c_int64),
+        ("batch", c_int32), ("max_seqlen_q", c_int32), ("window_left", c_int32), ("sink_tokens", c_int32),
+        ("softmax_scale", c_float), ("status", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class GaPagePool(ctypes.Structure):
+    _fields_ = [
+        ("base", c_void_p), ("page_stride", c_void_p), ("tok_bytes", c_void_p), ("chunk_tensor", c_void_p), ("chunk_first", c_void_p),
+        ("tensors", c_int32), ("chunks", c_int32), ("num_pages", c_int32), ("page_size", c_int32),
+        ("page_table", c_void_p), ("pt_stride_row", c_int64), ("pt_stride_col", c_int64), ("rows", c_int32), ("cols", c_int32),
+        ("seqlens", c_void_p), ("refs", c_void_p), ("status", c_void_p), ("scratch", c_void_p), ("scratch_bytes", c_size_t),
+    ]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -121,13 +151,25 @@ def lib() -> ctypes.CDLL:
         handle.ga_init.restype = c_int
         handle.ga_attn_workspace_bytes.argtypes = [c_int, c_int]
         handle.ga_attn_workspace_bytes.restype = c_size_t
+        handle.ga_paged_workspace_bytes.argtypes = [c_int, c_int]
+        handle.ga_paged_workspace_bytes.restype = c_size_t
         for name, ptype in (("ga_attn_decode", GaAttnParams), ("ga_attn_extend", GaAttnParams),
                             ("ga_attn_decode_noalloc", GaAttnParams),
                             ("ga_attn_merge", GaMergeParams), ("ga_attn_exchange_merge", GaExchangeParams),
+                            ("ga_paged_attend", GaPagedParams),
                             ("ga_gdn_recurrent", GaGdnParams),
                             ("ga_gdn_verify", GaGdnVerifyParams)):
             fn = getattr(handle, name)
             fn.argtypes = [POINTER(ptype), c_void_p]
+            fn.restype = c_int
+        pool = POINTER(GaPagePool)
+        handle.ga_pages_scratch_bytes.argtypes = [pool, c_int]
+        handle.ga_pages_scratch_bytes.restype = c_size_t
+        for name, more in (("copy", [c_void_p, c_void_p, c_int, c_int]), ("fork", [c_void_p, c_void_p, c_int, c_int]),
+                           ("free", [c_void_p, c_int, c_int]), ("evict", [c_void_p, c_int, c_int, c_int, c_int]),
+                           ("grow", [c_void_p, c_void_p, c_int, c_int, c_int]), ("compact", [c_void_p, c_void_p])):
+            fn = getattr(handle, f"ga_pages_{name}")
+            fn.argtypes = [pool, *more, c_void_p]
             fn.restype = c_int
         handle.ga_fp8_tensor_peak.argtypes = [c_void_p, c_void_p, POINTER(c_float)]
         handle.ga_fp8_tensor_peak.restype = c_int

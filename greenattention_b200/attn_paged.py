@@ -1,0 +1,234 @@
+"""Front-end of the attention over 16-bit and e4m3 paged caches, with first tokens that stay visible beside a window.
+
+The call contract is that of ``attn_decode`` (same names, layouts, causal and window rules), with these differences:
+
+* ``k_cache`` / ``v_cache`` are bf16, fp16 or e4m3; ``q`` has the cache's type (beside e4m3: e4m3, or bf16, which is
+  rounded to e4m3 in the kernel), ``out`` too (beside e4m3: bf16). ``head_dim`` 64, 128 or 256, any number of query
+  heads per kv head, any power-of-two page size from 1 token, any ``max_seqlen_q``;
+* ``sink_tokens=S`` with ``window_size=(W, 0)``: the query at position ``p`` attends the keys ``[p - W, p]`` and the
+  request's first ``S`` keys. The pages between the first tokens and the window are never read, so their page-table
+  entries may be those of released pages (``kv_pages.PagePool.evict``) and the lengths go on counting;
+* a row that sees no key gets zeros and an LSE of -inf; rows of ``out`` and ``lse`` behind the last request's are left
+  as they were. Non-finite values count where they are visible; a K or V row that no query of the call's request sees
+  is not read. (Among the new tokens of one request a later token's non-finite V row reaches the earlier rows.)
+
+Every call brings its own scratch (from torch's caching allocator, on the current stream), so calls on several streams
+and captured graphs do not share any. What the kernels cannot serve is declined with a reason (``dispatch.Declined``).
+
+``attend(**kw)`` is the direct entry. ``select`` is registered for the ops ``decode``, ``verify`` and ``extend``: calls with
+``sink_tokens`` come here, and with ``GREEN_ATTN_KV16=1`` every call over a paged bf16 / fp16 cache does.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import logging
+from typing import Callable, Optional, Union
+
+import torch
+
+from greenattention_b200 import _C, attn_decode, dispatch
+
+HEAD_DIMS = (64, 128, 256)
+KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
+FP8 = torch.float8_e4m3fn
+STATUS_NAMES = {
+    3: "a page id was out of range (its keys were taken as zeros)",
+    5: "a cache_seqlens entry exceeded page_table.shape[1] * page_size",
+}
+_ALLOWED = attn_decode._ALLOWED | {"sink_tokens"}
+_TENSORS = ("k_cache", "v_cache", "page_table", "cache_seqlens", "cu_seqlens_q")
+logger = logging.getLogger(__name__)
+
+_status: dict = {}           # device index -> int32 word the kernels leave a non-zero value in
+_workspace_bytes: dict = {}  # (device index, batch) -> bytes
+
+
+def ensure_ready(device: Union[torch.device, int, None] = None) -> None:
+    """Load the library and set up ``device``. Idempotent; runs at the first call and has to have run before a CUDA
+    graph is captured."""
+    if not torch.cuda.is_available():
+        raise _C.GreenAttentionError("no CUDA device: the green kernels have no CPU path")
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    if index in _status:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        raise _C.GreenAttentionError("ensure_ready() has to run before a CUDA graph is captured")
+    _C.init(index)
+    _status[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+    torch.cuda.synchronize(index)  # the word is zero before a kernel on any stream may set it
+
+
+def check_status(device: Union[torch.device, int, None] = None, reset: bool = True) -> int:
+    """The status word (0 = fine; ``STATUS_NAMES``), logged when it is not 0 and put back. Synchronises."""
+    dev = torch.device("cuda") if device is None else torch.device(device)
+    index = torch.cuda.current_device() if dev.index is None else dev.index
+    if index not in _status:
+        return 0
+    val = int(_status[index].item())
+    if val:
+        logger.error("green_attention: paged attention status %d on cuda:%d: %s", val, index, STATUS_NAMES.get(val, "unknown"))
+        if reset:
+            _status[index].zero_()
+    return val
+
+
+def _reason(kw: dict) -> Optional[str]:
+    for name, val in kw.items():
+        if name not in _ALLOWED and val is not None:
+            return f"unsupported arg {name}"
+    for name in ("q",) + _TENSORS:
+        if not isinstance(kw.get(name), torch.Tensor):
+            return f"not a paged varlen call ({name})"
+    q, kc, vc, pt, cs, cu = (kw[n] for n in ("q",) + _TENSORS)
+    if kc.dtype not in KV_TYPES or vc.dtype != kc.dtype:
+        return f"kv dtype {kc.dtype} / {vc.dtype}"
+    if q.dtype != kc.dtype and not (kc.dtype == FP8 and q.dtype == torch.bfloat16):
+        return f"q dtype {q.dtype} beside a {kc.dtype} cache"
+    if q.dim() != 3 or kc.dim() != 4 or kc.shape != vc.shape:
+        return "q or kv rank, or k/v shapes differ"
+    total, qh, hd = q.shape
+    pages, page, kvh, khd = kc.shape
+    if hd not in HEAD_DIMS or khd != hd or not kvh or not qh or qh % kvh:
+        return f"q shape: no kernel for (head_dim={hd}, q_heads={qh}, kv_heads={kvh})"
+    if page <= 0 or page & (page - 1):
+        return "page_size not a power of two"
+    el = kc.element_size()
+    for t in (kc, vc):
+        s0, s1, s2, s3 = t.stride()
+        if s3 != 1 or (s0 | s1 | s2) * el % 16 or t.data_ptr() % 16:
+            return "kv layout: last stride 1, other strides and the base multiples of 16 bytes"
+    s0, s1, s2 = q.stride()
+    if s2 != 1 or (s0 | s1) % 4 or q.data_ptr() % (4 * q.element_size()):
+        return "q layout: last stride 1, other strides and the base multiples of 4 elements"
+    if pt.dtype != torch.int32 or pt.dim() != 2 or cs.dtype != torch.int32 or cs.dim() != 1 or cu.dtype != torch.int32 or cu.dim() != 1:
+        return "page_table / cache_seqlens / cu_seqlens_q dtype or rank"
+    batch = cs.shape[0]
+    if batch == 0 or pt.shape[0] != batch or cu.shape[0] != batch + 1:
+        return "batch mismatch"
+    if cs.stride(0) != 1 and batch > 1 or cu.stride(0) != 1:
+        return "cache_seqlens / cu_seqlens_q stride"
+    mq = kw.get("max_seqlen_q")
+    if not isinstance(mq, int) or isinstance(mq, bool) or mq < 1:
+        return f"max_seqlen_q {mq} is not a positive int"
+    if mq > 1 and not kw.get("causal", False):
+        return "non-causal call with several query tokens"
+    if kw.get("softcap"):
+        return "softcap"
+    window = attn_decode._window_left(kw)
+    if isinstance(window, str):
+        return window
+    sinks = kw.get("sink_tokens")
+    if sinks is not None and (not isinstance(sinks, int) or isinstance(sinks, bool) or not 0 <= sinks < 1 << 31):
+        return f"sink_tokens {sinks} is not a count"
+    dev = q.device
+    for t in (kc, vc, pt, cs, cu):
+        if t.device != dev:
+            return f"a tensor is on {t.device}, q on {dev}"
+    for name in ("k_descale", "v_descale"):
+        t = kw.get(name)
+        if t is not None:
+            if t.device != dev:
+                return f"{name} is on {t.device}, q on {dev}"
+            why = attn_decode._descale_reason(t, batch, kvh, name)
+            if why:
+                return why
+    out = kw.get("out")
+    if out is not None:
+        want = torch.bfloat16 if kc.dtype == FP8 else kc.dtype
+        if not isinstance(out, torch.Tensor) or out.device != dev:
+            return "out is not a tensor on q's device"
+        if out.dtype != want or out.shape != q.shape or out.stride(2) != 1:
+            return f"out must be {want} of q's shape with last stride 1"
+        s0, s1, _ = out.stride()
+        if (s0 | s1) % 4 or out.data_ptr() % 8 or (qh > 1 and s1 < hd) or (total > 1 and s0 < hd):
+            return "out layout: rows must not overlap, strides and the base multiples of 4 elements"
+    if not q.is_cuda:
+        return "tensors are on the host: the green kernels have no CPU path"
+    return None
+
+
+def _launch(
+    *, q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, window_size=(-1, -1), sink_tokens=None,
+    softmax_scale=None, return_softmax_lse=False, out=None, k_descale=None, v_descale=None, causal=False, **_,
+):
+    dev = q.device
+    index = dev.index
+    if index not in _status:
+        ensure_ready(dev)
+    total, qh, hd = q.shape
+    kv = k_cache.dtype
+    if out is None:
+        out = torch.empty(q.shape, dtype=torch.bfloat16 if kv == FP8 else kv, device=dev)
+    lse = torch.empty((qh, total), dtype=torch.float32, device=dev) if return_softmax_lse else None
+    pages, page, kvh, _ = k_cache.shape
+    batch, cols = page_table.shape
+    lib = _C.lib()
+    nbytes = _workspace_bytes.get((index, batch))
+    if nbytes is None:
+        nbytes = _workspace_bytes[(index, batch)] = lib.ga_paged_workspace_bytes(index, batch)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    q0, q1, _ = q.stride()
+    k0, k1, k2, _ = k_cache.stride()
+    v0, v1, v2, _ = v_cache.stride()
+    o0, o1, _ = out.stride()
+    kd = vd = None
+    kd0 = kd1 = vd0 = vd1 = 0
+    if k_descale is not None:
+        kd, kd0, kd1 = k_descale.data_ptr(), k_descale.stride(0) if k_descale.shape[0] > 1 else 0, k_descale.stride(1)
+    if v_descale is not None:
+        vd, vd0, vd1 = v_descale.data_ptr(), v_descale.stride(0) if v_descale.shape[0] > 1 else 0, v_descale.stride(1)
+    left = -1 if window_size is None or window_size[0] is None else int(window_size[0])
+    p = _C.GaPagedParams(
+        KV_TYPES[kv], q.data_ptr(), q.dtype == torch.bfloat16, q0, q1, k_cache.data_ptr(), v_cache.data_ptr(),
+        k0, k1, k2, v0, v1, v2, pages, page, qh, kvh, hd,
+        page_table.data_ptr(), page_table.stride(0), page_table.stride(1), cols,
+        cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), kd, kd0, kd1, vd, vd0, vd1,
+        out.data_ptr(), o0, o1, None if lse is None else lse.data_ptr(), total,
+        batch, max_seqlen_q, min(left, 1 << 30), sink_tokens or 0, hd**-0.5 if softmax_scale is None else softmax_scale,
+        _status[index].data_ptr(), ws.data_ptr(), nbytes,
+    )
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == index:
+        rc = lib.ga_paged_attend(ctypes.byref(p), stream)
+    else:
+        with torch.cuda.device(dev):  # the library launches on the current device
+            rc = lib.ga_paged_attend(ctypes.byref(p), stream)
+    _C.check(rc, "ga_paged_attend")
+    return (out, lse) if return_softmax_lse else out
+
+
+def attend(**kw):
+    """Attention over a paged cache (see the module); ``out``, or ``(out, lse)`` with ``return_softmax_lse``. Raises
+    ``dispatch.Declined`` with the reason for a call outside what the kernels serve."""
+    why = _reason(kw)
+    if why is not None:
+        raise dispatch.Declined(f"attn_paged: {why}")
+    return _launch(**kw)
+
+
+def select(kw: dict) -> Union[Callable, str]:
+    """The launcher for this call or why there is none, from shapes, types and Python scalars only."""
+    why = _reason(kw)
+    if why is not None:
+        return why
+    if kw["q"].device.index not in _status:
+        return "kernel not prewarmed for this device"
+    return _launch
+
+
+def _select_routed(kw: dict) -> Union[Callable, str]:
+    if kw.get("sink_tokens") is None and not dispatch.takes_kv16(kw):
+        return "attn_paged: no sink_tokens, and no 16-bit cache with GREEN_ATTN_KV16=1"
+    return select(kw)
+
+
+def _prewarm(backend) -> None:
+    ensure_ready()
+    check_status()
+
+
+dispatch.register("decode", _select_routed, prewarm=_prewarm)
+dispatch.register("verify", _select_routed)
+dispatch.register("extend", _select_routed)

@@ -10,6 +10,7 @@ from __future__ import annotations
 from sglang.srt.layers.attention.flashattention_backend import FlashAttentionBackend
 
 from greenattention_b200 import attn_decode  # noqa: F401  (registers the decode/verify/extend kernels)
+from greenattention_b200 import attn_paged  # noqa: F401  (the same ops over 16-bit caches and with first tokens)
 from greenattention_b200 import dispatch
 
 SGLANG_READS = {

@@ -1,5 +1,5 @@
 """Ahead-of-time build of the CUDA library for sm_100a (replaces the reference's runtime nvcc JIT,
-``green_attention/jit.py:139-183``): one ``nvcc`` call over ``csrc/api.cu`` producing
+``green_attention/jit.py:139-183``): one ``nvcc`` call for each translation unit of ``csrc`` and one that links
 ``greenattention_b200/_lib/libgreen_attention.so`` in the source tree. nvcc cross-compiles, so no GPU is needed.
 
     python -m greenattention_b200.build [--force] [--verbose]
@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
@@ -21,9 +22,10 @@ LIB_PATH = os.path.join(LIB_DIR, "libgreen_attention.so")
 STAMP = os.path.join(LIB_DIR, "build.stamp")
 
 FLAGS = [
-    "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo", 
-    "-Xcompiler", "-fPIC", "-shared", "--expt-relaxed-constexpr",
+    "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
+    "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
 ]
+UNITS = ("api.cu", "paged.cu", "pages.cu")  # translation units, compiled side by side
 
 
 def _nvcc() -> str:
@@ -56,14 +58,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
     ident = _identity()
     if not force and os.path.exists(LIB_PATH) and os.path.exists(STAMP) and open(STAMP).read().strip() == ident:
         return LIB_PATH
-    cmd = [_nvcc(), *FLAGS, "-I", INCLUDE, "-o", LIB_PATH, os.path.join(CSRC, "api.cu")]
-    if verbose:
-        cmd.insert(1, "-Xptxas")
-        cmd.insert(2, "-v")
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or proc.returncode:
-        sys.stderr.write(proc.stdout + proc.stderr)
-    if proc.returncode:
+    more = ["-Xptxas", "-v"] if verbose else []
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, os.path.splitext(u)[0] + ".o") for u in UNITS]
+        cmds = [[_nvcc(), *more, *FLAGS, "-I", INCLUDE, "-c", "-o", o, os.path.join(CSRC, u)] for u, o in zip(UNITS, objs)]
+        procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for c in cmds]
+        said = [p.communicate()[0] for p in procs]
+        failed = any(p.returncode for p in procs)
+        if not failed:
+            link = subprocess.run([_nvcc(), *FLAGS, "-shared", "-o", LIB_PATH, *objs], capture_output=True, text=True)
+            said.append(link.stdout + link.stderr)
+            failed = link.returncode != 0
+    if verbose or failed:
+        sys.stderr.write("".join(said))
+    if failed:
         raise RuntimeError("nvcc failed building libgreen_attention.so")
     with open(STAMP, "w") as f:
         f.write(ident)

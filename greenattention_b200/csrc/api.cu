@@ -19,6 +19,7 @@
 #include "attn_wide.cuh"
 #include "gdn_recurrent.cuh"
 #include "gdn_verify.cuh"
+#include "api_internal.h"
 
 namespace {
 
@@ -374,7 +375,7 @@ int init_current_device(int device) {
     if (qres != cudaDriverEntryPointSuccess || !fn) return fail("cuTensorMapEncodeTiled is not available");
     g_encode = reinterpret_cast<EncodeTiledFn>(fn);
   }
-  if (set_all_smem_limits()) return 1;
+  if (set_all_smem_limits() || ga::api::init_paged() || ga::api::init_pages()) return 1;
   std::lock_guard<std::mutex> lock(g_mu);
   g_dev[device].sm_count = prop.multiProcessorCount;
   g_dev[device].ready = true;
@@ -382,6 +383,24 @@ int init_current_device(int device) {
 }
 
 }  // namespace
+
+namespace ga {
+namespace api {
+int fail(const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return 1;
+}
+int device(int* dev, int* sm) {
+  if (current_device(dev)) return 1;
+  *sm = g_dev[*dev].sm_count;
+  return 0;
+}
+void launches(int n) { g_launches = n; }
+}  // namespace api
+}  // namespace ga
 
 extern "C" {
 

@@ -1,0 +1,760 @@
+// Attention over paged caches of 16-bit (bf16, fp16) or e4m3 keys and values, with an optional left window and first
+// tokens that stay visible beside it. Decode, verify and (row block by row block) prompts.
+//
+// Mathematics, per query row i at position p_i = len - new + t of its request and for one kv head:
+//     s_ij = scale * k_descale * q_i . k_j,   key j visible iff j <= p_i and (W < 0 or j >= p_i - W or j < S)
+//     o_i  = v_descale * sum_j softmax_j(s_ij) v_j,   lse_i = ln sum_j exp s_ij;  a row without keys: o = 0, lse = -inf
+// evaluated in one pass with the running maximum m and sum l of the row (log2 domain):
+//     m' = max(m, max_j s_ij),  l' = l 2^(m - m') + sum_j 2^(s_ij - m'),  O' = O 2^(m - m') + sum_j 2^(s_ij - m') v_j.
+// Products run on the warp-level 16-bit tensor path with 32-bit accumulators; m, l, O and the partial results are
+// 32 bits. P is rounded to the cache's 16-bit type before P V (bf16 2^-9, fp16 2^-12 of each probability, below the
+// half step 2^-9 / 2^-12 of the output's own rounding); an e4m3 value is an exact fp16 value, so an e4m3 cache runs on
+// the fp16 path with P in fp16. Queries beside an e4m3 cache are e4m3, or bf16 rounded to e4m3 (the contract of the
+// FP8 kernels next to this one).
+//
+// What bounds it: the cache's bytes. A warp owns one kv head and a private ring of tiles in shared memory that it fills
+// with 16-byte cp.async and drains itself, so there is no barrier between warps: the warps of a CTA walk the same
+// tokens, one kv head each, which makes the bytes of a token run contiguous in DRAM within a short window whatever the
+// page size (from one token up), strides and alignment. CTAs with fewer kv heads than warps are several walkers of HG
+// warps each ("virtual CTAs"). The call is one stream of tiles ordered by (request, head group, row block), cut evenly
+// over the walkers on the device from the live lengths; a unit that is cut leaves normalised 32-bit partials and their
+// log2 LSE in the workspace, folded in slice order by attn_paged_combine (no atomics: results do not depend on
+// scheduling).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "ga_common.cuh"
+
+namespace ga {
+namespace paged {
+
+enum : int { KV_BF16 = 0, KV_FP16 = 1, KV_E4M3 = 2 };
+enum : int { Q_SAME = 0, Q_BF16_TO_E4M3 = 1 };
+
+constexpr int MAX_WARPS = 8;
+constexpr int SLOT_FLOATS = 32768;  // O floats of a CTA's workspace slot: warps x rows x head_dim of every instance
+constexpr int SLOT_ROWS = 256;      // rows of a CTA's workspace slot, at most
+
+struct PagedDev {
+  const uint8_t* q;
+  int q_kind;
+  long long q_s0, q_s1;  // elements
+  const uint8_t* k;
+  const uint8_t* v;
+  long long k_s0, k_s1, k_s2, v_s0, v_s1, v_s2;  // page, token, head (bytes)
+  int page_shift, page_mask, num_pages;
+  int kvh, gqa, q_heads;
+  const int* pt;
+  long long pt_s0, pt_s1;
+  int pt_cols;
+  const int* seqlens;
+  const int* cu;
+  const float* kd;
+  const float* vd;
+  long long kd_s0, kd_s1, vd_s0, vd_s1;
+  void* out;
+  long long o_s0, o_s1;  // elements
+  float* lse;
+  int total_q, batch, max_q;
+  int window, sinks;  // window < 0: none (sinks is 0 then)
+  float scale_log2;
+  int hg, groups, walkers;  // kv heads per walker, walkers' head groups per request, walkers per CTA
+  int nrb, upr;             // row blocks and units per request (split mode)
+  int* status;
+  int* prefix;
+  float* ws_o;
+  float* ws_lse;
+};
+
+// What the query tokens [t0, t0 + nt) of request b see: tiles of T tokens, the sinks' first, then one run that ends
+// with the last visible key. Tile i starts at token T * (i < ns ? i : tlo + i - ns).
+struct Req {
+  int q0, nq;    // first query row and tokens of the request
+  int pos0;      // position of token 0
+  int kend;      // keys from here on are invisible to every row
+  int lower;     // first key of the run (window) some row sees
+  int ns, tlo, cnt;
+};
+__device__ __forceinline__ int new_tokens(const PagedDev& p, int b, int& q0) {
+  q0 = p.cu[b];
+  int q1 = p.cu[b + 1];
+  if (q0 < 0 || q0 > p.total_q) return 0;
+  if (q1 > p.total_q) q1 = p.total_q;
+  return q1 - q0;
+}
+template <int T>
+__device__ __forceinline__ Req req_info(const PagedDev& p, int b, int t0, int nt) {
+  Req r;
+  int L = p.seqlens[b];
+  const long long cap = static_cast<long long>(p.pt_cols) << p.page_shift;
+  if (L > cap) {
+    L = static_cast<int>(cap);
+    atomicExch(p.status, GA_ST_LEN_RANGE);
+  }
+  const int ql = new_tokens(p, b, r.q0);
+  r.nq = ql < p.max_q ? ql : p.max_q;
+  r.pos0 = L - ql;
+  if (nt > r.nq - t0) nt = r.nq - t0;
+  r.kend = r.pos0 + t0 + nt;
+  r.lower = 0;
+  r.ns = r.tlo = r.cnt = 0;
+  if (L <= 0 || nt <= 0 || r.kend <= 0) return r;
+  if (p.window >= 0) {
+    const int lo = r.pos0 + t0 - p.window;
+    r.lower = lo > 0 ? lo : 0;
+  }
+  r.tlo = r.lower / T;
+  const int send = p.sinks < r.lower ? p.sinks : r.lower;
+  const int ns = (send + T - 1) / T;
+  r.ns = ns < r.tlo ? ns : r.tlo;
+  r.cnt = r.ns + (r.kend + T - 1) / T - r.tlo;
+  return r;
+}
+
+// T tiles are cut over at most G walkers, each of which gets MIN_TILES tiles at least; first tile of walker c's slice.
+constexpr int MIN_TILES = 2;
+__device__ __forceinline__ int walkers_for(long long T, int G) {
+  const long long most = T / MIN_TILES;
+  return most < G ? (most > 0 ? static_cast<int>(most) : 1) : G;
+}
+__device__ __forceinline__ long long slice(long long T, int G, int c) { return c >= G ? T : T * c / G; }
+
+// Exclusive prefix over the requests' counts, by the whole CTA (NT threads), and the request that holds item g0[s] for
+// each of the CTA's walkers s. find_b < 0: past the end. `publish`: this CTA writes p.prefix.
+template <int NT, typename CountFn>
+__device__ __forceinline__ long long plan(const PagedDev& p, CountFn count, int mul, long long (*g_of)(long long, int, int),
+                                          int G, int vc0, int walkers, int* find_b, long long* find_pre, bool publish) {
+  __shared__ long long wsum[NT / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.batch + NT - 1) / NT;
+  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += count(b);
+  long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 31) wsum[warp] = incl;
+  if (tid < MAX_WARPS) find_b[tid] = -1;
+  __syncthreads();
+  long long base = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 32; ++w) {
+    if (w < warp) base += wsum[w];
+    total += wsum[w];
+  }
+  const long long T = total * mul;
+  const long long pre = base + incl - mine;
+  for (int s = 0; s < walkers; ++s) {
+    const long long g0 = g_of(T, G, vc0 + s);
+    if (g0 < T && mine > 0 && pre * mul <= g0 && g0 < (pre + mine) * mul) {
+      long long at = pre;
+      for (int b = b0; b < b1; ++b) {
+        const int c = count(b);
+        if (g0 < (at + c) * mul) {
+          find_b[s] = b;
+          find_pre[s] = at;
+          break;
+        }
+        at += c;
+      }
+    }
+  }
+  if (publish) {
+    long long at = pre;
+    for (int b = b0; b < b1; ++b) {
+      p.prefix[b] = static_cast<int>(at);
+      at += count(b);
+    }
+    if (tid == 0) p.prefix[p.batch] = static_cast<int>(total);
+  }
+  __syncthreads();
+  return T;
+}
+__device__ __forceinline__ long long at_cut(long long T, int G, int c) { return slice(T, walkers_for(T, G), c); }
+__device__ __forceinline__ long long at_index(long long, int, int c) { return c; }
+
+// ---------------------------------------------------------------------------------------------------- fragments
+
+template <int KV>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (KV == KV_BF16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <int KV>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if (KV == KV_BF16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&v);
+  }
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+// Two e4m3 values (the low 16 bits) as two fp16 values: exact.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(v)));
+  return r;
+}
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Byte offset of 16-byte chunk `c` of row `r` in a tile whose rows hold RB bytes: rows lie one after the other in
+// 128-byte lines, and the chunks of a line are permuted so that eight rows' chunks c fall into different banks.
+template <int RB>
+__device__ __forceinline__ uint32_t swz(int r, int c) {
+  if (RB >= 128) return r * RB + (c >> 3) * 128 + (((c & 7) ^ (r & 7)) << 4);
+  const int line = r >> 1, cc = (r & 1) * 4 + c;  // RB == 64
+  return line * 128 + (((cc ^ line) & 7) << 4);
+}
+
+template <int HD_, int KV_, int MT_>
+struct Inst {
+  static constexpr int HD = HD_, KV = KV_, MT = MT_;
+  static constexpr int EB = KV == KV_E4M3 ? 1 : 2;
+  static constexpr int RB = HD * EB;                       // bytes of a row of one head
+  static constexpr int T = RB >= 256 ? 16 : 32;            // tokens per tile
+  static constexpr int CPR = RB / 16;                      // 16-byte chunks per row
+  static constexpr int KTILE = T * RB;
+  static constexpr int STAGE = 2 * KTILE;                  // K then V: 4, 8 or 16 KB
+  static constexpr int NW = STAGE > 8192 ? 4 : 8;          // warps
+  static constexpr int NST = STAGE <= 4096 ? 6 : 3;        // stages of a warp's ring: 192 KB of shared memory in all
+  static constexpr int SMEM = NW * NST * STAGE;
+  static constexpr int RC = 16 * MT;                       // rows of a unit
+  static constexpr int NT = NW * 32;
+};
+
+// ------------------------------------------------------------------------------------------------------- kernel
+
+// A walker's place in the tile stream.
+struct Cursor {
+  int b, group, block;  // request, head group, row block
+  Req r;
+  int t, t_end;    // tiles of the current segment
+  long long rem;   // tiles of the slice after this segment
+  bool live, whole, first;
+};
+
+template <class I, int MODE>
+__device__ __forceinline__ void open_segment(const PagedDev& p, Cursor& c, int t_off) {
+  const long long left = c.r.cnt - t_off;
+  const long long n = left < c.rem ? left : c.rem;
+  c.t = t_off;
+  c.t_end = t_off + static_cast<int>(n);
+  c.rem -= n;
+  c.whole = t_off == 0 && c.t_end == c.r.cnt;
+}
+// To the next tile; to the next unit behind the segment's last one.
+template <class I, int MODE>
+__device__ __forceinline__ void advance(const PagedDev& p, Cursor& c) {
+  if (++c.t < c.t_end) return;
+  if (MODE == 1 || c.rem <= 0) {
+    c.live = false;
+    return;
+  }
+  c.first = false;
+  if (++c.block == p.nrb) {
+    c.block = 0;
+    if (++c.group == p.groups) {
+      c.group = 0;
+      do {
+        if (++c.b >= p.batch) {
+          c.live = false;
+          return;
+        }
+        c.r = req_info<I::T>(p, c.b, 0, p.max_q);
+      } while (c.r.cnt == 0);
+    }
+  }
+  open_segment<I, MODE>(p, c, 0);
+}
+
+// MODE 0: the tile stream cut evenly over all walkers (decode, verify). MODE 1: a walker takes one (row block, head
+// group) with the tiles that block sees (prompts; blocks from the last to the first, the longest first).
+template <class I, int MODE>
+__global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_constant__ PagedDev p) {
+  constexpr int T = I::T, RB = I::RB, HD = I::HD, KV = I::KV, MT = I::MT;
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  __shared__ int find_b[MAX_WARPS];
+  __shared__ long long find_pre[MAX_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int walker = warp / p.hg;
+  const int vc = blockIdx.x * p.walkers + walker, G = gridDim.x * p.walkers;
+  const int g = lane >> 2, tq = lane & 3;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  Cursor ci;
+  ci.live = false;
+  if (MODE == 0) {
+    const long long total = plan<I::NT>(p, [&](int b) { return req_info<T>(p, b, 0, p.max_q).cnt; }, p.upr, at_cut, G,
+                                        blockIdx.x * p.walkers, p.walkers, find_b, find_pre, blockIdx.x == 0);
+    if (walker >= p.walkers || find_b[walker] < 0) return;
+    const int used = walkers_for(total, G);
+    const long long g0 = slice(total, used, vc), g1 = slice(total, used, vc + 1);
+    if (g1 <= g0) return;
+    ci.b = find_b[walker];
+    ci.r = req_info<T>(p, ci.b, 0, p.max_q);
+    const long long in = g0 - find_pre[walker] * p.upr;
+    const int unit = static_cast<int>(in / ci.r.cnt);
+    ci.group = unit / p.nrb;
+    ci.block = unit - ci.group * p.nrb;
+    ci.rem = g1 - g0;
+    ci.live = ci.first = true;
+    open_segment<I, MODE>(p, ci, static_cast<int>(in - static_cast<long long>(unit) * ci.r.cnt));
+  } else {
+    auto blocks = [&](int b) {
+      int q0;
+      const int ql = new_tokens(p, b, q0);
+      return ql > 0 ? static_cast<int>((static_cast<long long>(min(ql, p.max_q)) * p.gqa + I::RC - 1) / I::RC) : 0;
+    };
+    const long long total = plan<I::NT>(p, blocks, 1, at_index, G, blockIdx.x * p.walkers, p.walkers, find_b, find_pre, false);
+    if (walker >= p.walkers || find_b[walker] < 0 || vc >= total) return;
+    ci.b = find_b[walker];
+    ci.block = blocks(ci.b) - 1 - static_cast<int>(vc - find_pre[walker]);
+    const int t0 = ci.block * I::RC / p.gqa, t1 = (ci.block * I::RC + I::RC - 1) / p.gqa;
+    ci.r = req_info<T>(p, ci.b, t0, t1 - t0 + 1);
+    ci.group = blockIdx.y;
+    ci.rem = ci.r.cnt;
+    ci.live = ci.r.cnt > 0;
+    open_segment<I, MODE>(p, ci, 0);
+  }
+
+  const int hl = warp - walker * p.hg;
+  const uint32_t ring = smem_u32(smem_raw) + warp * (I::NST * I::STAGE);
+
+  // Page of this lane's token of the tile the cursor stands on; -1 where no row sees the token (its page-table entry
+  // may be a released page's, or padding) or the page does not exist: such rows are filled with zeros.
+  auto fetch_pages = [&](const Cursor& c) -> int {
+    if (!c.live || lane >= T) return -1;
+    const int n = (c.t < c.r.ns ? c.t : c.r.tlo + c.t - c.r.ns) * T + lane;
+    if (n >= c.r.kend || (n < c.r.lower && n >= p.sinks)) return -1;
+    const int page = p.pt[c.b * p.pt_s0 + (n >> p.page_shift) * p.pt_s1];
+    if (page < 0 || page >= p.num_pages) {
+      atomicExch(p.status, GA_ST_BAD_PAGE);
+      return -1;
+    }
+    return page;
+  };
+  auto issue = [&](const Cursor& c, int pages, int stage) {
+    if (c.live) {
+      const int h = c.group * p.hg + hl;
+      const int n0 = (c.t < c.r.ns ? c.t : c.r.tlo + c.t - c.r.ns) * T;
+      const uint32_t dst = ring + stage * I::STAGE;
+      constexpr int RPI = 32 / I::CPR;  // rows per instruction
+      const int chunk = lane % I::CPR;
+      const bool head_real = h < p.kvh;
+      const uint8_t* kb = p.k + (head_real ? h * p.k_s2 : 0) + chunk * 16;
+      const uint8_t* vb = p.v + (head_real ? h * p.v_s2 : 0) + chunk * 16;
+#pragma unroll
+      for (int it = 0; it < T / RPI; ++it) {
+        const int row = it * RPI + lane / I::CPR;
+        const int page = __shfl_sync(0xffffffffu, pages, row);
+        const bool real = page >= 0 && head_real;
+        const long long pg = real ? page : 0, tk = real ? ((n0 + row) & p.page_mask) : 0;
+        const uint32_t d = dst + swz<RB>(row, chunk);
+        cp_async_16_or_zero(d, kb + pg * p.k_s0 + tk * p.k_s1, real);
+        cp_async_16_or_zero(d + I::KTILE, vb + pg * p.v_s0 + tk * p.v_s1, real);
+      }
+    }
+    cp_async_commit();
+  };
+
+  Cursor cc = ci;  // the tile to consume; ci: the tile to load
+  int pages = fetch_pages(ci);
+#pragma unroll
+  for (int i = 0; i < I::NST - 1; ++i) {
+    issue(ci, pages, i);
+    if (ci.live) advance<I, MODE>(p, ci);
+    pages = fetch_pages(ci);
+  }
+
+  uint32_t qf[MT][HD / 16][4];
+  float o[MT][HD / 8][4];
+  float m[MT][2], l[MT][2];
+  int pos[MT][2];
+  float sl2 = 0.f;
+  int stage = 0, pos_first = 0, pos_last = 0;
+  bool fresh = true;
+  // A prompt's row block without a single visible key still has rows to write (zeros).
+  const bool blank = MODE == 1 && !cc.live;
+  while (cc.live || (blank && fresh)) {
+    const int block = cc.block;
+    const int h = cc.group * p.hg + hl;
+    const int rows = cc.r.nq * p.gqa - block * I::RC;  // rows of this block, may exceed RC
+    if (fresh) {
+      fresh = false;
+      sl2 = p.scale_log2 * (p.kd && h < p.kvh ? p.kd[cc.b * p.kd_s0 + h * p.kd_s1] : 1.f);
+      pos_first = cc.r.pos0 + block * I::RC / p.gqa;
+      pos_last = cc.r.pos0 + (block * I::RC + min(rows, I::RC) - 1) / p.gqa;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int row = mt * 16 + hf * 8 + g;
+          const bool real = row < rows && h < p.kvh;
+          const int rr = block * I::RC + row;
+          const int tok = rr / p.gqa;
+          pos[mt][hf] = real ? cc.r.pos0 + tok : -1;
+          m[mt][hf] = -INFINITY;
+          l[mt][hf] = 0.f;
+          const long long qo = real ? (cc.r.q0 + tok) * p.q_s0 + (h * p.gqa + rr - tok * p.gqa) * p.q_s1 : 0;
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks) {
+            uint32_t a0 = 0, a1 = 0;
+            if (real) {
+              if (KV != KV_E4M3) {
+                const uint8_t* s = p.q + (qo + ks * 16 + tq * 2) * 2;
+                a0 = *reinterpret_cast<const uint32_t*>(s);
+                a1 = *reinterpret_cast<const uint32_t*>(s + 16);
+              } else {
+                // the contraction's dims are taken in the order in which a thread finds them in an e4m3 K row: its
+                // four values 16 ks + 4 tq .. + 3
+                uint32_t raw;
+                if (p.q_kind == Q_BF16_TO_E4M3) {
+                  const uint2 w = *reinterpret_cast<const uint2*>(p.q + (qo + ks * 16 + tq * 4) * 2);
+                  raw = pack_e4m3x4(bf16_bits_to_f32(w.x & 0xffffu), bf16_bits_to_f32(w.x >> 16),
+                                    bf16_bits_to_f32(w.y & 0xffffu), bf16_bits_to_f32(w.y >> 16));
+                } else {
+                  raw = *reinterpret_cast<const uint32_t*>(p.q + qo + ks * 16 + tq * 4);
+                }
+                a0 = e4m3x2_to_f16x2(raw & 0xffffu);
+                a1 = e4m3x2_to_f16x2(raw >> 16);
+              }
+            }
+            qf[mt][ks][hf] = a0;
+            qf[mt][ks][2 + hf] = a1;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+      }
+    }
+    bool last = blank;
+    if (cc.live) {
+      cp_async_wait<I::NST - 2>();
+      __syncwarp();  // the tile of every lane is there, and every lane is done with the stage that is refilled next
+      {
+        int st = stage + I::NST - 1;
+        if (st >= I::NST) st -= I::NST;
+        issue(ci, pages, st);
+        if (ci.live) advance<I, MODE>(p, ci);
+        pages = fetch_pages(ci);
+      }
+      const uint32_t ka = ring + stage * I::STAGE, va = ka + I::KTILE;
+      const int n0 = (cc.t < cc.r.ns ? cc.t : cc.r.tlo + cc.t - cc.r.ns) * T;
+      float s[MT][T / 8][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int j = 0; j < T / 8; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
+      if (KV != KV_E4M3) {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ks += 2) {
+#pragma unroll
+          for (int j = 0; j < T / 8; ++j) {
+            uint32_t r0, r1, r2, r3;
+            ldsm_x4(ka + swz<RB>(j * 8 + (lane & 7), ks * 2 + (lane >> 3)), r0, r1, r2, r3);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) mma16<KV>(s[mt][j], qf[mt][ks], r0, r1);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) mma16<KV>(s[mt][j], qf[mt][ks + 1], r2, r3);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ks += 4) {
+#pragma unroll
+          for (int j = 0; j < T / 8; ++j) {
+            uint32_t r[4];
+            ldsm_x4(ka + swz<RB>(j * 8 + (lane & 7), ks + (lane >> 3)), r[0], r[1], r[2], r[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t b0 = e4m3x2_to_f16x2(r[i] & 0xffffu), b1 = e4m3x2_to_f16x2(r[i] >> 16);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) mma16<KV>(s[mt][j], qf[mt][ks + i], b0, b1);
+            }
+          }
+        }
+      }
+      const bool open = n0 + T - 1 <= pos_first && (p.window < 0 || n0 >= pos_last - p.window || n0 + T <= p.sinks);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < T / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float x = s[mt][j][e] * sl2;
+            if (!open) {
+              const int key = n0 + j * 8 + tq * 2 + (e & 1), at = pos[mt][e >> 1];
+              if (key > at || (p.window >= 0 && key < at - p.window && key >= p.sinks)) x = -INFINITY;
+            }
+            s[mt][j][e] = x;
+            mx[e >> 1] = fmaxf(mx[e >> 1], x);
+          }
+        float mu[2];
+        bool moved = false;
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+          mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+          moved |= mx[hf] > m[mt][hf];
+        }
+        if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            const float nm = fmaxf(m[mt][hf], mx[hf]);
+            const float f = nm == -INFINITY ? 1.f : ex2(m[mt][hf] - nm);
+            m[mt][hf] = nm;
+            l[mt][hf] *= f;
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j) {
+              o[mt][j][hf * 2] *= f;
+              o[mt][j][hf * 2 + 1] *= f;
+            }
+          }
+        }
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) mu[hf] = m[mt][hf] == -INFINITY ? 0.f : m[mt][hf];
+#pragma unroll
+        for (int j = 0; j < T / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = ex2(s[mt][j][e] - mu[e >> 1]);
+            s[mt][j][e] = x;
+            l[mt][e >> 1] += x;
+          }
+      }
+#pragma unroll
+      for (int ts = 0; ts < T / 16; ++ts) {
+        uint32_t a[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          a[mt][0] = pack16<KV>(s[mt][2 * ts][0], s[mt][2 * ts][1]);
+          a[mt][1] = pack16<KV>(s[mt][2 * ts][2], s[mt][2 * ts][3]);
+          a[mt][2] = pack16<KV>(s[mt][2 * ts + 1][0], s[mt][2 * ts + 1][1]);
+          a[mt][3] = pack16<KV>(s[mt][2 * ts + 1][2], s[mt][2 * ts + 1][3]);
+        }
+        const int row = ts * 16 + (lane & 15), cx = lane >> 4;
+        if (KV != KV_E4M3) {
+#pragma unroll
+          for (int d = 0; d < HD / 16; ++d) {
+            uint32_t r0, r1, r2, r3;
+            ldsm_x4_trans(va + swz<RB>(row, d * 2 + cx), r0, r1, r2, r3);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16<KV>(o[mt][2 * d], a[mt], r0, r1);
+              mma16<KV>(o[mt][2 * d + 1], a[mt], r2, r3);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < HD / 32; ++d) {
+            uint32_t r[4];
+            ldsm_x4_trans(va + swz<RB>(row, d * 2 + cx), r[0], r[1], r[2], r[3]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {  // chunk 2 d + i: its even dims, its odd dims
+              const uint32_t e0 = e4m3x2_to_f16x2(prmt(r[2 * i], 0, 0x4420)), e1 = e4m3x2_to_f16x2(prmt(r[2 * i + 1], 0, 0x4420));
+              const uint32_t o0 = e4m3x2_to_f16x2(prmt(r[2 * i], 0, 0x4431)), o1 = e4m3x2_to_f16x2(prmt(r[2 * i + 1], 0, 0x4431));
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                mma16<KV>(o[mt][4 * d + 2 * i], a[mt], e0, e1);
+                mma16<KV>(o[mt][4 * d + 2 * i + 1], a[mt], o0, o1);
+              }
+            }
+          }
+        }
+      }
+      if (++stage == I::NST) stage = 0;
+      last = cc.t + 1 >= cc.t_end;
+    }
+    if (last) {
+      const float vds = p.vd && h < p.kvh ? p.vd[cc.b * p.vd_s0 + h * p.vd_s1] : 1.f;
+      const int slot = 2 * (blockIdx.x * p.walkers + walker) + (cc.first ? 0 : 1);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          float sum = l[mt][hf];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          const int row = mt * 16 + hf * 8 + g;
+          if (row >= rows || h >= p.kvh) continue;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          const float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + lg2(sum);
+          if (MODE == 0 && !cc.whole) {
+            const long long wr = (static_cast<long long>(slot) * p.hg + hl) * I::RC + row;
+            float* w = p.ws_o + wr * HD;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
+              if (KV != KV_E4M3) {
+                *reinterpret_cast<float2*>(w + j * 8 + tq * 2) = make_float2(o[mt][j][hf * 2] * inv, o[mt][j][hf * 2 + 1] * inv);
+              } else {
+                *reinterpret_cast<float4*>(w + j * 8 + tq * 4) =
+                    make_float4(o[mt][j][hf * 2] * inv, o[mt][j + 1][hf * 2] * inv, o[mt][j][hf * 2 + 1] * inv, o[mt][j + 1][hf * 2 + 1] * inv);
+              }
+            }
+            if (tq == 0) p.ws_lse[wr] = lse2;
+          } else {
+            const int rr = block * I::RC + row, tok = rr / p.gqa;
+            const int qrow = cc.r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
+            uint8_t* dst = static_cast<uint8_t*>(p.out) + (qrow * p.o_s0 + qh * p.o_s1) * 2;
+            const float f = sum == 0.f ? 0.f : inv * vds;
+#pragma unroll
+            for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
+              if (KV != KV_E4M3) {
+                *reinterpret_cast<uint32_t*>(dst + (j * 8 + tq * 2) * 2) = pack16<KV>(o[mt][j][hf * 2] * f, o[mt][j][hf * 2 + 1] * f);
+              } else {
+                uint2 w;
+                w.x = pack16<KV_BF16>(o[mt][j][hf * 2] * f, o[mt][j + 1][hf * 2] * f);
+                w.y = pack16<KV_BF16>(o[mt][j][hf * 2 + 1] * f, o[mt][j + 1][hf * 2 + 1] * f);
+                *reinterpret_cast<uint2*>(dst + (j * 8 + tq * 4) * 2) = w;
+              }
+            }
+            if (tq == 0 && p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
+          }
+        }
+      }
+      fresh = true;
+      if (blank) break;
+    }
+    advance<I, MODE>(p, cc);
+  }
+  cp_async_wait<0>();
+}
+
+// Folds the pieces of every unit that the main kernel cut, in slice order, and writes the rows of requests without
+// visible keys. grid = (batch * upr, heads of a group, row shares); 4 warps. A row's pieces are spread over the warps
+// when there are many of them (one long sequence), the rows are when there are few.
+template <class I>
+__global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant__ PagedDev p, int G) {
+  constexpr int HD = I::HD, VEC = HD / 32, UNR = 8;
+  const int b = blockIdx.x / p.upr, j = blockIdx.x - b * p.upr;
+  const int group = j / p.nrb, block = j - group * p.nrb;
+  const int h = group * p.hg + blockIdx.y;
+  const Req r = req_info<I::T>(p, b, 0, p.max_q);
+  const int rows = min(r.nq * p.gqa - block * I::RC, I::RC);
+  const float vds = p.vd && h < p.kvh ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
+  grid_dep_wait();
+  grid_dep_launch();
+  if (rows <= 0 || h >= p.kvh) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto store = [&](int row, const float (&v)[VEC], float f, float lse2) {
+    const int rr = block * I::RC + row, tok = rr / p.gqa;
+    const int qrow = r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
+    uint8_t* dst = static_cast<uint8_t*>(p.out) + (qrow * p.o_s0 + qh * p.o_s1 + lane * VEC) * 2;
+    constexpr int OKV = I::KV == KV_E4M3 ? KV_BF16 : I::KV;
+#pragma unroll
+    for (int i = 0; i < VEC; i += 2) *reinterpret_cast<uint32_t*>(dst + i * 2) = pack16<OKV>(v[i] * f, v[i + 1] * f);
+    if (lane == 0 && p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
+  };
+  const int share = gridDim.z;
+  if (r.cnt == 0) {
+    const float zero[VEC] = {};
+    for (int row = blockIdx.z * 4 + warp; row < rows; row += 4 * share) store(row, zero, 0.f, -INFINITY);
+    return;
+  }
+  const long long total = static_cast<long long>(p.prefix[p.batch]) * p.upr;
+  G = walkers_for(total, G);
+  const long long u0 = static_cast<long long>(p.prefix[b]) * p.upr + static_cast<long long>(j) * r.cnt, u1 = u0 + r.cnt;
+  auto owner = [&](long long x) {  // the walker whose slice holds tile x
+    long long c = ((x + 1) * G - 1) / total;
+    while (c > 0 && slice(total, G, static_cast<int>(c)) > x) --c;
+    while (c < G - 1 && slice(total, G, static_cast<int>(c) + 1) <= x) ++c;
+    return static_cast<int>(c);
+  };
+  const int c0 = owner(u0), c1 = owner(u1 - 1);
+  if (c0 == c1) return;
+  const int n = c1 - c0 + 1;  // every walker between them holds a piece too
+  const int e0 = u0 <= slice(total, G, c0) ? 0 : 1;
+  auto piece = [&](int i) {  // workspace row 0 of the unit's piece i
+    return (static_cast<long long>(2 * (c0 + i) + (i == 0 ? e0 : 0)) * p.hg + blockIdx.y) * I::RC;
+  };
+  __shared__ float red_o[4][HD], red_m[4], red_l[4];
+  const bool many = n > UNR;
+  for (int row = many ? blockIdx.z : blockIdx.z * 4 + warp; row < rows; row += many ? share : 4 * share) {
+    float mx = -INFINITY, den = 0.f, acc[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) acc[i] = 0.f;
+    const int step = many ? 4 : 1;
+#pragma unroll 1
+    for (int i0 = many ? warp : 0; i0 < n; i0 += step * UNR) {
+      float w[UNR], v[UNR][VEC];
+      float mc = mx;
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        const int i = i0 + u * step;
+        w[u] = -INFINITY;
+        if (i < n) {
+          const long long at = piece(i);
+          w[u] = __ldcg(p.ws_lse + at + row);
+#pragma unroll
+          for (int x = 0; x < VEC; x += 2) {
+            const float2 t = __ldcg(reinterpret_cast<const float2*>(p.ws_o + (at + row) * HD + lane * VEC + x));
+            v[u][x] = t.x;
+            v[u][x + 1] = t.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) mc = fmaxf(mc, w[u]);
+      if (mc != mx) {
+        const float f = ex2(mx - mc);
+        den *= f;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) acc[x] *= f;
+        mx = mc;
+      }
+#pragma unroll
+      for (int u = 0; u < UNR; ++u) {
+        if (w[u] == -INFINITY) continue;
+        const float f = ex2(w[u] - mx);
+        den += f;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) acc[x] += f * v[u][x];
+      }
+    }
+    if (many) {
+#pragma unroll
+      for (int x = 0; x < VEC; ++x) red_o[warp][lane * VEC + x] = acc[x];
+      if (lane == 0) red_m[warp] = mx, red_l[warp] = den;
+      __syncthreads();
+      if (warp == 0) {
+        const float top = fmaxf(fmaxf(red_m[0], red_m[1]), fmaxf(red_m[2], red_m[3]));
+        den = 0.f;
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) acc[x] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = red_m[w] == -INFINITY && red_l[w] == 0.f ? 0.f : ex2(red_m[w] - top);
+          den += f * red_l[w];
+#pragma unroll
+          for (int x = 0; x < VEC; ++x) acc[x] += f * red_o[w][lane * VEC + x];
+        }
+        store(row, acc, den == 0.f ? 0.f : vds / den, den == 0.f ? -INFINITY : top + lg2(den));
+      }
+      __syncthreads();
+    } else {
+      store(row, acc, den == 0.f ? 0.f : vds / den, den == 0.f ? -INFINITY : mx + lg2(den));
+    }
+  }
+}
+
+}  // namespace paged
+}  // namespace ga

@@ -1,0 +1,535 @@
+// Upkeep of the pages of a paged cache: copying pages inside every layer's pool, sharing a request's pages with its
+// forks, releasing, allocating and closing gaps, all on the device (no host round trip, capturable).
+//
+// Books: refs[page] = number of page-table entries that hold the page; a page is free while its count is 0. A row of
+// the page table holds ceil(len / page_size) entries; -1 stands for a released page. New pages are the lowest free
+// ones, handed out in the order of the call's rows, so the outcome does not depend on scheduling (counts are changed
+// with integer atomics, whose order does not matter).
+//
+// What bounds it: the bytes of the copied tokens, read once and written once. The decisions (a few integers per row,
+// one count per page) are made by small kernels in front; a copy kernel then moves 16 KB pieces of pages, all layers
+// of all pairs in one launch, with enough CTAs per SM that a piece's chain of descriptor reads hides behind the others'.
+#pragma once
+
+#include "ga_common.cuh"
+
+namespace ga {
+namespace pages {
+
+enum : int { ST_BAD_PAGE = GA_ST_BAD_PAGE, ST_LEN_RANGE = GA_ST_LEN_RANGE, ST_BAD_INDEX = 7, ST_NO_PAGES = 8, ST_REFS = 9, ST_CLASH = 10 };
+
+constexpr int CHUNK = 16384;      // bytes of a copy item
+constexpr int COPY_THREADS = 256;
+constexpr int PLAN_THREADS = 1024;
+constexpr int SPAN = 16384;       // pages that a CTA looks through at a time (16 per thread)
+
+struct PoolDev {
+  const unsigned long long* base;  // [tensors] address of page 0
+  const long long* stride;         // [tensors] bytes between pages
+  const int* tok_bytes;            // [tensors] bytes of a token
+  const int* chunk_tensor;         // [chunks] tensor of a page's chunk
+  const int* chunk_first;          // [tensors] first chunk of a tensor
+  int tensors, chunks;
+  int num_pages, page_shift, page_size;
+  int* table;
+  long long t_s0, t_s1;
+  int rows, cols;
+  int* lens;
+  int* refs;
+  int* status;
+};
+
+__device__ __forceinline__ int pages_of(const PoolDev& p, int len) { return len <= 0 ? 0 : (len - 1) / p.page_size + 1; }
+__device__ __forceinline__ void flag(const PoolDev& p, int what) { atomicExch(p.status, what); }
+
+// Exclusive prefix of `v` over the CTA's threads, and the sum. `tmp`: 33 ints of shared memory.
+template <int NT>
+__device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int incl = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 31) tmp[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int w = lane < NT / 32 ? tmp[lane] : 0, wi = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, wi, d);
+      if (lane >= d) wi += o;
+    }
+    if (lane < NT / 32) tmp[lane] = wi - w;
+    if (lane == NT / 32 - 1) tmp[32] = wi;
+  }
+  __syncthreads();
+  const int before = tmp[warp] + incl - v;
+  total = tmp[32];
+  __syncthreads();
+  return before;
+}
+
+// ------------------------------------------------------------------------------------------------------ copying
+
+// One 16 KB piece (or what `tokens` leaves of it) of one tensor's page.
+__device__ __forceinline__ void copy_piece(const PoolDev& p, int c, int src, int dst, int tokens) {
+  const int t = p.chunk_tensor[c];
+  const long long stride = p.stride[t];
+  const int off = (c - p.chunk_first[t]) * CHUNK;
+  int n = tokens * p.tok_bytes[t] - off;
+  if (n <= 0) return;
+  if (n > CHUNK) n = CHUNK;
+  const uint8_t* base = reinterpret_cast<const uint8_t*>(p.base[t]);
+  const uint4* s = reinterpret_cast<const uint4*>(base + src * stride + off);
+  uint4* d = reinterpret_cast<uint4*>(const_cast<uint8_t*>(base) + dst * stride + off);
+  const int vecs = n >> 4;
+  constexpr int U = CHUNK / 16 / COPY_THREADS;
+  uint4 v[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * COPY_THREADS + threadIdx.x;
+    if (i < vecs) v[u] = __ldcs(s + i);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = u * COPY_THREADS + threadIdx.x;
+    if (i < vecs) __stcs(d + i, v[u]);
+  }
+}
+
+__device__ __forceinline__ long long index_at(const void* p, int is64, int i) {
+  return is64 ? static_cast<const long long*>(p)[i] : static_cast<const int*>(p)[i];
+}
+
+// Which pairs of a copy call are carried out: list[i] = (src, dst), src -1: not. Of several pairs with one destination
+// the last counts; a pair whose source another pair writes is not carried out (its content would depend on the order)
+// and flagged, and so is one that names no page. `mark`: num_pages ints.
+__global__ void __launch_bounds__(PLAN_THREADS) copy_plan_kernel(const __grid_constant__ PoolDev p, const void* src,
+                                                                 const void* dst, int is64, int n, int* mark, int2* list) {
+  grid_dep_wait();
+  grid_dep_launch();
+  auto get = [&](int i, int& s, int& d) {
+    const long long a = index_at(src, is64, i), b = index_at(dst, is64, i);
+    const bool ok = a >= 0 && a < p.num_pages && b >= 0 && b < p.num_pages;
+    s = ok ? static_cast<int>(a) : -1;
+    d = ok ? static_cast<int>(b) : -1;
+    return ok;
+  };
+  int s, d;
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
+    if (get(i, s, d)) mark[s] = mark[d] = -1;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS)
+    if (get(i, s, d) && s != d) atomicMax(mark + d, i);
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    const bool ok = get(i, s, d);
+    int use = ok && s != d && __ldcg(mark + d) == i ? s : -1;
+    if (!ok) flag(p, ST_BAD_INDEX);
+    if (use >= 0 && __ldcg(mark + s) >= 0) {
+      flag(p, ST_CLASH);
+      use = -1;
+    }
+    list[i] = make_int2(use, d);
+  }
+}
+
+__global__ void __launch_bounds__(COPY_THREADS) copy_kernel(const __grid_constant__ PoolDev p, const int2* list, int n) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const long long items = static_cast<long long>(n) * p.chunks;
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    const int i = static_cast<int>(it / p.chunks), c = static_cast<int>(it - static_cast<long long>(i) * p.chunks);
+    const int2 pair = list[i];
+    if (pair.x >= 0) copy_piece(p, c, pair.x, pair.y, p.page_size);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- releasing
+
+// One CTA per entry of `rows`. Releases the row's entries [first, last) that hold a page: all of them and the row's
+// length (evict = 0), or those whose keys lie behind the first `sinks` and before the window of the next query at
+// position len (evict = 1).
+__global__ void __launch_bounds__(256) release_kernel(const __grid_constant__ PoolDev p, const void* rows, int is64, int n,
+                                                      int evict, int window, int sinks) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int i = blockIdx.x;
+  const long long row64 = index_at(rows, is64, i);
+  if (row64 < 0 || row64 >= p.rows) {
+    if (threadIdx.x == 0) flag(p, ST_BAD_INDEX);
+    return;
+  }
+  bool again = false;  // a row named twice is released once
+  for (int k = threadIdx.x; k < i; k += blockDim.x) again |= index_at(rows, is64, k) == row64;
+  if (__syncthreads_or(again)) return;
+  const int row = static_cast<int>(row64);
+  const int len = p.lens[row];
+  int held = pages_of(p, len);
+  if (held > p.cols) {
+    held = p.cols;
+    if (threadIdx.x == 0) flag(p, ST_LEN_RANGE);
+  }
+  int first = 0, last = held;
+  if (evict) {
+    first = (sinks >> p.page_shift) + ((sinks & (p.page_size - 1)) != 0);
+    const int gone = len > window ? (len - window) >> p.page_shift : 0;
+    last = gone < held ? gone : held;
+  }
+  int* t = p.table + row * p.t_s0;
+  for (int j = first + threadIdx.x; j < last; j += blockDim.x) {
+    const int page = t[j * p.t_s1];
+    if (page < 0) continue;
+    t[j * p.t_s1] = -1;
+    if (page >= p.num_pages) {
+      flag(p, ST_BAD_PAGE);
+    } else if (atomicSub(p.refs + page, 1) <= 0) {
+      atomicAdd(p.refs + page, 1);
+      flag(p, ST_REFS);
+    }
+  }
+  __syncthreads();
+  if (!evict && threadIdx.x == 0) p.lens[row] = 0;
+}
+
+// --------------------------------------------------------------------------------------------------- allocating
+
+// Hands the lowest free pages to ranks 0, 1, ... < want: give(rank, page) by the thread that found it. Returns how
+// many there were. One CTA of PLAN_THREADS; stops as soon as enough are found.
+template <typename Give>
+__device__ __forceinline__ int hand_out(const PoolDev& p, int want, int* tmp, Give give) {
+  int found = 0;
+  for (int p0 = 0; p0 < p.num_pages && found < want; p0 += SPAN) {
+    const int at = p0 + threadIdx.x * 16;
+    unsigned free_bits = 0;
+    if (at + 16 <= p.num_pages && (reinterpret_cast<uintptr_t>(p.refs + at) & 15) == 0) {
+      int4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = __ldcg(reinterpret_cast<const int4*>(p.refs + at) + u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        free_bits |= ((v[u].x == 0) | (v[u].y == 0) << 1 | (v[u].z == 0) << 2 | (v[u].w == 0) << 3) << (4 * u);
+    } else {
+      for (int u = 0; u < 16; ++u)
+        if (at + u < p.num_pages && __ldcg(p.refs + at + u) == 0) free_bits |= 1u << u;
+    }
+    int total;
+    int rank = found + block_scan<PLAN_THREADS>(__popc(free_bits), tmp, total);
+    while (free_bits && rank < want) {
+      const int u = __ffs(free_bits) - 1;
+      free_bits &= free_bits - 1;
+      give(rank++, at + u);
+    }
+    found += total;
+  }
+  __syncthreads();
+  return found < want ? found : want;
+}
+// First i in [0, n) with incl[i] > rank (incl: non-decreasing inclusive prefix of the needs).
+__device__ __forceinline__ int holder(const int* incl, int n, int rank) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (incl[mid] > rank) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
+}
+// Only the first entry of a call that names a row counts: mark[row] = lowest i. `mark`: rows ints.
+template <typename RowOf>
+__device__ __forceinline__ void mark_first(int n, int* mark, RowOf row_of) {
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    const int r = row_of(i);
+    if (r >= 0) mark[r] = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    const int r = row_of(i);
+    if (r >= 0) atomicMin(mark + r, i);
+  }
+  __syncthreads();
+}
+
+// Rows grow to the given lengths with the lowest free pages, in the call's order. From the first row on whose pages
+// are not there, rows that need some are left as they were (flagged). One CTA; dynamic shared memory: n ints.
+__global__ void __launch_bounds__(PLAN_THREADS) grow_kernel(const __grid_constant__ PoolDev p, const void* rows,
+                                                            const void* to, int is64, int to64, int n, int* mark) {
+  extern __shared__ int incl[];
+  __shared__ int tmp[33];
+  grid_dep_wait();
+  grid_dep_launch();
+  auto row_of = [&](int i) {
+    const long long r = index_at(rows, is64, i);
+    return r >= 0 && r < p.rows ? static_cast<int>(r) : -1;
+  };
+  mark_first(n, mark, row_of);
+  int sum = 0;
+  for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+    const int i = i0 + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      const int r = row_of(i);
+      if (r < 0) {
+        flag(p, ST_BAD_INDEX);
+      } else if (__ldcg(mark + r) != i) {
+        flag(p, ST_CLASH);
+      } else {
+        const long long want = index_at(to, to64, i);
+        if (want > (static_cast<long long>(p.cols) << p.page_shift)) flag(p, ST_LEN_RANGE);
+        else need = max(0, pages_of(p, static_cast<int>(want < 0 ? 0 : want)) - pages_of(p, p.lens[r]));
+      }
+    }
+    int total;
+    const int before = block_scan<PLAN_THREADS>(need, tmp, total);
+    if (i < n) incl[i] = sum + before + need;
+    sum += total;
+  }
+  __syncthreads();
+  const int got = hand_out(p, sum, tmp, [&](int rank, int page) {
+    const int i = holder(incl, n, rank);
+    const int r = row_of(i), j = pages_of(p, p.lens[r]) + rank - (i ? incl[i - 1] : 0);
+    p.table[r * p.t_s0 + j * p.t_s1] = page;
+    p.refs[page] = 1;
+  });
+  __syncthreads();
+  if (got < sum) {  // the row that ran out gives back what it got
+    const int i = holder(incl, n, got);
+    const int r = row_of(i), j0 = pages_of(p, p.lens[r]);
+    for (int k = threadIdx.x; k < got - (i ? incl[i - 1] : 0); k += PLAN_THREADS) {
+      int* e = p.table + r * p.t_s0 + (j0 + k) * p.t_s1;
+      p.refs[*e] = 0;
+      *e = -1;
+    }
+    if (threadIdx.x == 0) flag(p, ST_NO_PAGES);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    const int r = row_of(i);
+    if (r < 0 || __ldcg(mark + r) != i) continue;
+    const long long want = index_at(to, to64, i);
+    const bool fits = incl[i] == (i ? incl[i - 1] : 0) || incl[i] <= got;
+    if (fits && want > p.lens[r] && want <= (static_cast<long long>(p.cols) << p.page_shift)) p.lens[r] = static_cast<int>(want);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------ forking
+
+// list[i] = (source of the partial last page or -1, its copy, tokens of the parent, 1 if the pair is carried out). A
+// child is an empty row that the call names once; a parent is taken as it was before the call. One CTA; dynamic shared
+// memory: n ints.
+__global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const __grid_constant__ PoolDev p, const void* parents,
+                                                                 const void* children, int is64, int n, int* mark, int4* list) {
+  extern __shared__ int incl[];
+  __shared__ int tmp[33];
+  grid_dep_wait();
+  grid_dep_launch();
+  auto child_of = [&](int i) {
+    const long long r = index_at(children, is64, i);
+    return r >= 0 && r < p.rows ? static_cast<int>(r) : -1;
+  };
+  mark_first(n, mark, child_of);
+  int sum = 0;
+  for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+    const int i = i0 + threadIdx.x;
+    int need = 0;
+    if (i < n) {
+      int4 e = make_int4(-1, -1, 0, 0);
+      const int c = child_of(i);
+      const long long a = index_at(parents, is64, i);
+      if (c < 0 || a < 0 || a >= p.rows) {
+        flag(p, ST_BAD_INDEX);
+      } else if (__ldcg(mark + c) != i || p.lens[c] != 0) {
+        flag(p, ST_CLASH);
+      } else {
+        const int len = p.lens[a], tail = len & (p.page_size - 1);
+        if (pages_of(p, len) > p.cols) {
+          flag(p, ST_LEN_RANGE);
+        } else if (len > 0) {
+          e = make_int4(-1, -1, len, 1);
+          if (tail) {
+            const int src = p.table[a * p.t_s0 + (len >> p.page_shift) * p.t_s1];
+            if (src < 0 || src >= p.num_pages) {
+              flag(p, ST_BAD_PAGE);
+              e.w = 0;
+            } else {
+              e.x = src;
+              need = 1;
+            }
+          }
+        }
+      }
+      list[i] = e;
+    }
+    int total;
+    const int before = block_scan<PLAN_THREADS>(need, tmp, total);
+    if (i < n) incl[i] = sum + before + need;
+    sum += total;
+  }
+  __syncthreads();
+  const int got = hand_out(p, sum, tmp, [&](int rank, int page) {
+    const int i = holder(incl, n, rank);
+    p.table[child_of(i) * p.t_s0 + (list[i].z >> p.page_shift) * p.t_s1] = page;
+    p.refs[page] = 1;
+    list[i].y = page;
+  });
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
+    int4 e = list[i];
+    if (e.x >= 0 && e.y < 0) {  // no page left for its copy
+      flag(p, ST_NO_PAGES);
+      e = make_int4(-1, -1, 0, 0);
+      list[i] = e;
+    }
+    if (e.w) p.lens[child_of(i)] = e.z;
+  }
+}
+
+// Items 0 .. n - 1: the pair's full pages are shared; the rest: pieces of the partial pages.
+__global__ void __launch_bounds__(COPY_THREADS) fork_apply_kernel(const __grid_constant__ PoolDev p, const void* parents,
+                                                                  const void* children, int is64, int n, const int4* list) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const long long items = n + static_cast<long long>(n) * p.chunks;
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    if (it < n) {
+      const int i = static_cast<int>(it);
+      const int4 e = list[i];
+      if (!e.w) continue;
+      const int* from = p.table + index_at(parents, is64, i) * p.t_s0;
+      int* to = p.table + index_at(children, is64, i) * p.t_s0;
+      for (int j = threadIdx.x; j < e.z >> p.page_shift; j += COPY_THREADS) {
+        const int page = from[j * p.t_s1];
+        to[j * p.t_s1] = page;
+        if (page >= p.num_pages) flag(p, ST_BAD_PAGE);
+        else if (page >= 0) atomicAdd(p.refs + page, 1);
+      }
+    } else {
+      const int i = static_cast<int>((it - n) / p.chunks), c = static_cast<int>((it - n) - static_cast<long long>(i) * p.chunks);
+      const int4 e = list[i];
+      if (e.x >= 0) copy_piece(p, c, e.x, e.y, e.z & (p.page_size - 1));
+    }
+  }
+}
+
+// --------------------------------------------------------------------------------------------------- compacting
+
+// Live pages of each span of SPAN pages.
+__device__ __forceinline__ unsigned live_bits(const PoolDev& p, int at) {
+  unsigned bits = 0;
+  if (at + 16 <= p.num_pages && (reinterpret_cast<uintptr_t>(p.refs + at) & 15) == 0) {
+    int4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = __ldcg(reinterpret_cast<const int4*>(p.refs + at) + u);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      bits |= ((v[u].x > 0) | (v[u].y > 0) << 1 | (v[u].z > 0) << 2 | (v[u].w > 0) << 3) << (4 * u);
+  } else {
+    for (int u = 0; u < 16; ++u)
+      if (at + u < p.num_pages && __ldcg(p.refs + at + u) > 0) bits |= 1u << u;
+  }
+  return bits;
+}
+__global__ void __launch_bounds__(PLAN_THREADS) compact_count_kernel(const __grid_constant__ PoolDev p, int* counts) {
+  __shared__ int tmp[33];
+  grid_dep_wait();
+  grid_dep_launch();
+  int total;
+  block_scan<PLAN_THREADS>(__popc(live_bits(p, blockIdx.x * SPAN + threadIdx.x * 16)), tmp, total);
+  if (threadIdx.x == 0) counts[blockIdx.x] = total;
+}
+// With L live pages, the live pages at L and above move, in order, to the free ones below L. map[page] = its new id,
+// -1 for a free page, -2 - k for the k-th page that moves (to gaps[k]; the apply kernel puts the id there).
+__global__ void __launch_bounds__(PLAN_THREADS) compact_rank_kernel(const __grid_constant__ PoolDev p, const int* counts,
+                                                                    int* map, int* movers, int* gaps, int* live, int* moved) {
+  __shared__ int tmp[33];
+  __shared__ int below;  // live pages before this CTA's span
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tid = threadIdx.x;
+  int mine = 0, before = 0;
+  for (int s = tid; s < static_cast<int>(gridDim.x); s += PLAN_THREADS) {
+    mine += counts[s];
+    if (s < static_cast<int>(blockIdx.x)) before += counts[s];
+  }
+  int L, B;
+  block_scan<PLAN_THREADS>(mine, tmp, L);
+  block_scan<PLAN_THREADS>(before, tmp, B);
+  if (tid == 0) below = B;
+  // live pages below L: the spans before L's and the part of L's own
+  const int ls = L / SPAN;
+  int low = 0;
+  for (int s = tid; s < ls; s += PLAN_THREADS) low += counts[s];
+  if (L % SPAN) {
+    const int at = ls * SPAN + tid * 16;
+    unsigned bits = live_bits(p, at);
+    if (at + 16 > L) bits &= at >= L ? 0u : (1u << (L - at)) - 1;
+    low += __popc(bits);
+  }
+  int low_total;
+  block_scan<PLAN_THREADS>(low, tmp, low_total);
+  if (blockIdx.x == 0 && tid == 0) {
+    *live = L;
+    *moved = L - low_total;
+  }
+  const int at = blockIdx.x * SPAN + tid * 16;
+  const unsigned bits = live_bits(p, at);
+  int total;
+  int rank = below + block_scan<PLAN_THREADS>(__popc(bits), tmp, total);  // live pages before page `at`
+  for (int u = 0; u < 16; ++u) {
+    const int id = at + u;
+    if (id >= p.num_pages) break;
+    if (bits >> u & 1) {
+      if (id >= L) {
+        movers[rank - low_total] = id;
+        map[id] = -2 - (rank - low_total);
+      } else {
+        map[id] = id;
+      }
+      ++rank;
+    } else {
+      if (id < L) gaps[id - rank] = id;
+      map[id] = -1;
+    }
+  }
+}
+// Rewrites the page table, moves the counts and copies the pages.
+__global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(const __grid_constant__ PoolDev p, int* map, const int* movers,
+                                                                     const int* gaps, const int* moved) {
+  grid_dep_wait();
+  grid_dep_launch();
+  const int n = *moved;
+  const long long items = p.rows + static_cast<long long>(n) * p.chunks;
+  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
+    if (it < p.rows) {
+      const int row = static_cast<int>(it);
+      const int held = min(pages_of(p, p.lens[row]), p.cols);
+      int* t = p.table + row * p.t_s0;
+      for (int j = threadIdx.x; j < held; j += COPY_THREADS) {
+        const int page = t[j * p.t_s1];
+        if (page < 0) continue;
+        if (page >= p.num_pages) {
+          flag(p, ST_BAD_PAGE);
+          continue;
+        }
+        const int to = __ldcg(map + page);
+        if (to == -1) flag(p, ST_REFS);  // the books say that the page is free: left alone
+        else if (to <= -2) t[j * p.t_s1] = gaps[-2 - to];
+        else if (to != page) t[j * p.t_s1] = to;
+      }
+    } else {
+      const int i = static_cast<int>((it - p.rows) / p.chunks), c = static_cast<int>((it - p.rows) - static_cast<long long>(i) * p.chunks);
+      const int src = movers[i], dst = gaps[i];
+      if (c == 0 && threadIdx.x == 0) {
+        p.refs[dst] = p.refs[src];
+        p.refs[src] = 0;
+        map[src] = dst;
+      }
+      copy_piece(p, c, src, dst, p.page_size);
+    }
+  }
+}
+
+}  // namespace pages
+}  // namespace ga

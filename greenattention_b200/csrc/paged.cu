@@ -1,0 +1,172 @@
+// C ABI of the attention over 16-bit and e4m3 paged caches with first tokens kept visible (attn_paged.cuh): argument
+// checks, choice of the instance, launches.
+#include "../../include/green_attention.h"
+#include "api_internal.h"
+#include "attn_paged.cuh"
+
+namespace {
+
+using ga::api::fail;
+using ga::paged::PagedDev;
+
+struct Launch {
+  PagedDev d;
+  cudaStream_t st;
+  int sm;
+  long long max_tokens;  // keys a page-table row can address
+  bool prompt;
+};
+
+size_t prefix_bytes(int batch) { return (static_cast<size_t>(batch) + 1 + 63) / 64 * 256; }
+size_t slots_bytes(int sm) { return static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) * 4; }
+
+template <class I>
+int limits() {
+  GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(ga::paged::attn_paged_kernel<I, 0>),
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
+  GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(ga::paged::attn_paged_kernel<I, 1>),
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
+  return 0;
+}
+
+template <class I>
+int run(Launch& a) {
+  PagedDev& d = a.d;
+  static_assert(I::NW * I::RC * I::HD <= ga::paged::SLOT_FLOATS && I::NW * I::RC <= ga::paged::SLOT_ROWS, "slot");
+  d.groups = (d.kvh + I::NW - 1) / I::NW;
+  d.hg = (d.kvh + d.groups - 1) / d.groups;
+  d.walkers = I::NW / d.hg;
+  const long long rows = static_cast<long long>(d.max_q) * d.gqa;
+  if (a.prompt) {
+    // a request of n tokens has ceil(n * gqa / RC) row blocks
+    const long long blocks = static_cast<long long>(d.total_q) * d.gqa / I::RC + d.batch;
+    const long long grid = (blocks + d.walkers - 1) / d.walkers;
+    if (grid > 0x7fffffffLL || d.groups > 65535) return fail("too many row blocks");
+    d.nrb = 1;
+    d.upr = d.groups;
+    GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 1>, dim3(static_cast<unsigned>(grid), d.groups), dim3(I::NT),
+                                  I::SMEM, a.st, d));
+    ga::api::launches(1);
+    return 0;
+  }
+  d.nrb = static_cast<int>((rows + I::RC - 1) / I::RC);
+  d.upr = d.groups * d.nrb;
+  const long long units = static_cast<long long>(d.batch) * d.upr;
+  const long long tiles = units * ((a.max_tokens + I::T - 1) / I::T);
+  if (units > 0x7fffffffLL) return fail("too many (request, head group, row block) units");
+  const long long want = (tiles + d.walkers - 1) / d.walkers;
+  const int grid = static_cast<int>(want < a.sm ? (want > 0 ? want : 1) : a.sm);
+  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 0>, dim3(grid), dim3(I::NT), I::SMEM, a.st, d));
+  // Enough CTAs to spread the rows of a small call over the SMs.
+  const long long pairs = units * d.hg;
+  const int block_rows = rows < I::RC ? static_cast<int>(rows) : I::RC;
+  long long z = (2LL * a.sm + pairs - 1) / pairs;
+  if (z > block_rows) z = block_rows;
+  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_combine<I>, dim3(static_cast<unsigned>(units), d.hg, static_cast<unsigned>(z)),
+                                dim3(128), 0, a.st, d, grid * d.walkers));
+  ga::api::launches(2);
+  return 0;
+}
+
+template <int KV>
+int run_kv(Launch& a, int hd) {
+  using namespace ga::paged;
+  const long long rows = static_cast<long long>(a.d.max_q) * a.d.gqa;
+  if (hd == 64) return a.prompt || rows > 16 ? run<Inst<64, KV, 2>>(a) : run<Inst<64, KV, 1>>(a);
+  if (hd == 128) return a.prompt || rows > 16 ? run<Inst<128, KV, 2>>(a) : run<Inst<128, KV, 1>>(a);
+  return run<Inst<256, KV, 1>>(a);
+}
+
+template <int KV>
+int limits_kv() {
+  using namespace ga::paged;
+  return limits<Inst<64, KV, 1>>() || limits<Inst<64, KV, 2>>() || limits<Inst<128, KV, 1>>() ||
+         limits<Inst<128, KV, 2>>() || limits<Inst<256, KV, 1>>();
+}
+
+}  // namespace
+
+int ga::api::init_paged() { return limits_kv<ga::paged::KV_BF16>() || limits_kv<ga::paged::KV_FP16>() || limits_kv<ga::paged::KV_E4M3>(); }
+
+extern "C" {
+
+size_t ga_paged_workspace_bytes(int device, int max_batch) {
+  const int sm = ga_sm_count(device);
+  return prefix_bytes(max_batch) + slots_bytes(sm > 0 ? sm : 160);
+}
+
+int ga_paged_attend(const GaPagedParams* a, void* stream) {
+  Launch l;
+  int dev;
+  if (ga::api::device(&dev, &l.sm)) return 1;
+  if (!a) return fail("null params");
+  if (a->kv_type < 0 || a->kv_type > 2) return fail("kv_type %d", a->kv_type);
+  if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256) return fail("head_dim %d: only 64, 128 and 256 are built", a->head_dim);
+  if (a->kv_heads <= 0 || a->q_heads <= 0 || a->q_heads % a->kv_heads) return fail("q_heads %d / kv_heads %d", a->q_heads, a->kv_heads);
+  if (a->page_size <= 0 || (a->page_size & (a->page_size - 1))) return fail("page_size %d is not a power of two", a->page_size);
+  if (a->batch <= 0 || a->num_pages < 0 || a->pt_cols < 0) return fail("batch %d, num_pages %d, pt_cols %d", a->batch, a->num_pages, a->pt_cols);
+  if (a->total_q < 0 || a->total_q > 0x7fffffffLL) return fail("total_q %lld", (long long)a->total_q);
+  if (a->max_seqlen_q < 1) return fail("max_seqlen_q %d", a->max_seqlen_q);
+  if (a->sink_tokens < 0) return fail("sink_tokens %d", a->sink_tokens);
+  if (a->total_q == 0) {
+    ga::api::launches(0);
+    return 0;
+  }
+  if (!a->q || !a->k_cache || !a->v_cache || !a->page_table || !a->cache_seqlens || !a->cu_seqlens_q || !a->out || !a->status)
+    return fail("null tensor pointer");
+  const int el = a->kv_type == ga::paged::KV_E4M3 ? 1 : 2;
+  const int64_t kv[6] = {a->k_stride_page, a->k_stride_tok, a->k_stride_head, a->v_stride_page, a->v_stride_tok, a->v_stride_head};
+  for (int64_t s : kv)
+    if (s < 0 || s * el % 16) return fail("k/v cache strides must be multiples of 16 bytes");
+  if ((reinterpret_cast<uintptr_t>(a->k_cache) | reinterpret_cast<uintptr_t>(a->v_cache)) & 15) return fail("k/v cache base must be 16-byte aligned");
+  const bool q8 = el == 1 && !a->q_is_bf16;
+  if (a->q_stride_tok % 4 || a->q_stride_head % 4 || reinterpret_cast<uintptr_t>(a->q) % (q8 ? 4 : 8)) return fail("q strides/base must allow 4-element vector loads");
+  if (a->o_stride_tok % 4 || a->o_stride_head % 4 || reinterpret_cast<uintptr_t>(a->out) % 8) return fail("out strides/base must allow 4-element vector stores");
+  // Only the route without split units needs no workspace, but which route a call takes is not the caller's business.
+  if (!a->workspace || a->workspace_bytes < prefix_bytes(a->batch) + slots_bytes(l.sm))
+    return fail("workspace too small: %zu < %zu bytes", a->workspace_bytes, prefix_bytes(a->batch) + slots_bytes(l.sm));
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 256) return fail("workspace must be 256-byte aligned");
+
+  PagedDev& d = l.d;
+  std::memset(&d, 0, sizeof(d));
+  d.q = static_cast<const uint8_t*>(a->q);
+  d.q_kind = el == 1 && a->q_is_bf16 ? ga::paged::Q_BF16_TO_E4M3 : ga::paged::Q_SAME;
+  d.q_s0 = a->q_stride_tok, d.q_s1 = a->q_stride_head;
+  d.k = static_cast<const uint8_t*>(a->k_cache);
+  d.v = static_cast<const uint8_t*>(a->v_cache);
+  d.k_s0 = a->k_stride_page * el, d.k_s1 = a->k_stride_tok * el, d.k_s2 = a->k_stride_head * el;
+  d.v_s0 = a->v_stride_page * el, d.v_s1 = a->v_stride_tok * el, d.v_s2 = a->v_stride_head * el;
+  d.page_shift = __builtin_ctz(a->page_size);
+  d.page_mask = a->page_size - 1;
+  d.num_pages = a->num_pages;
+  d.kvh = a->kv_heads, d.gqa = a->q_heads / a->kv_heads, d.q_heads = a->q_heads;
+  d.pt = a->page_table;
+  d.pt_s0 = a->pt_stride_row, d.pt_s1 = a->pt_stride_col, d.pt_cols = a->pt_cols;
+  d.seqlens = a->cache_seqlens;
+  d.cu = a->cu_seqlens_q;
+  d.kd = a->k_descale, d.kd_s0 = a->kd_stride_b, d.kd_s1 = a->kd_stride_h;
+  d.vd = a->v_descale, d.vd_s0 = a->vd_stride_b, d.vd_s1 = a->vd_stride_h;
+  d.out = a->out;
+  d.o_s0 = a->o_stride_tok, d.o_s1 = a->o_stride_head;
+  d.lse = a->lse;
+  d.total_q = static_cast<int>(a->total_q);
+  d.batch = a->batch;
+  d.max_q = a->max_seqlen_q < d.total_q ? a->max_seqlen_q : d.total_q;
+  constexpr int kFar = 1 << 30;  // no position is further away
+  d.window = a->window_left < 0 ? -1 : (a->window_left < kFar ? a->window_left : kFar);
+  d.sinks = d.window < 0 ? 0 : (a->sink_tokens < kFar ? a->sink_tokens : kFar);
+  d.scale_log2 = a->softmax_scale * 1.4426950408889634f;
+  d.status = a->status;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  d.prefix = reinterpret_cast<int*>(ws);
+  d.ws_lse = reinterpret_cast<float*>(ws + prefix_bytes(a->batch));
+  d.ws_o = d.ws_lse + static_cast<size_t>(2 * l.sm) * ga::paged::SLOT_ROWS;
+  l.st = static_cast<cudaStream_t>(stream);
+  l.max_tokens = static_cast<long long>(a->pt_cols) * a->page_size;
+  l.prompt = d.max_q > 16;
+  if (a->kv_type == ga::paged::KV_BF16) return run_kv<ga::paged::KV_BF16>(l, a->head_dim);
+  if (a->kv_type == ga::paged::KV_FP16) return run_kv<ga::paged::KV_FP16>(l, a->head_dim);
+  return run_kv<ga::paged::KV_E4M3>(l, a->head_dim);
+}
+
+}  // extern "C"

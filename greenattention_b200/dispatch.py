@@ -49,6 +49,7 @@ def _parse_disabled(raw: str) -> frozenset:
 
 DISABLED = _parse_disabled(os.environ.get("GREEN_ATTN_DISABLE", ""))
 STRICT = os.environ.get("GREEN_ATTN_STRICT", "1") != "0"
+KV16 = os.environ.get("GREEN_ATTN_KV16", "0") == "1"  # serve bf16 / fp16 caches too (attn_paged)
 
 _selectors: dict = defaultdict(list)
 _prewarms: list = []
@@ -130,11 +131,24 @@ def kvcache_op(max_seqlen_q: Any) -> Optional[str]:
 
 
 def owns(kwargs: dict) -> bool:
-    """True for the calls this backend exists for: attention over a paged e4m3 KV cache."""
+    """True for the calls this backend exists for: attention over a paged e4m3 KV cache, and any paged call with
+    first tokens kept visible (``sink_tokens``), which the stock function does not know."""
     kc = kwargs.get("k_cache")
     return (
         isinstance(kc, torch.Tensor)
-        and kc.dtype == torch.float8_e4m3fn
+        and (kc.dtype == torch.float8_e4m3fn or kwargs.get("sink_tokens") is not None)
+        and kwargs.get("page_table") is not None
+    )
+
+
+def takes_kv16(kwargs: dict) -> bool:
+    """True for paged calls over a bf16 / fp16 cache when the server asked for them (``GREEN_ATTN_KV16=1``); one that
+    the kernels decline goes to the stock function, whatever ``GREEN_ATTN_STRICT`` says."""
+    kc = kwargs.get("k_cache")
+    return (
+        KV16
+        and isinstance(kc, torch.Tensor)
+        and kc.dtype in (torch.bfloat16, torch.float16)
         and kwargs.get("page_table") is not None
     )
 
@@ -147,7 +161,7 @@ def with_kvcache(fallback: Callable) -> Callable:
     def flash_attn_with_kvcache(*args, **kwargs):
         mine = not args and owns(kwargs)
         op = kvcache_op(kwargs.get("max_seqlen_q"))
-        if op is None and mine:
+        if op is None and (mine or (not args and takes_kv16(kwargs))):
             op = "extend"
         if op is not None and args:
             log_fallback(op, ("positional arguments",), kwargs)

@@ -174,6 +174,71 @@ typedef struct GaGdnVerifyParams {
   float scale;
 } GaGdnVerifyParams;
 
+/* Attention over a paged cache of bf16, fp16 or e4m3 keys and values: decode, verify and prompts of any length, with an
+ * optional left window and `sink_tokens` first tokens that stay visible beside it. Key j is visible to the query at
+ * position p when j <= p and (window_left < 0 or j >= p - window_left or j < sink_tokens). Page-table entries of pages
+ * without a visible key are never read (they may be released pages' or padding). A row without visible keys gets zeros
+ * and an LSE of -inf; rows of q / out / lse past cu_seqlens_q[batch] are left alone. No counterpart in the reference
+ * (its kernels read e4m3 caches and have no first tokens). */
+typedef struct GaPagedParams {
+  int32_t kv_type;          /* 0 bf16, 1 fp16, 2 e4m3 */
+  const void* q;            /* [total_q, q_heads, head_dim]: the cache's type; beside e4m3 e4m3 or bf16 (rounded to e4m3) */
+  int32_t q_is_bf16;        /* only looked at beside an e4m3 cache */
+  int64_t q_stride_tok, q_stride_head; /* elements, multiples of 4 */
+  const void* k_cache;      /* [num_pages, page_size, kv_heads, head_dim], last stride 1, 16-byte aligned */
+  const void* v_cache;
+  int64_t k_stride_page, k_stride_tok, k_stride_head; /* elements, multiples of 16 bytes */
+  int64_t v_stride_page, v_stride_tok, v_stride_head;
+  int32_t num_pages, page_size;        /* page_size a power of two, from 1 */
+  int32_t q_heads, kv_heads, head_dim; /* head_dim 64, 128 or 256; q_heads % kv_heads == 0 */
+  const int32_t* page_table;    /* [batch, pt_cols] */
+  int64_t pt_stride_row, pt_stride_col;
+  int32_t pt_cols;
+  const int32_t* cache_seqlens; /* [batch] keys per request, new tokens included; cut to pt_cols * page_size (status 5) */
+  const int32_t* cu_seqlens_q;  /* [batch + 1] */
+  const float* k_descale;       /* [batch | 1, kv_heads] or NULL (= 1) */
+  int64_t kd_stride_b, kd_stride_h;
+  const float* v_descale;
+  int64_t vd_stride_b, vd_stride_h;
+  void* out;                /* [total_q, q_heads, head_dim]: the cache's type, bf16 beside e4m3 */
+  int64_t o_stride_tok, o_stride_head; /* elements, multiples of 4 */
+  float* lse;               /* [q_heads, total_q] natural log, or NULL */
+  int64_t total_q;
+  int32_t batch;
+  int32_t max_seqlen_q;     /* no request has more new tokens (what is beyond is left alone) */
+  int32_t window_left;      /* -1: none */
+  int32_t sink_tokens;      /* without a window nothing is hidden and this says nothing */
+  float softmax_scale;
+  int32_t* status;          /* device word, sticky: 3 a page id was out of range (its keys read as zeros), 5 as above */
+  void* workspace;          /* ga_paged_workspace_bytes() bytes, 256-byte aligned, this call's own until it has run */
+  size_t workspace_bytes;
+} GaPagedParams;
+
+/* The pages of a paged cache: one pool of pages per tensor (K and V of every layer), all with the same page ids, and the
+ * books that say who holds which page. refs[page] counts the page-table entries that hold a page (0: free); a row holds
+ * ceil(seqlens[row] / page_size) entries, -1 for a released page. Calls on a pool are ordered on one stream. Nothing
+ * is read or written outside the pool whatever the indices say; what a call could not do is left out and flagged in
+ * *status (sticky): 3 a page id out of range, 5 a length beyond the table's row, 7 a row or page index out of range, 8 no
+ * free page left, 9 the counts do not match the table, 10 entries of one call that contradict one another. `scratch`
+ * belongs to the call until it has run. No counterpart in the reference (its host owns the pages). */
+typedef struct GaPagePool {
+  const uint64_t* base;         /* [tensors] DEVICE array of the addresses of page 0, 16-byte aligned */
+  const int64_t* page_stride;   /* [tensors] bytes from page to page, multiples of 16; a page's tokens are dense */
+  const int32_t* tok_bytes;     /* [tensors] bytes of a token, multiples of 16 */
+  const int32_t* chunk_tensor;  /* [chunks] tensor of each 16 KB piece of a page, tensor by tensor */
+  const int32_t* chunk_first;   /* [tensors] its first piece */
+  int32_t tensors, chunks;
+  int32_t num_pages, page_size; /* page_size a power of two */
+  int32_t* page_table;          /* [rows, cols] */
+  int64_t pt_stride_row, pt_stride_col;
+  int32_t rows, cols;
+  int32_t* seqlens;             /* [rows] */
+  int32_t* refs;                /* [num_pages] */
+  int32_t* status;
+  void* scratch;                /* ga_pages_scratch_bytes() bytes, 256-byte aligned */
+  size_t scratch_bytes;
+} GaPagePool;
+
 /* Once per process and device, before the first launch and before any graph capture: resolves the
  * driver entry point used to encode TMA descriptors and raises the dynamic shared memory limit of every
  * kernel instance. Idempotent. */
@@ -206,6 +271,27 @@ int ga_attn_extend(const GaAttnParams* p, void* stream);
 int ga_attn_decode_noalloc(const GaAttnParams* p, void* stream);
 int ga_attn_merge(const GaMergeParams* p, void* stream);
 int ga_attn_exchange_merge(const GaExchangeParams* p, void* stream);
+/* Bytes of scratch one ga_paged_attend() call of at most `max_batch` requests needs on `device`. */
+size_t ga_paged_workspace_bytes(int device, int max_batch);
+int ga_paged_attend(const GaPagedParams* p, void* stream);
+/* Scratch of a call with `n` entries. Indices are int32, or int64 where is64 is 1. */
+size_t ga_pages_scratch_bytes(const GaPagePool* p, int n);
+/* Page dst[i] becomes a copy of page src[i] in every tensor. Of entries with one dst the last counts; an entry whose src
+ * another entry writes is left out (10). */
+int ga_pages_copy(const GaPagePool* p, const void* src, const void* dst, int is64, int n, void* stream);
+/* Row children[i] (empty) becomes a copy of row parents[i]: full pages are shared, the tokens of a partial last page are
+ * copied to a new one. New pages are the lowest free ones, in the entries' order. At most 32768 entries. */
+int ga_pages_fork(const GaPagePool* p, const void* parents, const void* children, int is64, int n, void* stream);
+/* The rows' pages are released and their lengths become 0. */
+int ga_pages_free(const GaPagePool* p, const void* rows, int is64, int n, void* stream);
+/* Releases the pages whose keys are neither among the first sink_tokens nor in the window [len - window_left, ..] of the
+ * row's next query; their entries become -1, the length stays. */
+int ga_pages_evict(const GaPagePool* p, const void* rows, int is64, int n, int window_left, int sink_tokens, void* stream);
+/* Rows grow to lens[i] tokens (a smaller length leaves a row alone) with the lowest free pages, in the entries' order. */
+int ga_pages_grow(const GaPagePool* p, const void* rows, const void* lens, int is64, int lens64, int n, void* stream);
+/* The *live held pages move below id *live: those at or above it, in order, into the free ids below. The table and the
+ * counts follow; map[page] is a page's new id, -1 for a free one. */
+int ga_pages_compact(const GaPagePool* p, int32_t* map, int32_t* live, void* stream);
 int ga_gdn_recurrent(const GaGdnParams* p, void* stream);
 int ga_gdn_verify(const GaGdnVerifyParams* p, void* stream);
 

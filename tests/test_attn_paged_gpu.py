@@ -1,0 +1,313 @@
+"""Attention over 16-bit and e4m3 paged caches with a window and first tokens, against the 64-bit definition. The bounds
+are the oracle's (``oracle/paged_oracle.attend``): roundings counted by half steps, the 32-bit sums by their lengths."""
+
+import pytest
+import torch
+
+from oracle import paged_oracle
+
+pytestmark = pytest.mark.gpu
+BF16, FP16, FP8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def make(dtype, lens, new, page, qh, kvh, hd, window=-1, sinks=0, seed=0, q_dtype=None, descale=False, stacked=False,
+         heads_first=False, q_wide=False, scale=None):
+    """A call over a shuffled pool. Pages without a visible key are not in the table (-1), what no query may see is NaN."""
+    g = torch.Generator().manual_seed(seed)
+    cols = max(1, max(-(-n // page) for n in lens)) + 2
+    table = torch.full((len(lens), cols), -1, dtype=torch.int64)
+    seen, b_of = [], []
+    for b, (n, t) in enumerate(zip(lens, new)):
+        lo = max(0, n - t - window) if window >= 0 else 0
+        vis = [j for j in range(n) if j >= lo or j < sinks] if n - t + t > 0 else []
+        held = sorted({j // page for j in vis})
+        seen.append(vis)
+        b_of += [(b, c) for c in held]
+    pages = len(b_of) + 2
+    ids = torch.randperm(pages, generator=g)[: len(b_of)]
+    for (b, c), i in zip(b_of, ids.tolist()):
+        table[b, c] = i
+    shape = (pages, kvh, page, hd) if heads_first else (pages, page, kvh, hd)
+    if stacked:
+        buf = torch.full((pages, 2, *shape[1:]), float("nan"))
+        caches = [buf[:, 0], buf[:, 1]]
+    else:
+        caches = [torch.full(shape, float("nan")) for _ in range(2)]
+    views = [c.transpose(1, 2) if heads_first else c for c in caches]
+    for b, vis in enumerate(seen):
+        if vis:
+            at = torch.tensor(vis)
+            for c in views:
+                c[table[b, at // page], at % page] = torch.randn((len(vis), kvh, hd), generator=g)
+    if stacked:
+        buf = buf.to(dtype).cuda()
+        kc, vc = buf[:, 0], buf[:, 1]
+    else:
+        kc, vc = (c.to(dtype).cuda() for c in caches)
+    if heads_first:
+        kc, vc = kc.transpose(1, 2), vc.transpose(1, 2)
+    total = sum(new)
+    q = torch.randn((total, qh, hd), generator=g)
+    q = q.to(q_dtype or (BF16 if dtype == FP8 else dtype)).cuda()
+    if q_wide:
+        wide = torch.zeros((total, qh + 1, hd + 8), dtype=q.dtype, device="cuda")
+        wide[:, :qh, :hd] = q
+        q = wide[:, :qh, :hd]
+    cu = torch.tensor([0] + new).cumsum(0).to(torch.int32).cuda()
+    kw = dict(q=q, k_cache=kc, v_cache=vc, page_table=table.to(torch.int32).cuda(),
+              cache_seqlens=torch.tensor(lens, dtype=torch.int32).cuda(), cu_seqlens_q=cu, max_seqlen_q=max(1, max(new)),
+              causal=True, return_softmax_lse=True, softmax_scale=scale)
+    if window >= 0:
+        kw |= dict(window_size=(window, 0), sink_tokens=sinks)
+    if descale:
+        kw |= {n: (torch.rand((len(lens), kvh), generator=g) + 0.5).cuda() for n in ("k_descale", "v_descale")}
+    return kw
+
+
+def check(kw, got=None):
+    from greenattention_b200 import attn_paged
+
+    out, lse = attn_paged.attend(**kw) if got is None else got
+    torch.cuda.synchronize()
+    want = paged_oracle.attend(kw)
+    rows = ~want["out"].isnan()
+    off = (out.cpu().double() - want["out"]).abs()
+    assert (off <= want["out_tol"])[rows].all(), f"out: {(off / want['out_tol'].clamp(min=1e-30))[rows].max()} of the bound"
+    zl, gl = want["lse"], lse.cpu().double()
+    fin = zl.isfinite()
+    assert torch.equal(gl[zl == -torch.inf], zl[zl == -torch.inf])
+    assert ((gl - zl).abs() <= want["lse_tol"])[fin].all()
+    assert attn_paged.check_status() == 0
+    return out, lse
+
+
+SHAPES = [(8, 2, 128), (6, 6, 64), (5, 1, 64), (16, 8, 128), (15, 5, 128), (12, 3, 256), (20, 10, 256), (24, 12, 64)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("qh,kvh,hd", SHAPES)
+def test_decode(dtype, qh, kvh, hd):
+    check(make(dtype, [1, 137, 64, 300, 0, 33], [1] * 6, 16, qh, kvh, hd, seed=hd + qh, descale=dtype == FP8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("page", [1, 2, 8, 64, 256])
+def test_page_sizes(dtype, page):
+    check(make(dtype, [1, 255, 256, 257, 90], [1] * 5, page, 8, 4, 128, seed=page))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (0, 1), (1, 0), (15, 4), (16, 16), (63, 5), (100, 33), (100, 129), (64, 0), (5000, 3)])
+def test_window_and_first_tokens(dtype, hd, window, sinks):
+    check(make(dtype, [1, 5, 129, 400, 97], [1] * 5, 16, 8, 4, hd, window, sinks, seed=window + sinks, descale=dtype == FP8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("qh,kvh,hd", [(8, 2, 128), (8, 8, 64), (16, 1, 128), (4, 1, 256), (64, 1, 64)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (40, 3)])
+def test_verify(dtype, qh, kvh, hd, window, sinks):
+    """Several new tokens, more of them than keys among them (their first rows see nothing), requests without any."""
+    check(make(dtype, [200, 3, 64, 31, 9], [5, 5, 1, 0, 16], 16, qh, kvh, hd, window, sinks, seed=qh))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("qh,kvh,hd,page", [(8, 2, 128, 16), (4, 4, 64, 1), (6, 2, 256, 64), (7, 1, 128, 32), (34, 2, 128, 128)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (50, 7), (0, 2), (200, 0)])
+def test_prompts(dtype, qh, kvh, hd, page, window, sinks):
+    check(make(dtype, [130, 257, 40, 1, 300], [130, 100, 17, 1, 64], page, qh, kvh, hd, window, sinks, seed=page + qh,
+               descale=dtype == FP8))
+
+
+def test_prompt_with_more_tokens_than_keys():
+    check(make(BF16, [20, 0, 70], [40, 33, 70], 16, 8, 2, 128, seed=5))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("new", [1, 5, 40])
+def test_layouts(dtype, new):
+    """Interleaved K / V, head-major pages, strided queries and outputs, an e4m3 query, a scalar descale."""
+    base = dict(page=16, qh=8, kvh=2, hd=128, window=70, sinks=4, seed=new)
+    check(make(dtype, [200, 90], [new, new], stacked=True, **base))
+    check(make(dtype, [200, 90], [new, new], heads_first=True, **base))
+    kw = make(dtype, [200, 90], [new, new], q_wide=True, **base)
+    wide = torch.full((2 * new + 3, 8, 136), float("nan"), dtype=BF16, device="cuda")
+    kw["out"] = wide[: 2 * new, :, :128]
+    check(kw)
+    assert wide[:, :, 128:].isnan().all() and wide[2 * new:].isnan().all()
+    if dtype == FP8:
+        kw = make(dtype, [200, 90], [new, new], q_dtype=FP8, **base)
+        kw |= dict(k_descale=torch.tensor([0.4], device="cuda").expand(2, 2), v_descale=torch.full((1, 2), 1.7, device="cuda"))
+        check(kw)
+
+
+@pytest.mark.parametrize("new", [1, 4, 50])
+def test_rows_behind_the_last_request_stay(new):
+    kw = make(BF16, [60, 99], [new, new], 16, 8, 2, 128, seed=3)
+    q = torch.cat([kw["q"], torch.full_like(kw["q"][:3], float("nan"))])
+    out = torch.full_like(q, 7.0)
+    kw |= dict(q=q, out=out)
+    from greenattention_b200 import attn_paged
+
+    got, lse = attn_paged.attend(**kw)
+    assert got is out and (out[2 * new:] == 7).all()
+    kw2 = dict(kw, q=q[: 2 * new], out=None)
+    check(kw2, (out[: 2 * new], lse[:, : 2 * new]))
+
+
+@pytest.mark.parametrize("batch,n", [(1, 20000), (300, 40), (3, 3000)])
+@pytest.mark.parametrize("kvh", [1, 8])
+def test_splits(batch, n, kvh):
+    """One long sequence over all SMs, and more requests than SMs; the split must not change what comes out."""
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(n // 2, n + 1, (batch,), generator=g).tolist()
+    kw = make(BF16, lens, [1] * batch, 64, 2 * kvh, kvh, 64, seed=n)
+    from greenattention_b200 import attn_paged
+
+    a, la = attn_paged.attend(**kw)
+    b, lb = attn_paged.attend(**kw)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+    few = list(range(0, batch, max(1, batch // 3)))[:3]
+    sub = dict(kw, q=kw["q"][few], page_table=kw["page_table"][few], cache_seqlens=kw["cache_seqlens"][few],
+               cu_seqlens_q=torch.arange(len(few) + 1, dtype=torch.int32, device="cuda"))
+    want = paged_oracle_fast(sub)
+    assert ((a[few].double() - want).abs() <= 2.0**-7 * want.abs() + 2.0**-8 * 4).all()
+
+
+def paged_oracle_fast(kw):
+    """One new token, no window: the definition on the GPU in 64 bits."""
+    page, kvh, hd = kw["k_cache"].shape[1:]
+    out = torch.empty(kw["q"].shape, dtype=torch.float64, device="cuda")
+    for b, n in enumerate(kw["cache_seqlens"].tolist()):
+        at = torch.arange(n, device="cuda")
+        ids = kw["page_table"][b, at // page].long()
+        k, v = (kw[x][ids, at % page].double().transpose(0, 1) for x in ("k_cache", "v_cache"))
+        q = kw["q"][b].double().view(kvh, -1, hd)
+        out[b] = (torch.softmax(q @ k.transpose(1, 2) * hd**-0.5, -1) @ v).reshape(-1, hd)
+    return out
+
+
+def test_offsets_beyond_32_bits():
+    """The call's pages lie behind 2^32 elements of the pool."""
+    page, kvh, hd = 64, 8, 128
+    pages = (1 << 32) // (page * kvh * hd) + 3
+    kw = make(BF16, [150, 70], [1, 1], page, 16, kvh, hd, seed=2)
+    for n in ("k_cache", "v_cache"):
+        big = torch.empty((pages, page, kvh, hd), dtype=BF16, device="cuda")
+        small = kw[n]
+        big[-small.shape[0]:] = small
+        kw["big_" + n] = big
+    shift = pages - kw["k_cache"].shape[0]
+    from greenattention_b200 import attn_paged
+
+    moved = {k: v for k, v in kw.items() if not k.startswith("big_")}
+    want = attn_paged.attend(**moved)
+    moved |= dict(k_cache=kw["big_k_cache"], v_cache=kw["big_v_cache"],
+                  page_table=torch.where(kw["page_table"] >= 0, kw["page_table"] + shift, kw["page_table"]))
+    got = attn_paged.attend(**moved)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_non_finite_values_count_where_they_are_seen():
+    kw = make(BF16, [50, 50, 50], [1, 1, 1], 16, 4, 2, 64, seed=8)
+    pt = kw["page_table"].tolist()
+    kw["v_cache"][pt[0][1], 3, 0, 5] = float("inf")
+    kw["k_cache"][pt[1][1], 3, 1, 0] = float("nan")
+    from greenattention_b200 import attn_paged
+
+    out, lse = attn_paged.attend(**kw)
+    out = out.view(3, 2, 2, 64)
+    assert (out[0, 0, :, 5] == float("inf")).all() and out[0, 0, :, :5].isfinite().all() and out[0, 1].isfinite().all()
+    assert out[1, 1].isnan().all() and lse[2:, 1].isnan().all() and out[1, 0].isfinite().all()
+    assert out[2].isfinite().all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_bad_pages_and_lengths_are_flagged(new):
+    from greenattention_b200 import attn_paged
+
+    kw = make(BF16, [100, 100], [new, new], 16, 4, 2, 64, seed=9)
+    good = attn_paged.attend(**kw)[0]
+    bad = dict(kw, page_table=kw["page_table"].clone())
+    bad["page_table"][0, 2] = kw["k_cache"].shape[0]
+    out, _ = attn_paged.attend(**bad)
+    assert attn_paged.check_status() == 3 and attn_paged.check_status() == 0
+    assert out[:new].isfinite().all() and torch.equal(out[new:], good[new:])
+    long = dict(kw, cache_seqlens=torch.tensor([100, 1 << 20], dtype=torch.int32, device="cuda"))
+    out, _ = attn_paged.attend(**long)
+    assert attn_paged.check_status() != 0
+    assert torch.equal(out[:new], good[:new])
+
+
+@pytest.mark.parametrize("new", [1, 33])
+def test_graph_replays_with_live_lengths(new):
+    """Two captured graphs and eager calls in turn, lengths and table changed between replays."""
+    from greenattention_b200 import attn_paged
+
+    attn_paged.ensure_ready()
+    kws = [make(BF16, [200, 130], [new, new], 16, 8, 2, 128, 90, 4, seed=s) for s in (1, 2)]
+    outs, graphs = [], []
+    for kw in kws:
+        out = torch.empty_like(kw["q"])
+        outs.append(out)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            attn_paged.attend(**dict(kw, out=out))
+        graphs.append(g)
+    for step in range(2):
+        want = [attn_paged.attend(**kw)[0] for kw in kws]
+        for o in outs:
+            o.fill_(3)
+        streams = [torch.cuda.Stream() for _ in graphs]
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        # bit by bit: with the shorter lengths the window reaches back to keys that the inputs hold as NaN
+        for w, o in zip(want, outs):
+            assert torch.equal(w.view(torch.int16), o.view(torch.int16))
+        assert want[0].isfinite().all() == (step == 0)
+        for kw in kws:
+            kw["cache_seqlens"].copy_(torch.tensor([190, 125], dtype=torch.int32))
+
+
+def test_calls_on_two_streams():
+    from greenattention_b200 import attn_paged
+
+    kws = [make(FP16, [3000, 500], [1, 1], 16, 8, 2, 128, seed=s) for s in (1, 2)]
+    want = [attn_paged.attend(**kw) for kw in kws]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in kws]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(attn_paged.attend(**kws[i])[0])
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w[0], x) for x in g)
+
+
+def test_through_the_backend_entry(monkeypatch):
+    """``with_kvcache``: calls with first tokens are served, 16-bit caches without them when the server asked."""
+    import importlib
+
+    from greenattention_b200 import attn_decode, attn_paged, dispatch
+
+    attn_decode.ensure_ready()
+    attn_paged.ensure_ready()
+    importlib.reload(attn_paged)
+    attn_paged.ensure_ready()
+    entry = dispatch.with_kvcache(lambda **kw: "stock")
+    for new in (1, 4, 40):
+        kw = make(FP8, [100, 70], [new, new], 16, 8, 2, 128, 30, 4, seed=new)
+        check(kw, entry(**kw))
+        kw = make(BF16, [100, 70], [new, new], 16, 8, 2, 128, seed=new)
+        assert entry(**kw) == "stock"
+        monkeypatch.setattr(dispatch, "KV16", True)
+        check(kw, entry(**kw))
+        assert entry(**dict(kw, softcap=30.0)) == "stock"
+        monkeypatch.setattr(dispatch, "KV16", False)
+    with pytest.raises(dispatch.Declined, match="softcap"):
+        entry(**dict(make(BF16, [9], [1], 16, 8, 2, 128, 30, 4), softcap=30.0))
