@@ -3,6 +3,7 @@
 #include "../../include/green_attention.h"
 #include "api_internal.h"
 #include "attn_paged.cuh"
+#include "attn_paged_tc.cuh"
 
 namespace {
 
@@ -26,6 +27,32 @@ int limits() {
                               cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
   GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(ga::paged::attn_paged_kernel<I, 1>),
                               cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
+  return 0;
+}
+
+template <class I>
+int limits_tc() {
+  GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(ga::paged::tc::attn_paged_tc_kernel<I>),
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
+  return 0;
+}
+
+// Prompts on the tensor cores; -1: the call is not one for them.
+template <class I>
+int run_tc(Launch& a, size_t ws_bytes) {
+  PagedDev& d = a.d;
+  // its rows go through 16-byte copies, and it takes the maximum before the scale
+  if (d.kd || !(d.scale_log2 > 0.f) || d.q_s0 % 8 || d.q_s1 % 8 || reinterpret_cast<uintptr_t>(d.q) % 16) return -1;
+  const long long blocks = static_cast<long long>(d.total_q) * d.gqa / I::ROWS + d.batch;
+  const size_t need = 256 + static_cast<size_t>(blocks) * 8;
+  if (need > ws_bytes || blocks * d.kvh > 0x7fffffffLL) return -1;
+  int* count = d.prefix;
+  int2* list = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(d.prefix) + 256);
+  GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_prompts_kernel<I::ROWS>, dim3(1), dim3(1024), 0, a.st, d, count, list));
+  const long long items = blocks * d.kvh;
+  GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(static_cast<unsigned>(items < a.sm ? items : a.sm)), dim3(I::NT),
+                                I::SMEM, a.st, d, const_cast<const int*>(count), const_cast<const int2*>(list)));
+  ga::api::launches(2);
   return 0;
 }
 
@@ -69,12 +96,26 @@ int run(Launch& a) {
 }
 
 template <int KV>
+int run_tc_kv(Launch& a, int hd, size_t ws_bytes) {
+  using namespace ga::paged::tc;
+  if (hd == 64) return run_tc<TcInst<64, KV>>(a, ws_bytes);
+  if (hd == 128) return run_tc<TcInst<128, KV>>(a, ws_bytes);
+  return run_tc<TcInst<256, KV>>(a, ws_bytes);
+}
+
+template <int KV>
 int run_kv(Launch& a, int hd) {
   using namespace ga::paged;
   const long long rows = static_cast<long long>(a.d.max_q) * a.d.gqa;
   if (hd == 64) return a.prompt || rows > 16 ? run<Inst<64, KV, 2>>(a) : run<Inst<64, KV, 1>>(a);
   if (hd == 128) return a.prompt || rows > 16 ? run<Inst<128, KV, 2>>(a) : run<Inst<128, KV, 1>>(a);
   return run<Inst<256, KV, 1>>(a);
+}
+
+template <int KV>
+int limits_tc_kv() {
+  using namespace ga::paged::tc;
+  return limits_tc<TcInst<64, KV>>() || limits_tc<TcInst<128, KV>>() || limits_tc<TcInst<256, KV>>();
 }
 
 template <int KV>
@@ -86,7 +127,10 @@ int limits_kv() {
 
 }  // namespace
 
-int ga::api::init_paged() { return limits_kv<ga::paged::KV_BF16>() || limits_kv<ga::paged::KV_FP16>() || limits_kv<ga::paged::KV_E4M3>(); }
+int ga::api::init_paged() {
+  return limits_kv<ga::paged::KV_BF16>() || limits_kv<ga::paged::KV_FP16>() || limits_kv<ga::paged::KV_E4M3>() ||
+         limits_tc_kv<ga::paged::KV_BF16>() || limits_tc_kv<ga::paged::KV_FP16>();
+}
 
 extern "C" {
 
@@ -164,6 +208,11 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   l.st = static_cast<cudaStream_t>(stream);
   l.max_tokens = static_cast<long long>(a->pt_cols) * a->page_size;
   l.prompt = d.max_q > 16;
+  if (l.prompt && a->kv_type != ga::paged::KV_E4M3) {
+    const int rc = a->kv_type == ga::paged::KV_BF16 ? run_tc_kv<ga::paged::KV_BF16>(l, a->head_dim, a->workspace_bytes)
+                                                    : run_tc_kv<ga::paged::KV_FP16>(l, a->head_dim, a->workspace_bytes);
+    if (rc >= 0) return rc;
+  }
   if (a->kv_type == ga::paged::KV_BF16) return run_kv<ga::paged::KV_BF16>(l, a->head_dim);
   if (a->kv_type == ga::paged::KV_FP16) return run_kv<ga::paged::KV_FP16>(l, a->head_dim);
   return run_kv<ga::paged::KV_E4M3>(l, a->head_dim);
