@@ -31,7 +31,7 @@ namespace tc {
 constexpr int TM = 128;          // query rows of a tile = tensor memory lanes
 constexpr int TK = 128;          // keys of a tile
 constexpr int STAGE = 16384;
-constexpr int KV_WARPS = 4, Q_WARPS = 2;
+constexpr int Q_WARPS = 2;
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
 
 template <int HD_, int KV_>
@@ -43,10 +43,24 @@ struct TcInst {
   static constexpr int ROWS = NQ * TM;
   static constexpr int Q_BYTES = NQ * SLABS * STAGE;
   static constexpr int NST = HD == 64 ? 8 : 10;
-  static constexpr int SOFT_WARPS = 4 * NQ;
-  static constexpr int WARPS = SOFT_WARPS + 1 + KV_WARPS + Q_WARPS;
+  static constexpr int EG = SLABS < 2 ? SLABS : 2;  // stages that are filled and released together
+  static constexpr int SPLIT = 2;                   // threads that share a row
+  static constexpr int SOFT_WARPS = 4 * NQ * SPLIT;
+  static constexpr int KV_WARPS = NQ == 1 ? 8 : 4;
+  static constexpr int WARPS = (SOFT_WARPS + 1 + KV_WARPS + Q_WARPS + 3) / 4 * 4;  // whole warpgroups
   static constexpr int NT = WARPS * 32;
-  static constexpr int SMEM = 2048 + Q_BYTES + NST * STAGE;  // barriers, 1024-byte alignment
+  // Registers a thread: what the block is launched with (limit of the launch bounds), and its split between the softmax
+  // warps and the others. The shares add up to no more than the launch's.
+  static constexpr int REGS = NQ == 1 ? 96 : 80;
+  static constexpr int REGS_SOFT = NQ == 1 ? 128 : 96, REGS_REST = NQ == 1 ? 72 : 48;
+  static_assert(SOFT_WARPS * REGS_SOFT + (WARPS - SOFT_WARPS) * REGS_REST <= WARPS * REGS, "register split");
+  // Row maxima that the halves of a row exchange: at NQ 1 two jobs' in turn; at NQ 2 a query tile's next scores are ready
+  // only after both halves are done with the job before.
+  static constexpr int TURNS = 3 - NQ;
+  static constexpr int X_BYTES = 2 * 2 * TM * 4;
+  // Operands first: they need the 1024-byte alignment that dynamic shared memory starts with (the kernel checks it).
+  static constexpr int SMEM = Q_BYTES + NST * STAGE + X_BYTES + 512;
+  static_assert(NST % EG == 0, "ring");
   static constexpr int O_COL = 256;
   static_assert(SMEM <= 232448, "shared memory");
 };
@@ -73,6 +87,10 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc ? 1 : 0)
       : "memory");
 }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -115,6 +133,38 @@ __device__ __forceinline__ void wait_or_flag(uint32_t bar, uint32_t parity, bool
   if (!mbar_wait(bar, parity)) {
     failed = true;
     atomicExch(status, code);
+  }
+}
+
+// One warp fills a stage with KEYS keys of CPK 16-byte chunks each, in slabs of eight chunks (128 bytes a key), swizzled by
+// key. page[u] is the page of key u * 32 + lane, or -1 for a row of zeros. Its own instruction stream is what a stage costs
+// here (32 copies a lane), so a copy is its address step and little else: within 32 keys of one page the source advances
+// by a constant, and the swizzle of the destination is a constant flipped in. Smaller pages and edges pass each row's
+// offset from the lane that looked it up.
+template <int CPK, int KEYS>
+__device__ __forceinline__ void gather(uint32_t dst, const uint8_t* base, long long s0, long long s1, int n0, int page_shift, int page_mask,
+                                       const int (&page)[4], int lane) {
+  constexpr int KPI = 32 / CPK;  // keys an instruction
+  const int c = lane % CPK, k0 = lane / CPK;
+  const uint32_t d0 = (c >> 3) * (KEYS * 128) + k0 * 128 + (((c ^ k0) & 7) << 4);
+  base += c * 16;
+  const long long step = s1 * KPI;
+#pragma unroll
+  for (int u = 0; u < (KEYS + 31) / 32; ++u) {
+    const int tok = (n0 + u * 32) & page_mask;
+    if (page_shift >= 5 && __all_sync(0xffffffffu, page[u] >= 0)) {
+      const uint8_t* src = base + page[u] * s0 + (tok + k0) * s1;
+#pragma unroll
+      for (int i = 0; i < CPK; ++i, src += step)
+        cp_async_16(dst + (u * 32 + i * KPI) * 128 + (d0 ^ (((i * KPI) & 7) << 4)), src);
+    } else {
+      const long long off = page[u] >= 0 ? page[u] * s0 + ((n0 + u * 32 + lane) & page_mask) * s1 : -1;
+#pragma unroll 4
+      for (int i = 0; i < CPK; ++i) {
+        const long long o = __shfl_sync(0xffffffffu, off, i * KPI + k0);
+        cp_async_16_or_zero(dst + (u * 32 + i * KPI) * 128 + (d0 ^ (((i * KPI) & 7) << 4)), base + (o >= 0 ? o : 0), o >= 0);
+      }
+    }
   }
 }
 
@@ -162,14 +212,91 @@ __global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constan
   if (tid == 0) *count = base;
 }
 
+// What a row sees: keys in [lo, pos], and those below `sinks` that are not behind pos. pmin, pmax: positions of the first
+// and the last row of the thread's warp, which decide for 32 keys at a time whether any row has to look at them.
+struct View {
+  int pos, lo, sinks, pmin, pmax, window;
+};
+enum : int { ALL, SOME, NONE };
+__device__ __forceinline__ int chunk_class(const View& w, int base) {
+  if (base > w.pmax) return NONE;
+  if (base + 31 <= w.pmin && (w.window < 0 || base >= w.pmax - w.window || base + 31 < w.sinks)) return ALL;
+  if (w.window >= 0 && base + 31 < w.pmin - w.window && base >= w.sinks) return NONE;
+  return SOME;
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); }
+__device__ __forceinline__ uint32_t seen_bits(const View& w, int base) {
+  return low_bits(w.pos + 1 - base) & (~low_bits(w.lo - base) | low_bits(w.sinks - base));
+}
+
+// Largest visible score of a thread's KEYS keys of a row, from `n0` on.
+template <int KEYS>
+__device__ __forceinline__ float part_max(uint32_t tS, int n0, const View& w) {
+  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int c = 0; c < KEYS / 32; ++c) {
+    const int cls = chunk_class(w, n0 + c * 32);
+    if (cls == NONE) continue;
+    uint32_t v[32];
+    tmem_ld32(tS + c * 32, v);
+    wait_ld();
+    if (cls == SOME) {
+      const uint32_t seen = seen_bits(w, n0 + c * 32);
+#pragma unroll
+      for (int k = 0; k < 32; ++k)
+        if (!(seen >> k & 1)) v[k] = 0xff800000u;
+    }
+#pragma unroll
+    for (int k = 0; k < 32; ++k) mx[k & 3] = fmaxf(mx[k & 3], __uint_as_float(v[k]));
+  }
+  return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+}
+// P = 2^(s * sl2 - mu) as 16-bit pairs over the front of the thread's scores; returns the sum of the unrounded P.
+template <int KV, int KEYS>
+__device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, int n0, const View& w) {
+  float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int c = 0; c < KEYS / 32; ++c) {
+    const int cls = chunk_class(w, n0 + c * 32);
+    uint32_t out[16];
+    if (cls == NONE) {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) out[k] = 0u;
+    } else {
+      uint32_t v[32];
+      tmem_ld32(tS + c * 32, v);
+      wait_ld();
+      if (cls == SOME) {
+        const uint32_t seen = seen_bits(w, n0 + c * 32);
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (!(seen >> k & 1)) v[k] = 0xff800000u;
+      }
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) {
+        const float e0 = ex2(fmaf(__uint_as_float(v[k]), sl2, -mu)), e1 = ex2(fmaf(__uint_as_float(v[k + 1]), sl2, -mu));
+        part[k & 2] += e0;
+        part[(k & 2) + 1] += e1;
+        out[k / 2] = pack16<KV>(e0, e1);
+      }
+    }
+    tmem_st16(tS + c * 16, out);
+  }
+  return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
 template <class I>
 __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_constant__ PagedDev p, const int* count, const int2* blocks) {
   constexpr int HD = I::HD, KV = I::KV, NQ = I::NQ, SLABS = I::SLABS, NST = I::NST, KC = I::KC;
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t head = (raw + 15u) & ~15u;                  // barriers
-  const uint32_t sQ = (head + 512 + 1023u) & ~1023u;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t sQ = smem_u32(smem_raw);
   const uint32_t ring = sQ + I::Q_BYTES;
+  const uint32_t sX = ring + NST * STAGE;
+  const uint32_t head = sX + I::X_BYTES;                     // barriers
+  if (sQ & 1023u) {
+    if (threadIdx.x == 0) atomicExch(p.status, GA_ST_WAIT_TMEM);
+    return;
+  }
   const uint32_t b_full = head, b_empty = b_full + 8 * NST;  // ring stages
   const uint32_t b_qfull = b_empty + 8 * NST, b_qempty = b_qfull + 8;
   const uint32_t b_s = b_qempty + 8, b_p = b_s + 16;         // [2] scores ready, [2] P ready
@@ -177,11 +304,11 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   const uint32_t b_ofull = b_pv + 8, b_ofree = b_ofull + 16; // [2] O complete / read
   const uint32_t slot_at = b_ofree + 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int MMA_WARP = I::SOFT_WARPS, KV_WARP = MMA_WARP + 1, Q_WARP = KV_WARP + KV_WARPS;
+  constexpr int MMA_WARP = I::SOFT_WARPS, KV_WARP = MMA_WARP + 1, Q_WARP = KV_WARP + I::KV_WARPS;
 
   if (tid == 0) {
-    for (int i = 0; i < NST; ++i) {
-      mbar_init(b_full + 8 * i, 32);
+    for (int i = 0; i < NST / I::EG; ++i) {
+      mbar_init(b_full + 8 * i, 32 * I::EG);
       mbar_init(b_empty + 8 * i, 1);
     }
     mbar_init(b_qfull, Q_WARPS * 32);
@@ -189,9 +316,9 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     mbar_init(b_pv, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(b_s + 8 * i, 1);
-      mbar_init(b_p + 8 * i, TM);
+      mbar_init(b_p + 8 * i, I::SPLIT * 4);
       mbar_init(b_ofull + 8 * i, 1);
-      mbar_init(b_ofree + 8 * i, TM);
+      mbar_init(b_ofree + 8 * i, I::SPLIT * 4);
     }
     mbar_fence_init();
   }
@@ -222,50 +349,50 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
 
   if (warp < I::SOFT_WARPS) {
     // ------------------------------------------------------------------------------------------ softmax, epilogue
-    const int g = warp >> 2;  // query tile
+    regs_up<I::REGS_SOFT>();
+    constexpr int SPLIT = I::SPLIT, KEYS = TK / SPLIT, DIMS = HD / SPLIT;
+    const int g = warp / (4 * SPLIT), half = SPLIT == 2 ? (warp >> 2) & 1 : 0;  // query tile, part of its keys
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tO = tmem + lanes + I::O_COL + g * HD;
+    const uint32_t tO = tmem + lanes + I::O_COL + g * HD + half * DIMS;  // this thread's part of the output dims
+    const uint32_t xm = sX + (g * 2 * TM + row) * 4;                         // [turn or query tile][half][row]
     int n = NQ == 2 ? g : 0;  // running job
     int done = 0;             // items with jobs so far
+    uint32_t turn = 0;
+    auto exchange = [&](float mine) {  // with the thread that has the row's other half
+      const uint32_t at = xm + turn * (2 * TM * 4);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + half * (TM * 4)), "f"(mine) : "memory");
+      named_bar_sync(1 + g, 2 * TM);
+      float other;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(at + (half ^ 1) * (TM * 4)) : "memory");
+      if (I::TURNS == 2) turn ^= 1;  // the slot is written again behind a barrier that its reader has passed
+      return other;
+    };
     for (int x = blockIdx.x; x < items; x += gridDim.x) {
       int b, block, h;
       Req r;
       item_of(x, b, block, h, r);
-      const int rr = block * I::ROWS + g * TM + row;
+      const int rr0 = block * I::ROWS + g * TM + (warp & 3) * 32, rr = rr0 + lane;
       const bool real = rr < r.nq * p.gqa;
       const int tok = rr / p.gqa;
-      const int pos = real ? r.pos0 + tok : -1;
-      const int first = r.pos0 + (block * I::ROWS + g * TM) / p.gqa;  // positions of the tile's first and last row
-      const int last = r.pos0 + (block * I::ROWS + g * TM + TM - 1) / p.gqa;
-      const int lo = p.window >= 0 ? pos - p.window : -(1 << 30);
+      View w;
+      w.pos = real ? r.pos0 + tok : -1;
+      w.lo = p.window >= 0 ? w.pos - p.window : -(1 << 30);
+      w.sinks = p.sinks;
+      w.window = p.window;
+      w.pmin = r.pos0 + rr0 / p.gqa;
+      w.pmax = r.pos0 + (rr0 + 31) / p.gqa;
       const float sl2 = p.scale_log2;
       float ref = -INFINITY, sum = 0.f;
       for (int i = 0; i < r.cnt; ++i, n += NQ) {
         const int buf = n & 1;
-        const uint32_t tS = tmem + lanes + buf * TK;
+        const uint32_t tS = tmem + lanes + buf * TK + half * KEYS;
         wait_or_flag(b_s + 8 * buf, (n >> 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
         __syncwarp();
         fence_after();
-        const int n0 = tile_at(r, i);
-        const bool open = n0 + TK - 1 <= first && (p.window < 0 || n0 >= last - p.window || n0 + TK <= p.sinks);
-        float mx = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32];
-          tmem_ld32(tS + c * 32, v);
-          wait_ld();
-          if (open) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) mx = fmaxf(mx, __uint_as_float(v[k]));
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int key = n0 + c * 32 + k;
-              if (key <= pos && (key >= lo || key < p.sinks)) mx = fmaxf(mx, __uint_as_float(v[k]));
-            }
-          }
-        }
+        const int n0 = tile_at(r, i) + half * KEYS;
+        float mx = part_max<KEYS>(tS, n0, w);
+        if (SPLIT == 2) mx = fmaxf(mx, exchange(mx));
         mx *= sl2;
         bool scale = false;
         float f = 1.f;
@@ -284,7 +411,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             fence_after();
           }
 #pragma unroll 1
-          for (int c = 0; c < HD / 32; ++c) {
+          for (int c = 0; c < DIMS / 32; ++c) {
             uint32_t v[32];
             tmem_ld32(tO + c * 32, v);
             wait_ld();
@@ -293,37 +420,20 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             tmem_st32(tO + c * 32, v);
           }
         }
-        const float mu = ref == -INFINITY ? 0.f : ref;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t v[32], w[16];
-          tmem_ld32(tS + c * 32, v);
-          wait_ld();
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            float e[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float a = fmaf(__uint_as_float(v[k + u]), sl2, -mu);
-              if (!open) {
-                const int key = n0 + c * 32 + k + u;
-                if (!(key <= pos && (key >= lo || key < p.sinks))) a = -INFINITY;
-              }
-              e[u] = ex2(a);
-              part[(k + u) & 3] += e[u];
-            }
-            w[k / 2] = pack16<KV>(e[0], e[1]);
-          }
-          tmem_st16(tS + c * 16, w);
-        }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        sum += part_exp<KV, KEYS>(tS, sl2, ref == -INFINITY ? 0.f : ref, n0, w);
         wait_st();
         fence_before();
-        mbar_arrive(b_p + 8 * buf);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_p + 8 * buf);
+      }
+      if (SPLIT == 2) {
+        if (I::TURNS == 1) named_bar_sync(1 + g, 2 * TM);
+        sum += exchange(sum);
+        if (I::TURNS == 1) named_bar_sync(1 + g, 2 * TM);
       }
       const int qrow = r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
-      uint8_t* dst = static_cast<uint8_t*>(p.out) + (static_cast<long long>(qrow) * p.o_s0 + static_cast<long long>(qh) * p.o_s1) * 2;
+      uint8_t* dst = static_cast<uint8_t*>(p.out) +
+                     (static_cast<long long>(qrow) * p.o_s0 + static_cast<long long>(qh) * p.o_s1 + half * DIMS) * 2;
       const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
       const float inv = sum == 0.f ? 0.f : vds / sum;
       if (r.cnt > 0) {
@@ -332,7 +442,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         fence_after();
       }
 #pragma unroll 1
-      for (int c = 0; c < HD / 32; ++c) {
+      for (int c = 0; c < DIMS / 32; ++c) {
         uint32_t v[32];
         if (r.cnt > 0) {
           tmem_ld32(tO + c * 32, v);
@@ -341,24 +451,27 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         if (real) {
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
-            uint2 w = make_uint2(0u, 0u);
+            uint2 o = make_uint2(0u, 0u);
             if (r.cnt > 0 && sum != 0.f) {
-              w.x = pack16<KV>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
-              w.y = pack16<KV>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
+              o.x = pack16<KV>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
+              o.y = pack16<KV>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
             }
-            *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = w;
+            *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = o;
           }
         }
       }
-      if (real && p.lse)
+      if (real && half == 0 && p.lse)
         p.lse[static_cast<long long>(qh) * p.total_q + qrow] = sum == 0.f ? -INFINITY : (ref + lg2(sum)) * 0.6931471805599453f;
       if (r.cnt > 0) {
         fence_before();
-        mbar_arrive(b_ofree + 8 * g);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_ofree + 8 * g);
         ++done;
       }
     }
-  } else if (warp == MMA_WARP) {
+  } else {
+  regs_down<I::REGS_REST>();
+  if (warp == MMA_WARP) {
     // -------------------------------------------------------------------------------------------------- MMA issue
     if (lane == 0) {
       const uint32_t id_qk = instr_desc(KV, TM, TK, 0), id_pv = instr_desc(KV, TM, HD, 1);
@@ -366,9 +479,11 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       const uint64_t dk = smem_desc(ring, 16, 1024), dv = smem_desc(ring, KC * 128, 1024);
       int rp = 0, use = 0;  // ring position of the next stage and how often the ring went round
       int n = 0, done = 0;  // first job of the item, items with jobs so far
+      // column of P's key `key` in its buffer: every part of the keys lies over the front of its own scores
+      auto p_col = [](int key) { return key / (TK / I::SPLIT) * (TK / I::SPLIT) + key % (TK / I::SPLIT) / 2; };
       auto take = [&]() {   // the next stage in ring order, filled
         const int at = rp;
-        wait_or_flag(b_full + 8 * at, use & 1, failed, p.status, GA_ST_WAIT_FULL);
+        if (at % I::EG == 0) wait_or_flag(b_full + 8 * (at / I::EG), use & 1, failed, p.status, GA_ST_WAIT_FULL);
         if (++rp == NST) rp = 0, ++use;
         return at;
       };
@@ -395,7 +510,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           commit(b_s + 8 * buf);
           if (NQ == 1 || g == 1)
 #pragma unroll
-            for (int s = 0; s < SLABS; ++s) commit(b_empty + 8 * ks[s]);
+            for (int s = 0; s < SLABS; s += I::EG) commit(b_empty + 8 * (ks[s] / I::EG));
           if (j == jobs - 1) commit(b_qempty);
         };
         wait_or_flag(b_qfull, done & 1, failed, p.status, GA_ST_WAIT_FULL);
@@ -417,12 +532,12 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           for (int s = 0; s < SLABS; ++s)
 #pragma unroll
             for (int k = 0; k < KC / 16; ++k)
-              mma_ts(tmem + I::O_COL + g * HD, tmem + buf * TK + s * (KC / 2) + k * 8, dv + ((vs[s] * STAGE + k * 2048) >> 4), id_pv,
+              mma_ts(tmem + I::O_COL + g * HD, tmem + buf * TK + p_col(s * KC + k * 16), dv + ((vs[s] * STAGE + k * 2048) >> 4), id_pv,
                      !opens || s > 0 || k > 0);
           if (NQ == 1) commit(b_pv);
           if (NQ == 1 || g == 1)
 #pragma unroll
-            for (int s = 0; s < SLABS; ++s) commit(b_empty + 8 * vs[s]);
+            for (int s = 0; s < SLABS; s += I::EG) commit(b_empty + 8 * (vs[s] / I::EG));
           if (j >= jobs - NQ) commit(b_ofull + 8 * g);
           if (j + 2 < jobs) qk(j + 2);
         }
@@ -438,18 +553,19 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     int pending = -1;    // stage filled by cp.async that are still in flight
     auto signal = [&]() {
       fence_proxy_async();
-      mbar_arrive(b_full + 8 * (pending % NST));
+      mbar_arrive(b_full + 8 * (pending % NST / I::EG));
       pending = -1;
     };
     auto stage_for = [&](const Req& r, int b, int h, int tile, int part, bool is_v) {
-      if (q % KV_WARPS == w) {
+      if (q % I::KV_WARPS == w) {
         const int at = q % NST, turn = q / NST;
-        if (turn > 0 && !failed && !mbar_test_wait(b_empty + 8 * at, (turn - 1) & 1)) {
+        const uint32_t empty = b_empty + 8 * (at / I::EG);
+        if (turn > 0 && !failed && !mbar_test_wait(empty, (turn - 1) & 1)) {
           if (pending >= 0) {  // nothing may wait for what this warp holds back
             cp_async_wait<0>();
             signal();
           }
-          wait_or_flag(b_empty + 8 * at, (turn - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
+          wait_or_flag(empty, (turn - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
         }
         failed = __any_sync(0xffffffffu, failed);
         const uint32_t dst = ring + at * STAGE;
@@ -469,32 +585,8 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             }
           }
         }
-        const uint8_t* base = (is_v ? p.v + h * p.v_s2 : p.k + h * p.k_s2 + part * 128);
-        const long long s0 = is_v ? p.v_s0 : p.k_s0, s1 = is_v ? p.v_s1 : p.k_s1;
-        if (!is_v) {
-          // 128 keys x 64 dims: eight chunks a key, four keys an instruction
-          const int c = lane & 7;
-#pragma unroll
-          for (int it = 0; it < 32; ++it) {
-            const int key = it * 4 + (lane >> 3);
-            const int pg = __shfl_sync(0xffffffffu, page[it / 8], key & 31);
-            const bool real = pg >= 0;
-            const uint8_t* src = base + (real ? pg * s0 + ((n0 + key) & p.page_mask) * s1 : 0) + c * 16;
-            cp_async_16_or_zero(dst + key * 128 + ((c ^ (key & 7)) << 4), src, real);
-          }
-        } else {
-          // KC keys x HD dims: HD / 8 chunks a key
-          constexpr int CPK = HD / 8, KPI = 32 / CPK;  // chunks a key, keys an instruction
-          const int c = lane % CPK;
-#pragma unroll
-          for (int it = 0; it < KC / KPI; ++it) {
-            const int key = it * KPI + lane / CPK;
-            const int pg = __shfl_sync(0xffffffffu, page[it * KPI / 32], key & 31);
-            const bool real = pg >= 0;
-            const uint8_t* src = base + (real ? pg * s0 + ((n0 + key) & p.page_mask) * s1 : 0) + c * 16;
-            cp_async_16_or_zero(dst + (c >> 3) * (KC * 128) + key * 128 + (((c & 7) ^ (key & 7)) << 4), src, real);
-          }
-        }
+        if (!is_v) gather<8, TK>(dst, p.k + h * p.k_s2 + part * 128, p.k_s0, p.k_s1, n0, p.page_shift, p.page_mask, page, lane);
+        else gather<HD / 8, KC>(dst, p.v + h * p.v_s2, p.v_s0, p.v_s1, n0, p.page_shift, p.page_mask, page, lane);
         cp_async_commit();
         if (pending >= 0) {
           cp_async_wait<1>();
@@ -520,7 +612,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       cp_async_wait<0>();
       signal();
     }
-  } else {
+  } else if (warp < Q_WARP + Q_WARPS) {
     // ---------------------------------------------------------------------------------------------------- Q gather
     const int w = warp - Q_WARP;
     int done = 0;
@@ -554,6 +646,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       mbar_arrive(b_qfull);
       ++done;
     }
+  }
   }
   // Every MMA has completed where its result was waited for: the softmax groups waited for O of the last item.
   fence_before();

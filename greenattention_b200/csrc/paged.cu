@@ -32,6 +32,9 @@ int limits() {
 
 template <class I>
 int limits_tc() {
+  cudaFuncAttributes at;
+  GA_TRY(cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(ga::paged::tc::attn_paged_tc_kernel<I>)));
+  if (at.numRegs < I::REGS) return fail("attn_paged_tc_kernel: built with %d registers a thread, its split needs %d", at.numRegs, I::REGS);
   GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(ga::paged::tc::attn_paged_tc_kernel<I>),
                               cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
   return 0;
