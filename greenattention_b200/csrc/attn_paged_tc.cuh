@@ -31,7 +31,6 @@ namespace tc {
 constexpr int TM = 128;          // query rows of a tile = tensor memory lanes
 constexpr int TK = 128;          // keys of a tile
 constexpr int STAGE = 16384;
-constexpr int Q_WARPS = 2;
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
 
 template <int HD_, int KV_>
@@ -46,8 +45,13 @@ struct TcInst {
   static constexpr int EG = SLABS < 2 ? SLABS : 2;  // stages that are filled and released together
   static constexpr int SPLIT = 2;                   // threads that share a row
   static constexpr int SOFT_WARPS = 4 * NQ * SPLIT;
-  static constexpr int KV_WARPS = NQ == 1 ? 8 : 4;
-  static constexpr int WARPS = (SOFT_WARPS + 1 + KV_WARPS + Q_WARPS + 3) / 4 * 4;  // whole warpgroups
+  // Gathering warps. A stage is always filled by the same warp: one that waits for use u of a stage to be released has
+  // filled that use itself, so the barrier cannot be a whole phase behind the wait (stages are not released in ring order
+  // when K and V are released by different lanes, and a parity cannot tell phase u - 2 from phase u).
+  static constexpr int KV_WARPS = NST % 5 == 0 ? 5 : 4;
+  static constexpr int Q_WARPS = NQ == 1 ? 4 : 6 - KV_WARPS;
+  static_assert(NST % KV_WARPS == 0, "gathering warps");
+  static constexpr int WARPS = (SOFT_WARPS + 2 + KV_WARPS + Q_WARPS + 3) / 4 * 4;  // whole warpgroups
   static constexpr int NT = WARPS * 32;
   // Registers a thread: what the block is launched with (limit of the launch bounds), and its split between the softmax
   // warps and the others. The shares add up to no more than the launch's.
@@ -300,21 +304,21 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   const uint32_t b_full = head, b_empty = b_full + 8 * NST;  // ring stages
   const uint32_t b_qfull = b_empty + 8 * NST, b_qempty = b_qfull + 8;
   const uint32_t b_s = b_qempty + 8, b_p = b_s + 16;         // [2] scores ready, [2] P ready
-  const uint32_t b_pv = b_p + 16;                            // PV of a job done
-  const uint32_t b_ofull = b_pv + 8, b_ofree = b_ofull + 16; // [2] O complete / read
+  const uint32_t b_pv = b_p + 16;                            // NQ 1: PV out of a buffer done
+  const uint32_t b_ofull = b_pv + 16, b_ofree = b_ofull + 16; // [2] O complete / read
   const uint32_t slot_at = b_ofree + 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int MMA_WARP = I::SOFT_WARPS, KV_WARP = MMA_WARP + 1, Q_WARP = KV_WARP + I::KV_WARPS;
+  constexpr int MMA_WARP = I::SOFT_WARPS, KV_WARP = MMA_WARP + 2, Q_WARP = KV_WARP + I::KV_WARPS;
 
   if (tid == 0) {
     for (int i = 0; i < NST / I::EG; ++i) {
       mbar_init(b_full + 8 * i, 32 * I::EG);
       mbar_init(b_empty + 8 * i, 1);
     }
-    mbar_init(b_qfull, Q_WARPS * 32);
+    mbar_init(b_qfull, I::Q_WARPS * 32);
     mbar_init(b_qempty, 1);
-    mbar_init(b_pv, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(b_pv + 8 * i, 1);
       mbar_init(b_s + 8 * i, 1);
       mbar_init(b_p + 8 * i, I::SPLIT * 4);
       mbar_init(b_ofull + 8 * i, 1);
@@ -406,7 +410,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           // NQ == 1: the PV before this job's may still be adding to O (it is waited for only here, where the barrier
           // is at most one phase ahead of what is waited for)
           if (NQ == 1) {
-            wait_or_flag(b_pv, (n - 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
+            wait_or_flag(b_pv + 8 * ((n - 1) & 1), ((n - 1) >> 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
             __syncwarp();
             fence_after();
           }
@@ -471,77 +475,101 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     }
   } else {
   regs_down<I::REGS_REST>();
-  if (warp == MMA_WARP) {
-    // -------------------------------------------------------------------------------------------------- MMA issue
-    if (lane == 0) {
+  if (warp < KV_WARP) {
+    // ------------------------------------------------------------------------------------------------- MMA issue
+    // NQ 2: one lane issues for both query tiles in turn (a lane for each measured 10 % slower). NQ 1: one lane for the QK
+    // MMAs, one for the PV MMAs; a QK waits for the PV two tiles before, whose P it overwrites.
+    const int role = warp - MMA_WARP;
+    if (lane == 0 && (NQ == 1 || role == 0)) {
       const uint32_t id_qk = instr_desc(KV, TM, TK, 0), id_pv = instr_desc(KV, TM, HD, 1);
       const uint64_t dq = smem_desc(sQ, 16, 1024);
       const uint64_t dk = smem_desc(ring, 16, 1024), dv = smem_desc(ring, KC * 128, 1024);
-      int rp = 0, use = 0;  // ring position of the next stage and how often the ring went round
-      int n = 0, done = 0;  // first job of the item, items with jobs so far
       // column of P's key `key` in its buffer: every part of the keys lies over the front of its own scores
       auto p_col = [](int key) { return key / (TK / I::SPLIT) * (TK / I::SPLIT) + key % (TK / I::SPLIT) / 2; };
-      auto take = [&]() {   // the next stage in ring order, filled
-        const int at = rp;
-        if (at % I::EG == 0) wait_or_flag(b_full + 8 * (at / I::EG), use & 1, failed, p.status, GA_ST_WAIT_FULL);
-        if (++rp == NST) rp = 0, ++use;
-        return at;
+      int unit = 0;         // K and V tiles of the items before, in ring order
+      int n = 0, done = 0;  // NQ 1: first job of the item; items with jobs so far
+      auto qk = [&](int u, int g, int buf, bool release) {
+        int at = u * SLABS % NST;
+        uint32_t par = (u * SLABS / NST) & 1;
+#pragma unroll
+        for (int s = 0; s < SLABS; s += I::EG) {
+          wait_or_flag(b_full + 8 * (at / I::EG), par, failed, p.status, GA_ST_WAIT_FULL);
+          if (failed) return;
+          fence_after();
+#pragma unroll
+          for (int e = 0; e < I::EG; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mma_ss(tmem + buf * TK, dq + (((g * SLABS + s + e) * STAGE + k * 32) >> 4), dk + (((at + e) * STAGE + k * 32) >> 4), id_qk, s + e > 0 || k > 0);
+          if (s + I::EG == SLABS) commit(b_s + 8 * buf);
+          if (release) commit(b_empty + 8 * (at / I::EG));
+          at += I::EG;
+          if (at == NST) at = 0, par ^= 1;
+        }
+      };
+      auto pv = [&](int u, int g, int buf, bool opens, bool release) {
+        int at = u * SLABS % NST;
+        uint32_t par = (u * SLABS / NST) & 1;
+#pragma unroll
+        for (int s = 0; s < SLABS; s += I::EG) {
+          wait_or_flag(b_full + 8 * (at / I::EG), par, failed, p.status, GA_ST_WAIT_FULL);
+          if (failed) return;
+          fence_after();
+#pragma unroll
+          for (int e = 0; e < I::EG; ++e)
+#pragma unroll
+            for (int k = 0; k < KC / 16; ++k)
+              mma_ts(tmem + I::O_COL + g * HD, tmem + buf * TK + p_col((s + e) * KC + k * 16), dv + (((at + e) * STAGE + k * 2048) >> 4), id_pv,
+                     !opens || s + e > 0 || k > 0);
+          if (release) commit(b_empty + 8 * (at / I::EG));
+          at += I::EG;
+          if (at == NST) at = 0, par ^= 1;
+        }
       };
       for (int x = blockIdx.x; x < items && !failed; x += gridDim.x) {
         int b, block, h;
         Req r;
         item_of(x, b, block, h, r);
         if (r.cnt == 0) continue;
-        const int jobs = r.cnt * NQ;
-        int ks[SLABS], vs[SLABS];
-        auto qk = [&](int j) {
-          const int g = NQ == 2 ? j & 1 : 0, buf = (n + j) & 1;
-          if (NQ == 1 || g == 0) {
-#pragma unroll
-            for (int s = 0; s < SLABS; ++s) ks[s] = take();
-            fence_after();
-          }
-          if (failed) return;
-#pragma unroll
-          for (int s = 0; s < SLABS; ++s)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              mma_ss(tmem + buf * TK, dq + (((g * SLABS + s) * STAGE + k * 32) >> 4), dk + ((ks[s] * STAGE + k * 32) >> 4), id_qk, s > 0 || k > 0);
-          commit(b_s + 8 * buf);
-          if (NQ == 1 || g == 1)
-#pragma unroll
-            for (int s = 0; s < SLABS; s += I::EG) commit(b_empty + 8 * (ks[s] / I::EG));
-          if (j == jobs - 1) commit(b_qempty);
-        };
-        wait_or_flag(b_qfull, done & 1, failed, p.status, GA_ST_WAIT_FULL);
-        fence_after();
-        qk(0);
-        if (jobs > 1) qk(1);
-        for (int j = 0; j < jobs && !failed; ++j) {
-          const int g = NQ == 2 ? j & 1 : 0, buf = (n + j) & 1;
-          const bool opens = j < NQ;
-          if (NQ == 1 || g == 0) {
-#pragma unroll
-            for (int s = 0; s < SLABS; ++s) vs[s] = take();
-          }
-          if (opens && done > 0) wait_or_flag(b_ofree + 8 * g, (done - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
-          wait_or_flag(b_p + 8 * buf, ((n + j) >> 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
-          if (failed) break;
+        if (NQ == 2) {
+          wait_or_flag(b_qfull, done & 1, failed, p.status, GA_ST_WAIT_FULL);
           fence_after();
-#pragma unroll
-          for (int s = 0; s < SLABS; ++s)
-#pragma unroll
-            for (int k = 0; k < KC / 16; ++k)
-              mma_ts(tmem + I::O_COL + g * HD, tmem + buf * TK + p_col(s * KC + k * 16), dv + ((vs[s] * STAGE + k * 2048) >> 4), id_pv,
-                     !opens || s > 0 || k > 0);
-          if (NQ == 1) commit(b_pv);
-          if (NQ == 1 || g == 1)
-#pragma unroll
-            for (int s = 0; s < SLABS; s += I::EG) commit(b_empty + 8 * (vs[s] / I::EG));
-          if (j >= jobs - NQ) commit(b_ofull + 8 * g);
-          if (j + 2 < jobs) qk(j + 2);
+          qk(unit, 0, 0, false);
+          qk(unit, 1, 1, true);
+          if (r.cnt == 1 && !failed) commit(b_qempty);
+          for (int j = 0; j < 2 * r.cnt && !failed; ++j) {
+            const int g = j & 1, i = j >> 1;
+            if (i == 0 && done > 0) wait_or_flag(b_ofree + 8 * g, (done - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
+            wait_or_flag(b_p + 8 * g, (n + i) & 1, failed, p.status, GA_ST_WAIT_FULL);
+            if (failed) break;
+            fence_after();
+            pv(unit + 2 * i + 1, g, g, i == 0, g == 1);
+            if (i == r.cnt - 1) commit(b_ofull + 8 * g);
+            if (i + 1 < r.cnt) qk(unit + 2 * i + 2, g, g, g == 1);
+            if (j == 2 * r.cnt - 3) commit(b_qempty);
+          }
+        } else if (role == 0) {
+          wait_or_flag(b_qfull, done & 1, failed, p.status, GA_ST_WAIT_FULL);
+          fence_after();
+          for (int i = 0; i < r.cnt && !failed; ++i) {
+            const int buf = (n + i) & 1;
+            if (n + i >= 2) wait_or_flag(b_pv + 8 * buf, ((n + i - 2) >> 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
+            qk(unit + (i == 0 ? 0 : 2 * i - 1), 0, buf, true);
+          }
+          if (!failed) commit(b_qempty);
+        } else {
+          for (int i = 0; i < r.cnt && !failed; ++i) {
+            const int buf = (n + i) & 1;
+            if (i == 0 && done > 0) wait_or_flag(b_ofree, (done - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
+            wait_or_flag(b_p + 8 * buf, ((n + i) >> 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
+            fence_after();
+            pv(unit + (i == r.cnt - 1 ? 2 * i + 1 : 2 * i + 2), 0, buf, i == 0, true);
+            commit(b_pv + 8 * buf);
+          }
+          if (!failed) commit(b_ofull);
         }
-        n += jobs;
+        n += r.cnt;
+        unit += 2 * r.cnt;
         ++done;
       }
     }
@@ -558,17 +586,6 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     };
     auto stage_for = [&](const Req& r, int b, int h, int tile, int part, bool is_v) {
       if (q % I::KV_WARPS == w) {
-        const int at = q % NST, turn = q / NST;
-        const uint32_t empty = b_empty + 8 * (at / I::EG);
-        if (turn > 0 && !failed && !mbar_test_wait(empty, (turn - 1) & 1)) {
-          if (pending >= 0) {  // nothing may wait for what this warp holds back
-            cp_async_wait<0>();
-            signal();
-          }
-          wait_or_flag(empty, (turn - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
-        }
-        failed = __any_sync(0xffffffffu, failed);
-        const uint32_t dst = ring + at * STAGE;
         const int n0 = tile_at(r, tile) + (is_v ? part * KC : 0);
         constexpr int MOST = 128 / 32;
         int page[MOST];
@@ -585,6 +602,17 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             }
           }
         }
+        const int at = q % NST, turn = q / NST;
+        const uint32_t empty = b_empty + 8 * (at / I::EG);
+        if (turn > 0 && !failed && !mbar_test_wait(empty, (turn - 1) & 1)) {
+          if (pending >= 0) {  // nothing may wait for what this warp holds back
+            cp_async_wait<0>();
+            signal();
+          }
+          wait_or_flag(empty, (turn - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
+        }
+        failed = __any_sync(0xffffffffu, failed);
+        const uint32_t dst = ring + at * STAGE;
         if (!is_v) gather<8, TK>(dst, p.k + h * p.k_s2 + part * 128, p.k_s0, p.k_s1, n0, p.page_shift, p.page_mask, page, lane);
         else gather<HD / 8, KC>(dst, p.v + h * p.v_s2, p.v_s0, p.v_s1, n0, p.page_shift, p.page_mask, page, lane);
         cp_async_commit();
@@ -612,7 +640,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       cp_async_wait<0>();
       signal();
     }
-  } else if (warp < Q_WARP + Q_WARPS) {
+  } else if (warp < Q_WARP + I::Q_WARPS) {
     // ---------------------------------------------------------------------------------------------------- Q gather
     const int w = warp - Q_WARP;
     int done = 0;
@@ -625,7 +653,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       failed = __any_sync(0xffffffffu, failed);
       const int rows = r.nq * p.gqa - block * I::ROWS;
       const int c = lane & 7;
-      for (int part = w; part < NQ * 4; part += Q_WARPS) {  // 32 rows
+      for (int part = w; part < NQ * 4; part += I::Q_WARPS) {  // 32 rows
         const int mine = part * 32 + lane;
         const int rr = block * I::ROWS + mine, tok = rr / p.gqa;
         const long long off = mine < rows ? static_cast<long long>(r.q0 + tok) * p.q_s0 + static_cast<long long>(h * p.gqa + rr - tok * p.gqa) * p.q_s1 : -1;
