@@ -399,6 +399,15 @@ int device(int* dev, int* sm) {
   return 0;
 }
 void launches(int n) { g_launches = n; }
+bool encode_map(CUtensorMap* map, const void* base, int hd, int page, int kvh, int pages, long long s_tok, long long s_head,
+                long long s_page, int box_tok) {
+  if (!g_encode) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)page, (cuuint64_t)kvh, (cuuint64_t)pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)s_tok, (cuuint64_t)s_head, (cuuint64_t)s_page};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_tok, 1, 1}, estr[4] = {1, 1, 1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 }  // namespace api
 }  // namespace ga
 

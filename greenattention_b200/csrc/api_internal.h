@@ -2,6 +2,7 @@
 // count, and each unit's part of ga_init().
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <cstring>
@@ -12,6 +13,9 @@ namespace api {
 
 int fail(const char* fmt, ...);         // records the text for ga_last_error(), returns 1
 int device(int* dev, int* sm);          // current device, which ga_init() has prepared, and its SMs
+// Tensor map of a 16-bit pool for boxes of 64 dims x `box` tokens of one head and page, 128-byte swizzle; false: it has none.
+bool encode_map(CUtensorMap* map, const void* base, int hd, int page, int kvh, int pages, long long s_tok, long long s_head,
+                long long s_page, int box);
 void launches(int n);                   // what ga_last_launch_count() reports
 int init_paged();                       // paged.cu: shared memory limits on the current device
 int init_pages();                       // pages.cu: the same

@@ -14,9 +14,10 @@
 //   * The row's reference maximum moves only when a tile exceeds it by more than 2^8 (P stays below 256, exact in the
 //     sums; the 16-bit rounding of P is relative), so O is rescaled in tensor memory in few tiles.
 //   * K and V come through one ring of 16 KB stages in the order in which the MMAs use them: a K stage is 128 keys x 64
-//     dims, a V stage 8192 / head_dim keys x all dims. Stages are filled with 16-byte cp.async (any page size, stride and
-//     alignment of 16 bytes; rows no query of the item sees, released pages among them, are filled with zeros), in the
-//     128-byte swizzle that the MMA descriptors name.
+//     dims, a V stage 8192 / head_dim keys x all dims, in the 128-byte swizzle that the MMA descriptors name. Where every
+//     key of a stage is seen by some query, TMA boxes of up to a page each fill it (pages of 8 tokens and more); edges of
+//     what is seen and smaller pages are filled with 16-byte cp.async, rows no query of the item sees (released pages
+//     among them) with zeros.
 // Tiles are the sinks' first, then the run that ends with the item's last visible key (Req). Items come from a list that a
 // small kernel lays out, later row blocks of a request first (they see more keys), all kv heads of a block side by side
 // (they share pages).
@@ -95,6 +96,9 @@ template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ void mbar_expect_tx_only(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -290,7 +294,8 @@ __device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, int 
 }
 
 template <class I>
-__global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_constant__ PagedDev p, const int* count, const int2* blocks) {
+__global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_constant__ PagedDev p, const int* count, const int2* blocks,
+                                                                 const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int boxes) {
   constexpr int HD = I::HD, KV = I::KV, NQ = I::NQ, SLABS = I::SLABS, NST = I::NST, KC = I::KC;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t sQ = smem_u32(smem_raw);
@@ -584,12 +589,47 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       mbar_arrive(b_full + 8 * (pending % NST / I::EG));
       pending = -1;
     };
+    auto wait_stage = [&](int at, int turn) {
+      const uint32_t empty = b_empty + 8 * (at / I::EG);
+      if (turn > 0 && !failed && !mbar_test_wait(empty, (turn - 1) & 1)) {
+        if (pending >= 0) {  // nothing may wait for what this warp holds back
+          cp_async_wait<0>();
+          signal();
+        }
+        wait_or_flag(empty, (turn - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
+      }
+      failed = __any_sync(0xffffffffu, failed);
+    };
     auto stage_for = [&](const Req& r, int b, int h, int tile, int part, bool is_v) {
       if (q % I::KV_WARPS == w) {
         const int n0 = tile_at(r, tile) + (is_v ? part * KC : 0);
+        const int keys = is_v ? KC : TK;
+        // Inside the run (or the sinks) every key is a real one: whole boxes of pages by TMA.
+        if (boxes && n0 + keys <= r.kend && (n0 >= r.lower || n0 + keys <= p.sinks)) {
+          const int box = min(p.page_mask + 1, keys), nb = keys / box;
+          const int k = lane % nb, slab = lane / nb;
+          const int at_key = n0 + k * box;
+          const int pg = p.pt[b * p.pt_s0 + (at_key >> p.page_shift) * p.pt_s1];
+          const int at = q % NST, turn = q / NST;
+          wait_stage(at, turn);
+          if (__all_sync(0xffffffffu, pg >= 0 && pg < p.num_pages)) {
+            const uint32_t full = b_full + 8 * (at / I::EG);
+            if (lane == 0) mbar_expect_tx_only(full, STAGE);
+            __syncwarp();
+            if (slab < (is_v ? SLABS : 1))
+              tma_load_4d(ring + at * STAGE + slab * (KC * 128) + k * box * 128, is_v ? &vmap : &kmap, full, (is_v ? slab : part) * 64,
+                          at_key & p.page_mask, h, pg);
+            if (pending >= 0) {
+              cp_async_wait<0>();
+              signal();
+            }
+            mbar_arrive(full);
+            ++q;
+            return;
+          }
+        }
         constexpr int MOST = 128 / 32;
         int page[MOST];
-        const int keys = is_v ? KC : TK;
 #pragma unroll
         for (int u = 0; u < MOST; ++u) {
           const int n = n0 + u * 32 + lane;
@@ -603,15 +643,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           }
         }
         const int at = q % NST, turn = q / NST;
-        const uint32_t empty = b_empty + 8 * (at / I::EG);
-        if (turn > 0 && !failed && !mbar_test_wait(empty, (turn - 1) & 1)) {
-          if (pending >= 0) {  // nothing may wait for what this warp holds back
-            cp_async_wait<0>();
-            signal();
-          }
-          wait_or_flag(empty, (turn - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
-        }
-        failed = __any_sync(0xffffffffu, failed);
+        wait_stage(at, turn);
         const uint32_t dst = ring + at * STAGE;
         if (!is_v) gather<8, TK>(dst, p.k + h * p.k_s2 + part * 128, p.k_s0, p.k_s1, n0, p.page_shift, p.page_mask, page, lane);
         else gather<HD / 8, KC>(dst, p.v + h * p.v_s2, p.v_s0, p.v_s1, n0, p.page_shift, p.page_mask, page, lane);

@@ -1,5 +1,8 @@
 // C ABI of the attention over 16-bit and e4m3 paged caches with first tokens kept visible (attn_paged.cuh): argument
 // checks, choice of the instance, launches.
+#include <mutex>
+#include <vector>
+
 #include "../../include/green_attention.h"
 #include "api_internal.h"
 #include "attn_paged.cuh"
@@ -30,6 +33,37 @@ int limits() {
   return 0;
 }
 
+// Tensor maps of paged pools [pages, page, kv_heads, head_dim] of 16-bit values, dimensions as (dim, token, head, page), for
+// boxes of 64 dims x `box` tokens. A map is a function of its key; the few last ones are kept.
+struct MapKey {
+  const void* base;
+  long long s_page, s_tok, s_head;
+  int pages, page, kvh, hd, box, pad;
+};
+struct MapEntry {
+  MapKey key;
+  CUtensorMap map;
+};
+std::mutex g_maps_mu;
+std::vector<MapEntry> g_maps;
+
+bool pool_map(const MapKey& key, CUtensorMap* out) {
+  std::lock_guard<std::mutex> lock(g_maps_mu);
+  for (const MapEntry& e : g_maps)
+    if (std::memcmp(&e.key, &key, sizeof(MapKey)) == 0) {
+      *out = e.map;
+      return true;
+    }
+  MapEntry e;
+  std::memset(&e, 0, sizeof(e));
+  e.key = key;
+  if (!ga::api::encode_map(&e.map, key.base, key.hd, key.page, key.kvh, key.pages, key.s_tok, key.s_head, key.s_page, key.box)) return false;
+  if (g_maps.size() >= 64) g_maps.erase(g_maps.begin());
+  g_maps.push_back(e);
+  *out = e.map;
+  return true;
+}
+
 template <class I>
 int limits_tc() {
   cudaFuncAttributes at;
@@ -53,8 +87,24 @@ int run_tc(Launch& a, size_t ws_bytes) {
   int2* list = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(d.prefix) + 256);
   GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_prompts_kernel<I::ROWS>, dim3(1), dim3(1024), 0, a.st, d, count, list));
   const long long items = blocks * d.kvh;
+  CUtensorMap maps[2];
+  std::memset(maps, 0, sizeof(maps));
+  const int page = d.page_mask + 1;
+  bool boxes = page >= 8 && d.num_pages > 0;
+  if (boxes) {
+    MapKey kk, vk;
+    std::memset(&kk, 0, sizeof(kk));
+    kk.base = d.k, kk.s_page = d.k_s0, kk.s_tok = d.k_s1, kk.s_head = d.k_s2;
+    kk.pages = d.num_pages, kk.page = page, kk.kvh = d.kvh, kk.hd = I::HD;
+    kk.box = page < ga::paged::tc::TK ? page : ga::paged::tc::TK;
+    vk = kk;
+    vk.base = d.v, vk.s_page = d.v_s0, vk.s_tok = d.v_s1, vk.s_head = d.v_s2;
+    vk.box = page < I::KC ? page : I::KC;
+    boxes = pool_map(kk, &maps[0]) && pool_map(vk, &maps[1]);  // strides that a map cannot hold: without
+  }
   GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(static_cast<unsigned>(items < a.sm ? items : a.sm)), dim3(I::NT),
-                                I::SMEM, a.st, d, const_cast<const int*>(count), const_cast<const int2*>(list)));
+                                I::SMEM, a.st, d, const_cast<const int*>(count), const_cast<const int2*>(list), maps[0], maps[1],
+                                static_cast<int>(boxes)));
   ga::api::launches(2);
   return 0;
 }
