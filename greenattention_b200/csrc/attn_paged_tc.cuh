@@ -18,7 +18,8 @@
 //     key of a stage is seen by some query, TMA boxes of up to a page each fill it (pages of 8 tokens and more); edges of
 //     what is seen and smaller pages are filled with 16-byte cp.async, rows no query of the item sees (released pages
 //     among them) with zeros.
-// Tiles are the sinks' first, then the run that ends with the item's last visible key (Req). Items come from a list that a
+// Keys are taken in groups of 32: the sinks' groups, then those of the run that ends with the item's last visible key (Req);
+// a tile is the next four, so a few first tokens cost 32 keys of a tile and not one of their own. Items come from a list that a
 // small kernel lays out, later row blocks of a request first (they see more keys), all kv heads of a block side by side
 // (they share pages).
 #pragma once
@@ -31,6 +32,7 @@ namespace tc {
 
 constexpr int TM = 128;          // query rows of a tile = tensor memory lanes
 constexpr int TK = 128;          // keys of a tile
+constexpr int GK = 32;           // keys of a group
 constexpr int STAGE = 16384;
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
 
@@ -145,13 +147,14 @@ __device__ __forceinline__ void wait_or_flag(uint32_t bar, uint32_t parity, bool
 }
 
 // One warp fills a stage with KEYS keys of CPK 16-byte chunks each, in slabs of eight chunks (128 bytes a key), swizzled by
-// key. page[u] is the page of key u * 32 + lane, or -1 for a row of zeros. Its own instruction stream is what a stage costs
+// key. n0[u] is the first token of the stage's group u, page[u]
+// the page of its token `lane`, or -1 for a row of zeros. Its own instruction stream is what a stage costs
 // here (32 copies a lane), so a copy is its address step and little else: within 32 keys of one page the source advances
 // by a constant, and the swizzle of the destination is a constant flipped in. Smaller pages and edges pass each row's
 // offset from the lane that looked it up.
 template <int CPK, int KEYS>
-__device__ __forceinline__ void gather(uint32_t dst, const uint8_t* base, long long s0, long long s1, int n0, int page_shift, int page_mask,
-                                       const int (&page)[4], int lane) {
+__device__ __forceinline__ void gather(uint32_t dst, const uint8_t* base, long long s0, long long s1, const int (&n0)[4], int page_shift,
+                                       int page_mask, const int (&page)[4], int lane) {
   constexpr int KPI = 32 / CPK;  // keys an instruction
   const int c = lane % CPK, k0 = lane / CPK;
   const uint32_t d0 = (c >> 3) * (KEYS * 128) + k0 * 128 + (((c ^ k0) & 7) << 4);
@@ -159,14 +162,14 @@ __device__ __forceinline__ void gather(uint32_t dst, const uint8_t* base, long l
   const long long step = s1 * KPI;
 #pragma unroll
   for (int u = 0; u < (KEYS + 31) / 32; ++u) {
-    const int tok = (n0 + u * 32) & page_mask;
+    const int tok = n0[u] & page_mask;
     if (page_shift >= 5 && __all_sync(0xffffffffu, page[u] >= 0)) {
       const uint8_t* src = base + page[u] * s0 + (tok + k0) * s1;
 #pragma unroll
       for (int i = 0; i < CPK; ++i, src += step)
         cp_async_16(dst + (u * 32 + i * KPI) * 128 + (d0 ^ (((i * KPI) & 7) << 4)), src);
     } else {
-      const long long off = page[u] >= 0 ? page[u] * s0 + ((n0 + u * 32 + lane) & page_mask) * s1 : -1;
+      const long long off = page[u] >= 0 ? page[u] * s0 + ((n0[u] + lane) & page_mask) * s1 : -1;
 #pragma unroll 4
       for (int i = 0; i < CPK; ++i) {
         const long long o = __shfl_sync(0xffffffffu, off, i * KPI + k0);
@@ -237,19 +240,19 @@ __device__ __forceinline__ uint32_t seen_bits(const View& w, int base) {
   return low_bits(w.pos + 1 - base) & (~low_bits(w.lo - base) | low_bits(w.sinks - base));
 }
 
-// Largest visible score of a thread's KEYS keys of a row, from `n0` on.
+// Largest visible score of a thread's KEYS keys of a row; base[c]: first token of its group c.
 template <int KEYS>
-__device__ __forceinline__ float part_max(uint32_t tS, int n0, const View& w) {
+__device__ __forceinline__ float part_max(uint32_t tS, const int (&base)[KEYS / GK], const View& w) {
   float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
   for (int c = 0; c < KEYS / 32; ++c) {
-    const int cls = chunk_class(w, n0 + c * 32);
+    const int cls = chunk_class(w, base[c]);
     if (cls == NONE) continue;
     uint32_t v[32];
     tmem_ld32(tS + c * 32, v);
     wait_ld();
     if (cls == SOME) {
-      const uint32_t seen = seen_bits(w, n0 + c * 32);
+      const uint32_t seen = seen_bits(w, base[c]);
 #pragma unroll
       for (int k = 0; k < 32; ++k)
         if (!(seen >> k & 1)) v[k] = 0xff800000u;
@@ -261,11 +264,11 @@ __device__ __forceinline__ float part_max(uint32_t tS, int n0, const View& w) {
 }
 // P = 2^(s * sl2 - mu) as 16-bit pairs over the front of the thread's scores; returns the sum of the unrounded P.
 template <int KV, int KEYS>
-__device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, int n0, const View& w) {
+__device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, const int (&base)[KEYS / GK], const View& w) {
   float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < KEYS / 32; ++c) {
-    const int cls = chunk_class(w, n0 + c * 32);
+    const int cls = chunk_class(w, base[c]);
     uint32_t out[16];
     if (cls == NONE) {
 #pragma unroll
@@ -275,7 +278,7 @@ __device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, int 
       tmem_ld32(tS + c * 32, v);
       wait_ld();
       if (cls == SOME) {
-        const uint32_t seen = seen_bits(w, n0 + c * 32);
+        const uint32_t seen = seen_bits(w, base[c]);
 #pragma unroll
         for (int k = 0; k < 32; ++k)
           if (!(seen >> k & 1)) v[k] = 0xff800000u;
@@ -352,9 +355,11 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     b = e.x;
     block = e.y;
     const int t0 = block * I::ROWS / p.gqa, t1 = (block * I::ROWS + I::ROWS - 1) / p.gqa;
-    r = req_info<TK>(p, b, t0, t1 - t0 + 1);
+    r = req_info<GK>(p, b, t0, t1 - t0 + 1);
+    r.cnt = (r.cnt + TK / GK - 1) / (TK / GK);  // tiles
   };
-  auto tile_at = [](const Req& r, int i) { return (i < r.ns ? i : r.tlo + i - r.ns) * TK; };
+  // first token of a group; groups behind the last one lie past every visible key
+  auto group_at = [](const Req& r, int i) { return (i < r.ns ? i : r.tlo + i - r.ns) * GK; };
 
   if (warp < I::SOFT_WARPS) {
     // ------------------------------------------------------------------------------------------ softmax, epilogue
@@ -399,8 +404,10 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         wait_or_flag(b_s + 8 * buf, (n >> 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
         __syncwarp();
         fence_after();
-        const int n0 = tile_at(r, i) + half * KEYS;
-        float mx = part_max<KEYS>(tS, n0, w);
+        int base[KEYS / GK];
+#pragma unroll
+        for (int c = 0; c < KEYS / GK; ++c) base[c] = group_at(r, i * (TK / GK) + half * (KEYS / GK) + c);
+        float mx = part_max<KEYS>(tS, base, w);
         if (SPLIT == 2) mx = fmaxf(mx, exchange(mx));
         mx *= sl2;
         bool scale = false;
@@ -429,7 +436,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             tmem_st32(tO + c * 32, v);
           }
         }
-        sum += part_exp<KV, KEYS>(tS, sl2, ref == -INFINITY ? 0.f : ref, n0, w);
+        sum += part_exp<KV, KEYS>(tS, sl2, ref == -INFINITY ? 0.f : ref, base, w);
         wait_st();
         fence_before();
         __syncwarp();
@@ -602,13 +609,20 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     };
     auto stage_for = [&](const Req& r, int b, int h, int tile, int part, bool is_v) {
       if (q % I::KV_WARPS == w) {
-        const int n0 = tile_at(r, tile) + (is_v ? part * KC : 0);
+        constexpr int MOST = TK / GK;
         const int keys = is_v ? KC : TK;
-        // Inside the run (or the sinks) every key is a real one: whole boxes of pages by TMA.
-        if (boxes && n0 + keys <= r.kend && (n0 >= r.lower || n0 + keys <= p.sinks)) {
-          const int box = min(p.page_mask + 1, keys), nb = keys / box;
+        int n0[MOST];
+        bool inside = boxes != 0;  // every key of the stage is a real one
+#pragma unroll
+        for (int u = 0; u < MOST; ++u) {
+          n0[u] = group_at(r, tile * MOST + (is_v ? part * (KC / GK) : 0) + u);
+          if (u * GK < keys) inside &= n0[u] + GK <= r.kend && (n0[u] >= r.lower || n0[u] + GK <= p.sinks);
+        }
+        if (inside) {  // whole boxes of pages by TMA
+          const int box = min(p.page_mask + 1, GK), nb = keys / box;
           const int k = lane % nb, slab = lane / nb;
-          const int at_key = n0 + k * box;
+          const int gu = k * box / GK;
+          const int at_key = (gu == 0 ? n0[0] : gu == 1 ? n0[1] : gu == 2 ? n0[2] : n0[3]) + k * box % GK;
           const int pg = p.pt[b * p.pt_s0 + (at_key >> p.page_shift) * p.pt_s1];
           const int at = q % NST, turn = q / NST;
           wait_stage(at, turn);
@@ -628,13 +642,12 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             return;
           }
         }
-        constexpr int MOST = 128 / 32;
         int page[MOST];
 #pragma unroll
         for (int u = 0; u < MOST; ++u) {
-          const int n = n0 + u * 32 + lane;
+          const int n = n0[u] + lane;
           page[u] = -1;
-          if (u * 32 < keys && n < r.kend && (n >= r.lower || n < p.sinks)) {
+          if (u * GK < keys && n < r.kend && (n >= r.lower || n < p.sinks)) {
             page[u] = p.pt[b * p.pt_s0 + (n >> p.page_shift) * p.pt_s1];
             if (page[u] < 0 || page[u] >= p.num_pages) {
               atomicExch(p.status, GA_ST_BAD_PAGE);

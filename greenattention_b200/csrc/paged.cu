@@ -96,10 +96,9 @@ int run_tc(Launch& a, size_t ws_bytes) {
     std::memset(&kk, 0, sizeof(kk));
     kk.base = d.k, kk.s_page = d.k_s0, kk.s_tok = d.k_s1, kk.s_head = d.k_s2;
     kk.pages = d.num_pages, kk.page = page, kk.kvh = d.kvh, kk.hd = I::HD;
-    kk.box = page < ga::paged::tc::TK ? page : ga::paged::tc::TK;
+    kk.box = page < ga::paged::tc::GK ? page : ga::paged::tc::GK;
     vk = kk;
     vk.base = d.v, vk.s_page = d.v_s0, vk.s_tok = d.v_s1, vk.s_head = d.v_s2;
-    vk.box = page < I::KC ? page : I::KC;
     boxes = pool_map(kk, &maps[0]) && pool_map(vk, &maps[1]);  // strides that a map cannot hold: without
   }
   GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(static_cast<unsigned>(items < a.sm ? items : a.sm)), dim3(I::NT),
