@@ -193,6 +193,16 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def raw_stream(index: int) -> int:
+    """The current stream of a device as an address, without building a Stream object where torch offers that."""
+    import torch
+
+    global raw_stream
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    raw_stream = fast if fast is not None else lambda i: torch.cuda.current_stream(i).cuda_stream
+    return raw_stream(index)
+
+
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise GreenAttentionError(f"{what}: {lib().ga_last_error().decode(errors='replace')}")

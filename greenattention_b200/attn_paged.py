@@ -37,7 +37,6 @@ STATUS_NAMES = {
     5: "a cache_seqlens entry exceeded page_table.shape[1] * page_size",
 }
 _ALLOWED = attn_decode._ALLOWED | {"sink_tokens"}
-_TENSORS = ("k_cache", "v_cache", "page_table", "cache_seqlens", "cu_seqlens_q")
 logger = logging.getLogger(__name__)
 
 _status: dict = {}           # device index -> int32 word the kernels leave a non-zero value in
@@ -75,83 +74,90 @@ def check_status(device: Union[torch.device, int, None] = None, reset: bool = Tr
 
 
 def _reason(kw: dict) -> Optional[str]:
-    for name, val in kw.items():
-        if name not in _ALLOWED and val is not None:
+    more = kw.keys() - _ALLOWED
+    for name in more:
+        if kw[name] is not None:
             return f"unsupported arg {name}"
-    for name in ("q",) + _TENSORS:
-        if not isinstance(kw.get(name), torch.Tensor):
-            return f"not a paged varlen call ({name})"
-    q, kc, vc, pt, cs, cu = (kw[n] for n in ("q",) + _TENSORS)
-    if kc.dtype not in KV_TYPES or vc.dtype != kc.dtype:
-        return f"kv dtype {kc.dtype} / {vc.dtype}"
-    if q.dtype != kc.dtype and not (kc.dtype == FP8 and q.dtype == torch.bfloat16):
-        return f"q dtype {q.dtype} beside a {kc.dtype} cache"
-    if q.dim() != 3 or kc.dim() != 4 or kc.shape != vc.shape:
+    get = kw.get
+    q, kc, vc, pt, cs, cu = get("q"), get("k_cache"), get("v_cache"), get("page_table"), get("cache_seqlens"), get("cu_seqlens_q")
+    for t in (q, kc, vc, pt, cs, cu):
+        if not isinstance(t, torch.Tensor):
+            return "not a paged varlen call"
+    kv, qt = kc.dtype, q.dtype
+    if kv not in KV_TYPES or vc.dtype != kv:
+        return f"kv dtype {kv} / {vc.dtype}"
+    if qt != kv and not (kv == FP8 and qt == torch.bfloat16):
+        return f"q dtype {qt} beside a {kv} cache"
+    shape, kshape = q.shape, kc.shape
+    if len(shape) != 3 or len(kshape) != 4 or kshape != vc.shape:
         return "q or kv rank, or k/v shapes differ"
-    total, qh, hd = q.shape
-    pages, page, kvh, khd = kc.shape
+    total, qh, hd = shape
+    _, page, kvh, khd = kshape
     if hd not in HEAD_DIMS or khd != hd or not kvh or not qh or qh % kvh:
         return f"q shape: no kernel for (head_dim={hd}, q_heads={qh}, kv_heads={kvh})"
     if page <= 0 or page & (page - 1):
         return "page_size not a power of two"
-    el = kc.element_size()
-    for t in (kc, vc):
-        s0, s1, s2, s3 = t.stride()
-        if s3 != 1 or (s0 | s1 | s2) * el % 16 or t.data_ptr() % 16:
-            return "kv layout: last stride 1, other strides and the base multiples of 16 bytes"
+    align = 15 if kv == FP8 else 7  # elements of 16 bytes
+    k0, k1, k2, k3 = kc.stride()
+    v0, v1, v2, v3 = vc.stride()
+    if k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & align or (kc.data_ptr() | vc.data_ptr()) & 15:
+        return "kv layout: last stride 1, other strides and the base multiples of 16 bytes"
     s0, s1, s2 = q.stride()
-    if s2 != 1 or (s0 | s1) % 4 or q.data_ptr() % (4 * q.element_size()):
+    if s2 != 1 or (s0 | s1) & 3 or q.data_ptr() & (3 if qt == FP8 else 7):
         return "q layout: last stride 1, other strides and the base multiples of 4 elements"
-    if pt.dtype != torch.int32 or pt.dim() != 2 or cs.dtype != torch.int32 or cs.dim() != 1 or cu.dtype != torch.int32 or cu.dim() != 1:
+    i32 = torch.int32
+    ps = pt.shape
+    if pt.dtype != i32 or cs.dtype != i32 or cu.dtype != i32 or len(ps) != 2 or cs.dim() != 1 or cu.dim() != 1:
         return "page_table / cache_seqlens / cu_seqlens_q dtype or rank"
     batch = cs.shape[0]
-    if batch == 0 or pt.shape[0] != batch or cu.shape[0] != batch + 1:
+    if batch == 0 or ps[0] != batch or cu.shape[0] != batch + 1:
         return "batch mismatch"
-    if cs.stride(0) != 1 and batch > 1 or cu.stride(0) != 1:
+    if batch > 1 and cs.stride(0) != 1 or cu.stride(0) != 1:
         return "cache_seqlens / cu_seqlens_q stride"
-    mq = kw.get("max_seqlen_q")
-    if not isinstance(mq, int) or isinstance(mq, bool) or mq < 1:
+    mq = get("max_seqlen_q")
+    if type(mq) is not int or mq < 1:
         return f"max_seqlen_q {mq} is not a positive int"
-    if mq > 1 and not kw.get("causal", False):
+    if mq > 1 and not get("causal", False):
         return "non-causal call with several query tokens"
-    if kw.get("softcap"):
+    if get("softcap"):
         return "softcap"
-    window = attn_decode._window_left(kw)
-    if isinstance(window, str):
-        return window
-    sinks = kw.get("sink_tokens")
-    if sinks is not None and (not isinstance(sinks, int) or isinstance(sinks, bool) or not 0 <= sinks < 1 << 31):
+    if get("window_size") is not None:
+        window = attn_decode._window_left(kw)
+        if isinstance(window, str):
+            return window
+    sinks = get("sink_tokens")
+    if sinks is not None and (type(sinks) is not int or not 0 <= sinks < 1 << 31):
         return f"sink_tokens {sinks} is not a count"
     dev = q.device
     for t in (kc, vc, pt, cs, cu):
         if t.device != dev:
             return f"a tensor is on {t.device}, q on {dev}"
     for name in ("k_descale", "v_descale"):
-        t = kw.get(name)
+        t = get(name)
         if t is not None:
-            if t.device != dev:
-                return f"{name} is on {t.device}, q on {dev}"
+            if not isinstance(t, torch.Tensor) or t.device != dev:
+                return f"{name} is on {getattr(t, 'device', None)}, q on {dev}"
             why = attn_decode._descale_reason(t, batch, kvh, name)
             if why:
                 return why
-    out = kw.get("out")
+    out = get("out")
     if out is not None:
-        want = torch.bfloat16 if kc.dtype == FP8 else kc.dtype
+        want = torch.bfloat16 if kv == FP8 else kv
         if not isinstance(out, torch.Tensor) or out.device != dev:
             return "out is not a tensor on q's device"
-        if out.dtype != want or out.shape != q.shape or out.stride(2) != 1:
+        if out.dtype != want or out.shape != shape or out.stride(2) != 1:
             return f"out must be {want} of q's shape with last stride 1"
         s0, s1, _ = out.stride()
-        if (s0 | s1) % 4 or out.data_ptr() % 8 or (qh > 1 and s1 < hd) or (total > 1 and s0 < hd):
+        if (s0 | s1) & 3 or out.data_ptr() & 7 or (qh > 1 and s1 < hd) or (total > 1 and s0 < hd):
             return "out layout: rows must not overlap, strides and the base multiples of 4 elements"
-    if not q.is_cuda:
+    if dev.type != "cuda":
         return "tensors are on the host: the green kernels have no CPU path"
     return None
 
 
 def _launch(
-    *, q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, window_size=(-1, -1), sink_tokens=None,
-    softmax_scale=None, return_softmax_lse=False, out=None, k_descale=None, v_descale=None, causal=False, **_,
+    *, q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, window_size=None, sink_tokens=None,
+    softmax_scale=None, return_softmax_lse=False, out=None, k_descale=None, v_descale=None, **_,
 ):
     dev = q.device
     index = dev.index
@@ -160,19 +166,18 @@ def _launch(
     total, qh, hd = q.shape
     kv = k_cache.dtype
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16 if kv == FP8 else kv, device=dev)
-    lse = torch.empty((qh, total), dtype=torch.float32, device=dev) if return_softmax_lse else None
+        out = q.new_empty(q.shape, dtype=torch.bfloat16 if kv == FP8 else kv)
+    lse = q.new_empty((qh, total), dtype=torch.float32) if return_softmax_lse else None
     pages, page, kvh, _ = k_cache.shape
     batch, cols = page_table.shape
     lib = _C.lib()
     nbytes = _workspace_bytes.get((index, batch))
     if nbytes is None:
         nbytes = _workspace_bytes[(index, batch)] = lib.ga_paged_workspace_bytes(index, batch)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     q0, q1, _ = q.stride()
-    k0, k1, k2, _ = k_cache.stride()
-    v0, v1, v2, _ = v_cache.stride()
     o0, o1, _ = out.stride()
+    t0, t1 = page_table.stride()
     kd = vd = None
     kd0 = kd1 = vd0 = vd1 = 0
     if k_descale is not None:
@@ -182,20 +187,20 @@ def _launch(
     left = -1 if window_size is None or window_size[0] is None else int(window_size[0])
     p = _C.GaPagedParams(
         KV_TYPES[kv], q.data_ptr(), q.dtype == torch.bfloat16, q0, q1, k_cache.data_ptr(), v_cache.data_ptr(),
-        k0, k1, k2, v0, v1, v2, pages, page, qh, kvh, hd,
-        page_table.data_ptr(), page_table.stride(0), page_table.stride(1), cols,
+        *k_cache.stride()[:3], *v_cache.stride()[:3], pages, page, qh, kvh, hd,
+        page_table.data_ptr(), t0, t1, cols,
         cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), kd, kd0, kd1, vd, vd0, vd1,
         out.data_ptr(), o0, o1, None if lse is None else lse.data_ptr(), total,
         batch, max_seqlen_q, min(left, 1 << 30), sink_tokens or 0, hd**-0.5 if softmax_scale is None else softmax_scale,
         _status[index].data_ptr(), ws.data_ptr(), nbytes,
     )
-    stream = torch.cuda.current_stream(dev).cuda_stream
     if torch.cuda.current_device() == index:
-        rc = lib.ga_paged_attend(ctypes.byref(p), stream)
+        rc = lib.ga_paged_attend(ctypes.byref(p), _C.raw_stream(index))
     else:
         with torch.cuda.device(dev):  # the library launches on the current device
-            rc = lib.ga_paged_attend(ctypes.byref(p), stream)
-    _C.check(rc, "ga_paged_attend")
+            rc = lib.ga_paged_attend(ctypes.byref(p), _C.raw_stream(index))
+    if rc:
+        _C.check(rc, "ga_paged_attend")
     return (out, lse) if return_softmax_lse else out
 
 

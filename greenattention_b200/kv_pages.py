@@ -30,6 +30,7 @@ STATUS_NAMES = {
     8: "no free page was left", 9: "the page counts did not match the page table",
     10: "entries of one call contradict one another, or a forked row was not empty",
 }
+_NO_SCRATCH = ("ga_pages_free", "ga_pages_evict")
 logger = logging.getLogger(__name__)
 
 
@@ -85,6 +86,7 @@ class PagePool:
         _C.init(dev.index)
         self.caches, self.page_table, self.seqlens, self.refs = caches, page_table, seqlens, refs
         self.device, self.page_size, self.num_pages = dev, page_size, pages
+        self._scratch_bytes: dict = {}  # entries of a call -> bytes
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         # what the kernels read about the tensors
         self._base = torch.tensor([s[0] for s in seen], dtype=torch.int64, device=dev)
@@ -121,17 +123,21 @@ class PagePool:
         lib = _C.lib()
         # A copy of the handle's struct: calls of several host threads do not share one.
         p = _C.GaPagePool.from_buffer_copy(self._p)
-        p.scratch_bytes = lib.ga_pages_scratch_bytes(ctypes.byref(p), n)
-        scratch = torch.empty(p.scratch_bytes, dtype=torch.uint8, device=self.device)
-        p.scratch = scratch.data_ptr()
-        stream = torch.cuda.current_stream(self.device).cuda_stream
+        if name not in _NO_SCRATCH:
+            nbytes = self._scratch_bytes.get(n)
+            if nbytes is None:
+                nbytes = self._scratch_bytes[n] = lib.ga_pages_scratch_bytes(ctypes.byref(p), n)
+            scratch = self.refs.new_empty(nbytes, dtype=torch.uint8)
+            p.scratch, p.scratch_bytes = scratch.data_ptr(), nbytes
         fn = getattr(lib, name)
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(ctypes.byref(p), *args, stream)
+        index = self.device.index
+        if torch.cuda.current_device() == index:
+            rc = fn(ctypes.byref(p), *args, _C.raw_stream(index))
         else:
             with torch.cuda.device(self.device):  # the library launches on the current device
-                rc = fn(ctypes.byref(p), *args, stream)
-        _C.check(rc, name)
+                rc = fn(ctypes.byref(p), *args, _C.raw_stream(index))
+        if rc:
+            _C.check(rc, name)
 
     def check_status(self, reset: bool = True) -> int:
         """The status word (0 = fine; ``STATUS_NAMES``), logged when it is not 0 and put back. Synchronises."""
