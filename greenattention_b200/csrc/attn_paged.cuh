@@ -237,6 +237,7 @@ struct Inst {
   static constexpr int SMEM = NW * NST * STAGE;
   static constexpr int RC = 16 * MT;                       // rows of a unit
   static constexpr int NT = NW * 32;
+  static __device__ __forceinline__ Req req(const PagedDev& p, int b) { return req_info<T>(p, b, 0, p.max_q); }
 };
 
 // ------------------------------------------------------------------------------------------------------- kernel
@@ -648,7 +649,7 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
   const int b = blockIdx.x / p.upr, j = blockIdx.x - b * p.upr;
   const int group = j / p.nrb, block = j - group * p.nrb;
   const int h = group * p.hg + blockIdx.y;
-  const Req r = req_info<I::T>(p, b, 0, p.max_q);
+  const Req r = I::req(p, b);
   const int rows = min(r.nq * p.gqa - block * I::RC, I::RC);
   const float vds = p.vd && h < p.kvh ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
   grid_dep_wait();

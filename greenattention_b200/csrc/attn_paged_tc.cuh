@@ -36,15 +36,17 @@ constexpr int GK = 32;           // keys of a group
 constexpr int STAGE = 16384;
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
 
-template <int HD_, int KV_>
+// SPLIT_KV: at most 128 rows of each (request, kv head), its keys cut over CTAs (verify). Else row blocks of prompts.
+template <int HD_, int KV_, bool SPLIT_KV_>
 struct TcInst {
   static constexpr int HD = HD_, KV = KV_;
-  static constexpr int NQ = HD == 256 ? 1 : 2;
+  static constexpr bool SPLIT_KV = SPLIT_KV_;
+  static constexpr int NQ = HD == 256 || SPLIT_KV ? 1 : 2;
   static constexpr int SLABS = HD / 64;            // K stages of a tile, and V stages
   static constexpr int KC = 8192 / HD;             // keys of a V stage
   static constexpr int ROWS = NQ * TM;
   static constexpr int Q_BYTES = NQ * SLABS * STAGE;
-  static constexpr int NST = HD == 64 ? 8 : 10;
+  static constexpr int NST = HD == 256 ? 10 : (NQ == 1 ? 12 : (HD == 64 ? 8 : 10));
   static constexpr int EG = SLABS < 2 ? SLABS : 2;  // stages that are filled and released together
   static constexpr int SPLIT = 2;                   // threads that share a row
   static constexpr int SOFT_WARPS = 4 * NQ * SPLIT;
@@ -69,6 +71,12 @@ struct TcInst {
   static constexpr int SMEM = Q_BYTES + NST * STAGE + X_BYTES + 512;
   static_assert(NST % EG == 0, "ring");
   static constexpr int O_COL = 256;
+  static constexpr int RC = ROWS;  // rows of a unit, for the combine kernel
+  static __device__ __forceinline__ Req req(const PagedDev& p, int b) {
+    Req r = req_info<GK>(p, b, 0, p.max_q);
+    r.cnt = (r.cnt + TK / GK - 1) / (TK / GK);
+    return r;
+  }
   static_assert(SMEM <= 232448, "shared memory");
 };
 
@@ -179,9 +187,57 @@ __device__ __forceinline__ void gather(uint32_t dst, const uint8_t* base, long l
   }
 }
 
-// The call's row blocks: blocks[0] = how many, then (request, row block) pairs, a request's last block first.
+// Where each gang's slice of the call's tiles begins: (request, tile, tiles of the slice), tiles 0: none. A unit is a whole
+// request; gang g is the CTAs g * kv_heads + h, one kv head each, which walk the same pages at the same time.
+template <class I>
+__global__ void __launch_bounds__(1024) plan_split_kernel(const __grid_constant__ PagedDev p, int G, int4* list) {
+  __shared__ long long wsum[32];
+  grid_dep_wait();
+  grid_dep_launch();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.batch + 1023) / 1024;
+  const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += I::req(p, b).cnt;
+  long long incl = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += o;
+  }
+  if (lane == 31) wsum[warp] = incl;
+  __syncthreads();
+  long long at = incl - mine, total = 0;
+  for (int w = 0; w < 32; ++w) {
+    if (w < warp) at += wsum[w];
+    total += wsum[w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    p.prefix[b] = static_cast<int>(at);
+    at += I::req(p, b).cnt;
+  }
+  if (tid == 0) p.prefix[p.batch] = static_cast<int>(total);
+  __syncthreads();
+  const int used = walkers_for(total, G);
+  for (int g = tid; g < G; g += 1024) {
+    const long long g0 = slice(total, used, g), g1 = slice(total, used, g + 1);
+    int4 e = make_int4(0, 0, 0, 0);
+    if (g1 > g0) {
+      int lo = 0, hi = p.batch - 1;  // the last request whose tiles begin at g0 or before
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.prefix[mid] <= g0) lo = mid;
+        else hi = mid - 1;
+      }
+      e = make_int4(lo, static_cast<int>(g0 - p.prefix[lo]), static_cast<int>(g1 - g0), 0);
+    }
+    list[g] = e;
+  }
+}
+
+// The call's row blocks: *count = how many, then (request, row block), a request's last block first.
 template <int ROWS>
-__global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constant__ PagedDev p, int* count, int2* blocks) {
+__global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constant__ PagedDev p, int* count, int4* blocks) {
   __shared__ int wsum[32];
   __shared__ int base;
   grid_dep_wait();
@@ -214,7 +270,7 @@ __global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constan
     // a warp lays out its requests' blocks together
     for (int src = 0; src < 32; ++src) {
       const int m = __shfl_sync(0xffffffffu, n, src), to = __shfl_sync(0xffffffffu, at, src);
-      for (int k = lane; k < m; k += 32) blocks[to + k] = make_int2(b0 + warp * 32 + src, m - 1 - k);
+      for (int k = lane; k < m; k += 32) blocks[to + k] = make_int4(b0 + warp * 32 + src, m - 1 - k, 0, 0);
     }
     __syncthreads();
     if (tid == 0) base += total;
@@ -297,7 +353,7 @@ __device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, cons
 }
 
 template <class I>
-__global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_constant__ PagedDev p, const int* count, const int2* blocks,
+__global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_constant__ PagedDev p, const int* count, const int4* list,
                                                                  const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int boxes) {
   constexpr int HD = I::HD, KV = I::KV, NQ = I::NQ, SLABS = I::SLABS, NST = I::NST, KC = I::KC;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -346,17 +402,63 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   grid_dep_wait();
   grid_dep_launch();
 
-  const int items = *count * p.kvh;
   bool failed = false;
-  auto item_of = [&](int x, int& b, int& block, int& h, Req& r) {
-    const int k = x / p.kvh;
-    h = x - k * p.kvh;
-    const int2 e = blocks[k];
-    b = e.x;
-    block = e.y;
-    const int t0 = block * I::ROWS / p.gqa, t1 = (block * I::ROWS + I::ROWS - 1) / p.gqa;
-    r = req_info<GK>(p, b, t0, t1 - t0 + 1);
-    r.cnt = (r.cnt + TK / GK - 1) / (TK / GK);  // tiles
+  // The CTA's segments: a row block of a prompt with all its tiles, or what its gang's slice holds of a request.
+  struct Seg {
+    int b, block, h;
+    int i0;    // first tile
+    int slot;  // < 0: the rows' final result; >= 0: a piece, into this workspace slot
+    Req r;     // r.cnt: tiles of the segment
+  };
+  struct Work {
+    int x, end;                 // prompts: item and their number
+    int b, off, rem, gang, h;   // split: place in the slice
+    bool first;
+  };
+  auto begin = [&]() {
+    Work w;
+    if (I::SPLIT_KV) {
+      w.gang = blockIdx.x / p.kvh;
+      w.h = blockIdx.x - w.gang * p.kvh;
+      const int4 e = list[w.gang];
+      w.b = e.x, w.off = e.y, w.rem = e.z;
+      w.first = true;
+    } else {
+      w.x = blockIdx.x;
+      w.end = *count * p.kvh;
+    }
+    return w;
+  };
+  auto next = [&](Work& w, Seg& s) {
+    if (I::SPLIT_KV) {
+      if (w.rem <= 0) return false;
+      s.r = I::req(p, w.b);
+      while (s.r.cnt == 0) {  // requests without visible keys
+        if (++w.b >= p.batch) return false;
+        s.r = I::req(p, w.b);
+      }
+      const int all = s.r.cnt;
+      const int n = min(all - w.off, w.rem);
+      s.b = w.b, s.block = 0, s.h = w.h;
+      s.i0 = w.off;
+      s.slot = n == all ? -1 : (2 * w.gang + (w.first ? 0 : 1)) * p.kvh + w.h;
+      s.r.cnt = n;
+      w.rem -= n;
+      w.off = 0;
+      w.first = false;
+      return ++w.b < p.batch || (w.rem = 0, true);
+    }
+    if (w.x >= w.end) return false;
+    const int k = w.x / p.kvh;
+    s.h = w.x - k * p.kvh;
+    const int4 e = list[k];
+    s.b = e.x, s.block = e.y;
+    const int t0 = s.block * I::ROWS / p.gqa, t1 = (s.block * I::ROWS + I::ROWS - 1) / p.gqa;
+    s.r = req_info<GK>(p, s.b, t0, t1 - t0 + 1);
+    s.r.cnt = (s.r.cnt + TK / GK - 1) / (TK / GK);
+    s.i0 = 0, s.slot = -1;
+    w.x += gridDim.x;
+    return true;
   };
   // first token of a group; groups behind the last one lie past every visible key
   auto group_at = [](const Req& r, int i) { return (i < r.ns ? i : r.tlo + i - r.ns) * GK; };
@@ -382,10 +484,11 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       if (I::TURNS == 2) turn ^= 1;  // the slot is written again behind a barrier that its reader has passed
       return other;
     };
-    for (int x = blockIdx.x; x < items; x += gridDim.x) {
-      int b, block, h;
-      Req r;
-      item_of(x, b, block, h, r);
+    Work work = begin();
+    Seg seg;
+    while (next(work, seg)) {
+      const int b = seg.b, block = seg.block, h = seg.h;
+      const Req& r = seg.r;
       const int rr0 = block * I::ROWS + g * TM + (warp & 3) * 32, rr = rr0 + lane;
       const bool real = rr < r.nq * p.gqa;
       const int tok = rr / p.gqa;
@@ -394,8 +497,9 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       w.lo = p.window >= 0 ? w.pos - p.window : -(1 << 30);
       w.sinks = p.sinks;
       w.window = p.window;
-      w.pmin = r.pos0 + rr0 / p.gqa;
-      w.pmax = r.pos0 + (rr0 + 31) / p.gqa;
+      const bool any = rr0 < r.nq * p.gqa;  // a warp of padding rows sees nothing and looks at nothing
+      w.pmin = any ? r.pos0 + rr0 / p.gqa : -1;
+      w.pmax = any ? r.pos0 + (rr0 + 31) / p.gqa : -1;
       const float sl2 = p.scale_log2;
       float ref = -INFINITY, sum = 0.f;
       for (int i = 0; i < r.cnt; ++i, n += NQ) {
@@ -406,7 +510,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         fence_after();
         int base[KEYS / GK];
 #pragma unroll
-        for (int c = 0; c < KEYS / GK; ++c) base[c] = group_at(r, i * (TK / GK) + half * (KEYS / GK) + c);
+        for (int c = 0; c < KEYS / GK; ++c) base[c] = group_at(r, (seg.i0 + i) * (TK / GK) + half * (KEYS / GK) + c);
         float mx = part_max<KEYS>(tS, base, w);
         if (SPLIT == 2) mx = fmaxf(mx, exchange(mx));
         mx *= sl2;
@@ -464,7 +568,16 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           tmem_ld32(tO + c * 32, v);
           wait_ld();
         }
-        if (real) {
+        if (I::SPLIT_KV && seg.slot >= 0) {
+          const float one = sum == 0.f ? 0.f : 1.f / sum;
+          float* ws = p.ws_o + (static_cast<long long>(seg.slot) * TM + row) * HD + half * DIMS + c * 32;
+          if (real) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4*>(ws + k) = make_float4(__uint_as_float(v[k]) * one, __uint_as_float(v[k + 1]) * one,
+                                                               __uint_as_float(v[k + 2]) * one, __uint_as_float(v[k + 3]) * one);
+          }
+        } else if (real) {
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
             uint2 o = make_uint2(0u, 0u);
@@ -476,7 +589,9 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           }
         }
       }
-      if (real && half == 0 && p.lse)
+      if (I::SPLIT_KV && seg.slot >= 0) {
+        if (real && half == 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = sum == 0.f ? -INFINITY : ref + lg2(sum);
+      } else if (real && half == 0 && p.lse)
         p.lse[static_cast<long long>(qh) * p.total_q + qrow] = sum == 0.f ? -INFINITY : (ref + lg2(sum)) * 0.6931471805599453f;
       if (r.cnt > 0) {
         fence_before();
@@ -538,10 +653,10 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           if (at == NST) at = 0, par ^= 1;
         }
       };
-      for (int x = blockIdx.x; x < items && !failed; x += gridDim.x) {
-        int b, block, h;
-        Req r;
-        item_of(x, b, block, h, r);
+      Work work = begin();
+      Seg seg;
+      while (!failed && next(work, seg)) {
+        const Req& r = seg.r;
         if (r.cnt == 0) continue;
         if (NQ == 2) {
           wait_or_flag(b_qfull, done & 1, failed, p.status, GA_ST_WAIT_FULL);
@@ -669,16 +784,17 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       }
       ++q;
     };
-    for (int x = blockIdx.x; x < items && !failed; x += gridDim.x) {
-      int b, block, h;
-      Req r;
-      item_of(x, b, block, h, r);
+    Work work = begin();
+    Seg seg;
+    while (!failed && next(work, seg)) {
+      const int b = seg.b, h = seg.h;
+      const Req& r = seg.r;
       constexpr int AHEAD = NQ == 1 ? 2 : 1;  // K tiles in front of the V tile they go with
       for (int i = 0; i < r.cnt + AHEAD; ++i) {
         if (i >= AHEAD)
-          for (int s = 0; s < SLABS; ++s) stage_for(r, b, h, i - AHEAD, s, true);
+          for (int s = 0; s < SLABS; ++s) stage_for(r, b, h, seg.i0 + i - AHEAD, s, true);
         if (i < r.cnt)
-          for (int s = 0; s < SLABS; ++s) stage_for(r, b, h, i, s, false);
+          for (int s = 0; s < SLABS; ++s) stage_for(r, b, h, seg.i0 + i, s, false);
       }
     }
     if (pending >= 0) {
@@ -689,10 +805,11 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     // ---------------------------------------------------------------------------------------------------- Q gather
     const int w = warp - Q_WARP;
     int done = 0;
-    for (int x = blockIdx.x; x < items && !failed; x += gridDim.x) {
-      int b, block, h;
-      Req r;
-      item_of(x, b, block, h, r);
+    Work work = begin();
+    Seg seg;
+    while (!failed && next(work, seg)) {
+      const int block = seg.block, h = seg.h;
+      const Req& r = seg.r;
       if (r.cnt == 0) continue;
       if (done > 0) wait_or_flag(b_qempty, (done - 1) & 1, failed, p.status, GA_ST_WAIT_EMPTY);
       failed = __any_sync(0xffffffffu, failed);

@@ -1,5 +1,6 @@
 // C ABI of the attention over 16-bit and e4m3 paged caches with first tokens kept visible (attn_paged.cuh): argument
 // checks, choice of the instance, launches.
+#include <cstdlib>
 #include <mutex>
 #include <vector>
 
@@ -74,35 +75,71 @@ int limits_tc() {
   return 0;
 }
 
+// Maps of the call's K and V pools; false: the tensor-core kernel gathers without them.
+template <class I>
+bool pool_maps(const PagedDev& d, CUtensorMap (&maps)[2]) {
+  std::memset(maps, 0, sizeof(maps));
+  const int page = d.page_mask + 1;
+  if (page < 8 || d.num_pages <= 0) return false;
+  MapKey kk, vk;
+  std::memset(&kk, 0, sizeof(kk));
+  kk.base = d.k, kk.s_page = d.k_s0, kk.s_tok = d.k_s1, kk.s_head = d.k_s2;
+  kk.pages = d.num_pages, kk.page = page, kk.kvh = d.kvh, kk.hd = I::HD;
+  kk.box = page < ga::paged::tc::GK ? page : ga::paged::tc::GK;
+  vk = kk;
+  vk.base = d.v, vk.s_page = d.v_s0, vk.s_tok = d.v_s1, vk.s_head = d.v_s2;
+  return pool_map(kk, &maps[0]) && pool_map(vk, &maps[1]);  // not for strides that a map cannot hold
+}
+
+// What the tensor-core kernel takes: its query rows go through 16-byte copies, and it takes the maximum before the scale.
+bool tc_takes(const PagedDev& d) {
+  return !d.kd && d.scale_log2 > 0.f && d.q_s0 % 8 == 0 && d.q_s1 % 8 == 0 && reinterpret_cast<uintptr_t>(d.q) % 16 == 0;
+}
+
+// Enough CTAs to spread the rows of a small call over the SMs.
+unsigned combine_shares(long long pairs, int rows, int sm) {
+  const long long z = (2LL * sm + pairs - 1) / pairs;
+  return static_cast<unsigned>(z < 1 ? 1 : (z > rows ? rows : z));
+}
+
+// Verify on the tensor cores (at most 128 rows of a kv head): gangs of kv_heads CTAs, slices of the requests' tiles, and the
+// combine kernel; -1: the call is not one for it.
+template <class I>
+int run_tc_split(Launch& a) {
+  PagedDev& d = a.d;
+  if (!tc_takes(d) || d.kvh > a.sm) return -1;
+  CUtensorMap maps[2];
+  const bool boxes = pool_maps<I>(d, maps);
+  const int gangs = a.sm / d.kvh;
+  d.hg = d.kvh, d.groups = 1, d.nrb = 1, d.upr = 1, d.walkers = 1;
+  int4* list = reinterpret_cast<int4*>(d.ws_lse + static_cast<size_t>(2 * a.sm) * ga::paged::tc::TM);
+  static_assert(ga::paged::SLOT_ROWS >= ga::paged::tc::TM + 16 && I::HD * ga::paged::tc::TM <= ga::paged::SLOT_FLOATS, "workspace");
+  GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_split_kernel<I>, dim3(1), dim3(1024), 0, a.st, d, gangs, list));
+  GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(gangs * d.kvh), dim3(I::NT), I::SMEM, a.st, d,
+                                static_cast<const int*>(nullptr), const_cast<const int4*>(list), maps[0], maps[1], static_cast<int>(boxes)));
+  const int rows = d.max_q * d.gqa;
+  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_combine<I>, dim3(d.batch, d.kvh, combine_shares(static_cast<long long>(d.batch) * d.kvh, rows, a.sm)),
+                                dim3(128), 0, a.st, d, gangs));
+  ga::api::launches(3);
+  return 0;
+}
+
 // Prompts on the tensor cores; -1: the call is not one for them.
 template <class I>
 int run_tc(Launch& a, size_t ws_bytes) {
   PagedDev& d = a.d;
-  // its rows go through 16-byte copies, and it takes the maximum before the scale
-  if (d.kd || !(d.scale_log2 > 0.f) || d.q_s0 % 8 || d.q_s1 % 8 || reinterpret_cast<uintptr_t>(d.q) % 16) return -1;
+  if (!tc_takes(d)) return -1;
   const long long blocks = static_cast<long long>(d.total_q) * d.gqa / I::ROWS + d.batch;
-  const size_t need = 256 + static_cast<size_t>(blocks) * 8;
+  const size_t need = 256 + static_cast<size_t>(blocks) * 16;
   if (need > ws_bytes || blocks * d.kvh > 0x7fffffffLL) return -1;
   int* count = d.prefix;
-  int2* list = reinterpret_cast<int2*>(reinterpret_cast<uint8_t*>(d.prefix) + 256);
-  GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_prompts_kernel<I::ROWS>, dim3(1), dim3(1024), 0, a.st, d, count, list));
+  int4* list = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(d.prefix) + 256);
   const long long items = blocks * d.kvh;
   CUtensorMap maps[2];
-  std::memset(maps, 0, sizeof(maps));
-  const int page = d.page_mask + 1;
-  bool boxes = page >= 8 && d.num_pages > 0;
-  if (boxes) {
-    MapKey kk, vk;
-    std::memset(&kk, 0, sizeof(kk));
-    kk.base = d.k, kk.s_page = d.k_s0, kk.s_tok = d.k_s1, kk.s_head = d.k_s2;
-    kk.pages = d.num_pages, kk.page = page, kk.kvh = d.kvh, kk.hd = I::HD;
-    kk.box = page < ga::paged::tc::GK ? page : ga::paged::tc::GK;
-    vk = kk;
-    vk.base = d.v, vk.s_page = d.v_s0, vk.s_tok = d.v_s1, vk.s_head = d.v_s2;
-    boxes = pool_map(kk, &maps[0]) && pool_map(vk, &maps[1]);  // strides that a map cannot hold: without
-  }
+  const bool boxes = pool_maps<I>(d, maps);
+  GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_prompts_kernel<I::ROWS>, dim3(1), dim3(1024), 0, a.st, d, count, list));
   GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(static_cast<unsigned>(items < a.sm ? items : a.sm)), dim3(I::NT),
-                                I::SMEM, a.st, d, const_cast<const int*>(count), const_cast<const int2*>(list), maps[0], maps[1],
+                                I::SMEM, a.st, d, const_cast<const int*>(count), const_cast<const int4*>(list), maps[0], maps[1],
                                 static_cast<int>(boxes)));
   ga::api::launches(2);
   return 0;
@@ -136,12 +173,9 @@ int run(Launch& a) {
   const long long want = (tiles + d.walkers - 1) / d.walkers;
   const int grid = static_cast<int>(want < a.sm ? (want > 0 ? want : 1) : a.sm);
   GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 0>, dim3(grid), dim3(I::NT), I::SMEM, a.st, d));
-  // Enough CTAs to spread the rows of a small call over the SMs.
-  const long long pairs = units * d.hg;
   const int block_rows = rows < I::RC ? static_cast<int>(rows) : I::RC;
-  long long z = (2LL * a.sm + pairs - 1) / pairs;
-  if (z > block_rows) z = block_rows;
-  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_combine<I>, dim3(static_cast<unsigned>(units), d.hg, static_cast<unsigned>(z)),
+  const unsigned z = combine_shares(units * d.hg, block_rows, a.sm);
+  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_combine<I>, dim3(static_cast<unsigned>(units), d.hg, z),
                                 dim3(128), 0, a.st, d, grid * d.walkers));
   ga::api::launches(2);
   return 0;
@@ -150,9 +184,17 @@ int run(Launch& a) {
 template <int KV>
 int run_tc_kv(Launch& a, int hd, size_t ws_bytes) {
   using namespace ga::paged::tc;
-  if (hd == 64) return run_tc<TcInst<64, KV>>(a, ws_bytes);
-  if (hd == 128) return run_tc<TcInst<128, KV>>(a, ws_bytes);
-  return run_tc<TcInst<256, KV>>(a, ws_bytes);
+  if (hd == 64) return run_tc<TcInst<64, KV, false>>(a, ws_bytes);
+  if (hd == 128) return run_tc<TcInst<128, KV, false>>(a, ws_bytes);
+  return run_tc<TcInst<256, KV, false>>(a, ws_bytes);
+}
+
+template <int KV>
+int run_tc_split_kv(Launch& a, int hd) {
+  using namespace ga::paged::tc;
+  if (hd == 64) return run_tc_split<TcInst<64, KV, true>>(a);
+  if (hd == 128) return run_tc_split<TcInst<128, KV, true>>(a);
+  return run_tc_split<TcInst<256, KV, true>>(a);
 }
 
 template <int KV>
@@ -167,7 +209,8 @@ int run_kv(Launch& a, int hd) {
 template <int KV>
 int limits_tc_kv() {
   using namespace ga::paged::tc;
-  return limits_tc<TcInst<64, KV>>() || limits_tc<TcInst<128, KV>>() || limits_tc<TcInst<256, KV>>();
+  return limits_tc<TcInst<64, KV, true>>() || limits_tc<TcInst<128, KV, true>>() || limits_tc<TcInst<256, KV, true>>() ||
+         limits_tc<TcInst<64, KV, false>>() || limits_tc<TcInst<128, KV, false>>() || limits_tc<TcInst<256, KV, false>>();
 }
 
 template <int KV>
@@ -263,6 +306,13 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   if (l.prompt && a->kv_type != ga::paged::KV_E4M3) {
     const int rc = a->kv_type == ga::paged::KV_BF16 ? run_tc_kv<ga::paged::KV_BF16>(l, a->head_dim, a->workspace_bytes)
                                                     : run_tc_kv<ga::paged::KV_FP16>(l, a->head_dim, a->workspace_bytes);
+    if (rc >= 0) return rc;
+  }
+  const long long rows = static_cast<long long>(d.max_q) * d.gqa;
+  static const int tc_rows = [] { const char* e = std::getenv("GA_TC_ROWS"); return e ? std::atoi(e) : 17; }();
+  if (!l.prompt && a->kv_type != ga::paged::KV_E4M3 && rows >= tc_rows && rows <= ga::paged::tc::TM) {
+    const int rc = a->kv_type == ga::paged::KV_BF16 ? run_tc_split_kv<ga::paged::KV_BF16>(l, a->head_dim)
+                                                    : run_tc_split_kv<ga::paged::KV_FP16>(l, a->head_dim);
     if (rc >= 0) return rc;
   }
   if (a->kv_type == ga::paged::KV_BF16) return run_kv<ga::paged::KV_BF16>(l, a->head_dim);
