@@ -46,27 +46,29 @@ struct TcInst {
   static constexpr int KC = 8192 / HD;             // keys of a V stage
   static constexpr int ROWS = NQ * TM;
   static constexpr int Q_BYTES = NQ * SLABS * STAGE;
-  static constexpr int NST = HD == 256 ? 10 : (NQ == 1 ? 12 : (HD == 64 ? 8 : 10));
+  static constexpr int NST = HD == 64 ? (NQ == 1 ? 12 : 8) : 10;
   static constexpr int EG = SLABS < 2 ? SLABS : 2;  // stages that are filled and released together
-  static constexpr int SPLIT = 2;                   // threads that share a row
+  // Threads that share a row. With few rows only the warps of the first lanes have any (tensor memory lanes belong to the
+  // warps of one place in their group of four), so there more threads take part in a row.
+  static constexpr int SPLIT = SPLIT_KV && HD == 128 ? 4 : 2;  // (head_dim 256: no shared memory for it)
   static constexpr int SOFT_WARPS = 4 * NQ * SPLIT;
   // Gathering warps. A stage is always filled by the same warp: one that waits for use u of a stage to be released has
   // filled that use itself, so the barrier cannot be a whole phase behind the wait (stages are not released in ring order
   // when K and V are released by different lanes, and a parity cannot tell phase u - 2 from phase u).
   static constexpr int KV_WARPS = NST % 5 == 0 ? 5 : 4;
-  static constexpr int Q_WARPS = NQ == 1 ? 4 : 6 - KV_WARPS;
+  static constexpr int Q_WARPS = SOFT_WARPS == 16 ? 6 - KV_WARPS : 4;
   static_assert(NST % KV_WARPS == 0, "gathering warps");
   static constexpr int WARPS = (SOFT_WARPS + 2 + KV_WARPS + Q_WARPS + 3) / 4 * 4;  // whole warpgroups
   static constexpr int NT = WARPS * 32;
   // Registers a thread: what the block is launched with (limit of the launch bounds), and its split between the softmax
   // warps and the others. The shares add up to no more than the launch's.
-  static constexpr int REGS = NQ == 1 ? 96 : 80;
-  static constexpr int REGS_SOFT = NQ == 1 ? 128 : 96, REGS_REST = NQ == 1 ? 72 : 48;
+  static constexpr int REGS = SOFT_WARPS == 16 ? 80 : 96;
+  static constexpr int REGS_SOFT = SOFT_WARPS == 16 ? 96 : 128, REGS_REST = SOFT_WARPS == 16 ? 48 : 72;
   static_assert(SOFT_WARPS * REGS_SOFT + (WARPS - SOFT_WARPS) * REGS_REST <= WARPS * REGS, "register split");
   // Row maxima that the halves of a row exchange: at NQ 1 two jobs' in turn; at NQ 2 a query tile's next scores are ready
   // only after both halves are done with the job before.
   static constexpr int TURNS = 3 - NQ;
-  static constexpr int X_BYTES = 2 * 2 * TM * 4;
+  static constexpr int X_BYTES = (NQ == 1 ? 2 * SPLIT : 2 * 2) * TM * 4;
   // Operands first: they need the 1024-byte alignment that dynamic shared memory starts with (the kernel checks it).
   static constexpr int SMEM = Q_BYTES + NST * STAGE + X_BYTES + 512;
   static_assert(NST % EG == 0, "ring");
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     // ------------------------------------------------------------------------------------------ softmax, epilogue
     regs_up<I::REGS_SOFT>();
     constexpr int SPLIT = I::SPLIT, KEYS = TK / SPLIT, DIMS = HD / SPLIT;
-    const int g = warp / (4 * SPLIT), half = SPLIT == 2 ? (warp >> 2) & 1 : 0;  // query tile, part of its keys
+    const int g = warp / (4 * SPLIT), half = (warp >> 2) % SPLIT;  // query tile, part of its keys
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + lanes + I::O_COL + g * HD + half * DIMS;  // this thread's part of the output dims
@@ -475,14 +477,19 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     int n = NQ == 2 ? g : 0;  // running job
     int done = 0;             // items with jobs so far
     uint32_t turn = 0;
-    auto exchange = [&](float mine) {  // with the thread that has the row's other half
-      const uint32_t at = xm + turn * (2 * TM * 4);
+    auto exchange = [&](float mine, bool add) {  // maximum or sum over the threads that have the row's parts
+      const uint32_t at = xm + turn * (SPLIT * TM * 4);
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + half * (TM * 4)), "f"(mine) : "memory");
-      named_bar_sync(1 + g, 2 * TM);
-      float other;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(other) : "r"(at + (half ^ 1) * (TM * 4)) : "memory");
+      named_bar_sync(1 + g, SPLIT * TM);
+      float all = add ? 0.f : mine;
+#pragma unroll
+      for (int k = 0; k < SPLIT; ++k) {
+        float v;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at + k * (TM * 4)) : "memory");
+        all = add ? all + v : fmaxf(all, v);
+      }
       if (I::TURNS == 2) turn ^= 1;  // the slot is written again behind a barrier that its reader has passed
-      return other;
+      return all;
     };
     Work work = begin();
     Seg seg;
@@ -512,8 +519,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
 #pragma unroll
         for (int c = 0; c < KEYS / GK; ++c) base[c] = group_at(r, (seg.i0 + i) * (TK / GK) + half * (KEYS / GK) + c);
         float mx = part_max<KEYS>(tS, base, w);
-        if (SPLIT == 2) mx = fmaxf(mx, exchange(mx));
-        mx *= sl2;
+        mx = exchange(mx, false) * sl2;
         bool scale = false;
         float f = 1.f;
         if (mx > ref + RISE || (ref == -INFINITY && mx > ref)) {
@@ -546,11 +552,9 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(b_p + 8 * buf);
       }
-      if (SPLIT == 2) {
-        if (I::TURNS == 1) named_bar_sync(1 + g, 2 * TM);
-        sum += exchange(sum);
-        if (I::TURNS == 1) named_bar_sync(1 + g, 2 * TM);
-      }
+      if (I::TURNS == 1) named_bar_sync(1 + g, SPLIT * TM);
+      sum = exchange(sum, true);
+      if (I::TURNS == 1) named_bar_sync(1 + g, SPLIT * TM);
       const int qrow = r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
       uint8_t* dst = static_cast<uint8_t*>(p.out) +
                      (static_cast<long long>(qrow) * p.o_s0 + static_cast<long long>(qh) * p.o_s1 + half * DIMS) * 2;
