@@ -13,11 +13,11 @@
 // FP8 kernels next to this one).
 //
 // What bounds it: the cache's bytes. A warp owns one kv head and a private ring of tiles in shared memory that it fills
-// with 16-byte cp.async and drains itself, so there is no barrier between warps: the warps of a CTA walk the same
-// tokens, one kv head each, which makes the bytes of a token run contiguous in DRAM within a short window whatever the
-// page size (from one token up), strides and alignment. CTAs with fewer kv heads than warps are several walkers of HG
-// warps each ("virtual CTAs"). The call is one stream of tiles ordered by (request, head group, row block), cut evenly
-// over the walkers on the device from the live lengths; a unit that is cut leaves normalised 32-bit partials and their
+// with 16-byte cp.async and drains itself, so there is no barrier between warps: the kv_heads warps of a gang (neighbours
+// in the grid, whatever CTAs they are in) walk the same tokens, one kv head each, which makes the bytes of a token run
+// contiguous in DRAM within a short window whatever the page size (from one token up), strides and alignment. The call is
+// one stream of tiles ordered by (request, row block), cut evenly over the gangs on the device from the live lengths; a
+// unit that is cut leaves normalised 32-bit partials and their
 // log2 LSE in the workspace, folded in slice order by attn_paged_combine (no atomics: results do not depend on
 // scheduling).
 #pragma once
@@ -59,8 +59,7 @@ struct PagedDev {
   int total_q, batch, max_q;
   int window, sinks;  // window < 0: none (sinks is 0 then)
   float scale_log2;
-  int hg, groups, walkers;  // kv heads per walker, walkers' head groups per request, walkers per CTA
-  int nrb, upr;             // row blocks and units per request (split mode)
+  int nrb;           // row blocks = units of a request (split mode)
   int* status;
   int* prefix;
   float* ws_o;
@@ -112,19 +111,23 @@ __device__ __forceinline__ Req req_info(const PagedDev& p, int b, int t0, int nt
   return r;
 }
 
-// T tiles are cut over at most G walkers, each of which gets MIN_TILES tiles at least; first tile of walker c's slice.
+// T tiles are cut over at most G gangs, each of which gets MIN_TILES tiles at least; first tile of gang c's slice.
 constexpr int MIN_TILES = 2;
-__device__ __forceinline__ int walkers_for(long long T, int G) {
+__device__ __forceinline__ int gangs_for(long long T, int G) {
   const long long most = T / MIN_TILES;
   return most < G ? (most > 0 ? static_cast<int>(most) : 1) : G;
 }
-__device__ __forceinline__ long long slice(long long T, int G, int c) { return c >= G ? T : T * c / G; }
+__device__ __forceinline__ long long slice(long long T, int G, int c) {
+  if (c >= G) return T;
+  const unsigned long long x = static_cast<unsigned long long>(T) * c;
+  return x <= 0xffffffffull ? static_cast<unsigned>(x) / static_cast<unsigned>(G) : x / G;  // 32 bits: a third of the latency
+}
 
 // Exclusive prefix over the requests' counts, by the whole CTA (NT threads), and the request that holds item g0[s] for
-// each of the CTA's walkers s. find_b < 0: past the end. `publish`: this CTA writes p.prefix.
+// each of the gangs vc0 + s of the CTA's warps. find_b < 0: past the end. `publish`: this CTA writes p.prefix.
 template <int NT, typename CountFn>
 __device__ __forceinline__ long long plan(const PagedDev& p, CountFn count, int mul, long long (*g_of)(long long, int, int),
-                                          int G, int vc0, int walkers, int* find_b, long long* find_pre, bool publish) {
+                                          int G, int vc0, int gangs, int* find_b, long long* find_pre, bool publish) {
   __shared__ long long wsum[NT / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + NT - 1) / NT;
@@ -148,7 +151,7 @@ __device__ __forceinline__ long long plan(const PagedDev& p, CountFn count, int 
   }
   const long long T = total * mul;
   const long long pre = base + incl - mine;
-  for (int s = 0; s < walkers; ++s) {
+  for (int s = 0; s < gangs; ++s) {
     const long long g0 = g_of(T, G, vc0 + s);
     if (g0 < T && mine > 0 && pre * mul <= g0 && g0 < (pre + mine) * mul) {
       long long at = pre;
@@ -174,7 +177,7 @@ __device__ __forceinline__ long long plan(const PagedDev& p, CountFn count, int 
   __syncthreads();
   return T;
 }
-__device__ __forceinline__ long long at_cut(long long T, int G, int c) { return slice(T, walkers_for(T, G), c); }
+__device__ __forceinline__ long long at_cut(long long T, int G, int c) { return slice(T, gangs_for(T, G), c); }
 __device__ __forceinline__ long long at_index(long long, int, int c) { return c; }
 
 // ---------------------------------------------------------------------------------------------------- fragments
@@ -244,7 +247,7 @@ struct Inst {
 
 // A walker's place in the tile stream.
 struct Cursor {
-  int b, group, block;  // request, head group, row block
+  int b, block;    // request, row block
   Req r;
   int t, t_end;    // tiles of the current segment
   long long rem;   // tiles of the slice after this segment
@@ -271,22 +274,19 @@ __device__ __forceinline__ void advance(const PagedDev& p, Cursor& c) {
   c.first = false;
   if (++c.block == p.nrb) {
     c.block = 0;
-    if (++c.group == p.groups) {
-      c.group = 0;
-      do {
-        if (++c.b >= p.batch) {
-          c.live = false;
-          return;
-        }
-        c.r = req_info<I::T>(p, c.b, 0, p.max_q);
-      } while (c.r.cnt == 0);
-    }
+    do {
+      if (++c.b >= p.batch) {
+        c.live = false;
+        return;
+      }
+      c.r = req_info<I::T>(p, c.b, 0, p.max_q);
+    } while (c.r.cnt == 0);
   }
   open_segment<I, MODE>(p, c, 0);
 }
 
-// MODE 0: the tile stream cut evenly over all walkers (decode, verify). MODE 1: a walker takes one (row block, head
-// group) with the tiles that block sees (prompts; blocks from the last to the first, the longest first).
+// MODE 0: the tile stream cut evenly over all gangs (decode, verify). MODE 1: a gang takes one row block with the tiles that
+// block sees (prompts; blocks from the last to the first, the longest first).
 template <class I, int MODE>
 __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_constant__ PagedDev p) {
   constexpr int T = I::T, RB = I::RB, HD = I::HD, KV = I::KV, MT = I::MT;
@@ -294,8 +294,13 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
   __shared__ int find_b[MAX_WARPS];
   __shared__ long long find_pre[MAX_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int walker = warp / p.hg;
-  const int vc = blockIdx.x * p.walkers + walker, G = gridDim.x * p.walkers;
+  // This warp's gang and kv head, and the gangs that the CTA's warps belong to (the grid's last, incomplete one is left out).
+  const long long w0 = static_cast<long long>(blockIdx.x) * I::NW;
+  const int G = static_cast<int>(static_cast<long long>(gridDim.x) * I::NW / p.kvh);
+  const int vc0 = static_cast<int>(w0 / p.kvh), vc = static_cast<int>((w0 + warp) / p.kvh);
+  const int h = static_cast<int>(w0 + warp - static_cast<long long>(vc) * p.kvh);
+  const int gangs = min(static_cast<int>((w0 + I::NW - 1) / p.kvh), G - 1) - vc0 + 1;
+  const int me = vc - vc0;
   const int g = lane >> 2, tq = lane & 3;
   grid_dep_wait();
   grid_dep_launch();
@@ -303,18 +308,17 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
   Cursor ci;
   ci.live = false;
   if (MODE == 0) {
-    const long long total = plan<I::NT>(p, [&](int b) { return req_info<T>(p, b, 0, p.max_q).cnt; }, p.upr, at_cut, G,
-                                        blockIdx.x * p.walkers, p.walkers, find_b, find_pre, blockIdx.x == 0);
-    if (walker >= p.walkers || find_b[walker] < 0) return;
-    const int used = walkers_for(total, G);
+    const long long total = plan<I::NT>(p, [&](int b) { return req_info<T>(p, b, 0, p.max_q).cnt; }, p.nrb, at_cut, G, vc0,
+                                        gangs, find_b, find_pre, blockIdx.x == 0);
+    if (vc >= G || find_b[me] < 0) return;
+    const int used = gangs_for(total, G);
     const long long g0 = slice(total, used, vc), g1 = slice(total, used, vc + 1);
     if (g1 <= g0) return;
-    ci.b = find_b[walker];
+    ci.b = find_b[me];
     ci.r = req_info<T>(p, ci.b, 0, p.max_q);
-    const long long in = g0 - find_pre[walker] * p.upr;
+    const long long in = g0 - find_pre[me] * p.nrb;
     const int unit = static_cast<int>(in / ci.r.cnt);
-    ci.group = unit / p.nrb;
-    ci.block = unit - ci.group * p.nrb;
+    ci.block = unit;
     ci.rem = g1 - g0;
     ci.live = ci.first = true;
     open_segment<I, MODE>(p, ci, static_cast<int>(in - static_cast<long long>(unit) * ci.r.cnt));
@@ -324,19 +328,17 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
       const int ql = new_tokens(p, b, q0);
       return ql > 0 ? static_cast<int>((static_cast<long long>(min(ql, p.max_q)) * p.gqa + I::RC - 1) / I::RC) : 0;
     };
-    const long long total = plan<I::NT>(p, blocks, 1, at_index, G, blockIdx.x * p.walkers, p.walkers, find_b, find_pre, false);
-    if (walker >= p.walkers || find_b[walker] < 0 || vc >= total) return;
-    ci.b = find_b[walker];
-    ci.block = blocks(ci.b) - 1 - static_cast<int>(vc - find_pre[walker]);
+    const long long total = plan<I::NT>(p, blocks, 1, at_index, G, vc0, gangs, find_b, find_pre, false);
+    if (vc >= G || vc >= total || find_b[me] < 0) return;
+    ci.b = find_b[me];
+    ci.block = blocks(ci.b) - 1 - static_cast<int>(vc - find_pre[me]);
     const int t0 = ci.block * I::RC / p.gqa, t1 = (ci.block * I::RC + I::RC - 1) / p.gqa;
     ci.r = req_info<T>(p, ci.b, t0, t1 - t0 + 1);
-    ci.group = blockIdx.y;
     ci.rem = ci.r.cnt;
     ci.live = ci.r.cnt > 0;
     open_segment<I, MODE>(p, ci, 0);
   }
 
-  const int hl = warp - walker * p.hg;
   const uint32_t ring = smem_u32(smem_raw) + warp * (I::NST * I::STAGE);
 
   // Page of this lane's token of the tile the cursor stands on; -1 where no row sees the token (its page-table entry
@@ -354,19 +356,17 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
   };
   auto issue = [&](const Cursor& c, int pages, int stage) {
     if (c.live) {
-      const int h = c.group * p.hg + hl;
       const int n0 = (c.t < c.r.ns ? c.t : c.r.tlo + c.t - c.r.ns) * T;
       const uint32_t dst = ring + stage * I::STAGE;
       constexpr int RPI = 32 / I::CPR;  // rows per instruction
       const int chunk = lane % I::CPR;
-      const bool head_real = h < p.kvh;
-      const uint8_t* kb = p.k + (head_real ? h * p.k_s2 : 0) + chunk * 16;
-      const uint8_t* vb = p.v + (head_real ? h * p.v_s2 : 0) + chunk * 16;
+      const uint8_t* kb = p.k + h * p.k_s2 + chunk * 16;
+      const uint8_t* vb = p.v + h * p.v_s2 + chunk * 16;
 #pragma unroll
       for (int it = 0; it < T / RPI; ++it) {
         const int row = it * RPI + lane / I::CPR;
         const int page = __shfl_sync(0xffffffffu, pages, row);
-        const bool real = page >= 0 && head_real;
+        const bool real = page >= 0;
         const long long pg = real ? page : 0, tk = real ? ((n0 + row) & p.page_mask) : 0;
         const uint32_t d = dst + swz<RB>(row, chunk);
         cp_async_16_or_zero(d, kb + pg * p.k_s0 + tk * p.k_s1, real);
@@ -396,11 +396,10 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
   const bool blank = MODE == 1 && !cc.live;
   while (cc.live || (blank && fresh)) {
     const int block = cc.block;
-    const int h = cc.group * p.hg + hl;
     const int rows = cc.r.nq * p.gqa - block * I::RC;  // rows of this block, may exceed RC
     if (fresh) {
       fresh = false;
-      sl2 = p.scale_log2 * (p.kd && h < p.kvh ? p.kd[cc.b * p.kd_s0 + h * p.kd_s1] : 1.f);
+      sl2 = p.scale_log2 * (p.kd ? p.kd[cc.b * p.kd_s0 + h * p.kd_s1] : 1.f);
       pos_first = cc.r.pos0 + block * I::RC / p.gqa;
       pos_last = cc.r.pos0 + (block * I::RC + min(rows, I::RC) - 1) / p.gqa;
 #pragma unroll
@@ -408,7 +407,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
           const int row = mt * 16 + hf * 8 + g;
-          const bool real = row < rows && h < p.kvh;
+          const bool real = row < rows;
           const int rr = block * I::RC + row;
           const int tok = rr / p.gqa;
           pos[mt][hf] = real ? cc.r.pos0 + tok : -1;
@@ -586,8 +585,8 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
       last = cc.t + 1 >= cc.t_end;
     }
     if (last) {
-      const float vds = p.vd && h < p.kvh ? p.vd[cc.b * p.vd_s0 + h * p.vd_s1] : 1.f;
-      const int slot = 2 * (blockIdx.x * p.walkers + walker) + (cc.first ? 0 : 1);
+      const float vds = p.vd ? p.vd[cc.b * p.vd_s0 + h * p.vd_s1] : 1.f;
+      const int slot = 2 * vc + (cc.first ? 0 : 1);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -596,11 +595,11 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
           const int row = mt * 16 + hf * 8 + g;
-          if (row >= rows || h >= p.kvh) continue;
+          if (row >= rows) continue;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
           const float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + lg2(sum);
           if (MODE == 0 && !cc.whole) {
-            const long long wr = (static_cast<long long>(slot) * p.hg + hl) * I::RC + row;
+            const long long wr = (static_cast<long long>(slot) * p.kvh + h) * I::RC + row;
             float* w = p.ws_o + wr * HD;
 #pragma unroll
             for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
@@ -641,20 +640,19 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
 }
 
 // Folds the pieces of every unit that the main kernel cut, in slice order, and writes the rows of requests without
-// visible keys. grid = (batch * upr, heads of a group, row shares); 4 warps. A row's pieces are spread over the warps
+// visible keys. grid = (batch * nrb, kv heads, row shares); 4 warps. A row's pieces are spread over the warps
 // when there are many of them (one long sequence), the rows are when there are few.
 template <class I>
 __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant__ PagedDev p, int G) {
   constexpr int HD = I::HD, VEC = HD / 32, UNR = 8;
-  const int b = blockIdx.x / p.upr, j = blockIdx.x - b * p.upr;
-  const int group = j / p.nrb, block = j - group * p.nrb;
-  const int h = group * p.hg + blockIdx.y;
+  const int b = blockIdx.x / p.nrb, block = blockIdx.x - b * p.nrb;
+  const int h = blockIdx.y;
   const Req r = I::req(p, b);
   const int rows = min(r.nq * p.gqa - block * I::RC, I::RC);
-  const float vds = p.vd && h < p.kvh ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
+  const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
   grid_dep_wait();
   grid_dep_launch();
-  if (rows <= 0 || h >= p.kvh) return;
+  if (rows <= 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto store = [&](int row, const float (&v)[VEC], float f, float lse2) {
     const int rr = block * I::RC + row, tok = rr / p.gqa;
@@ -671,21 +669,22 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
     for (int row = blockIdx.z * 4 + warp; row < rows; row += 4 * share) store(row, zero, 0.f, -INFINITY);
     return;
   }
-  const long long total = static_cast<long long>(p.prefix[p.batch]) * p.upr;
-  G = walkers_for(total, G);
-  const long long u0 = static_cast<long long>(p.prefix[b]) * p.upr + static_cast<long long>(j) * r.cnt, u1 = u0 + r.cnt;
-  auto owner = [&](long long x) {  // the walker whose slice holds tile x
-    long long c = ((x + 1) * G - 1) / total;
+  const long long total = static_cast<long long>(p.prefix[p.batch]) * p.nrb;
+  G = gangs_for(total, G);
+  const long long u0 = static_cast<long long>(p.prefix[b]) * p.nrb + static_cast<long long>(block) * r.cnt, u1 = u0 + r.cnt;
+  auto owner = [&](long long x) {  // the gang whose slice holds tile x
+    const unsigned long long at = static_cast<unsigned long long>(x + 1) * G - 1;
+    long long c = at <= 0xffffffffull && total <= 0xffffffffll ? static_cast<unsigned>(at) / static_cast<unsigned>(total) : at / total;
     while (c > 0 && slice(total, G, static_cast<int>(c)) > x) --c;
     while (c < G - 1 && slice(total, G, static_cast<int>(c) + 1) <= x) ++c;
     return static_cast<int>(c);
   };
   const int c0 = owner(u0), c1 = owner(u1 - 1);
   if (c0 == c1) return;
-  const int n = c1 - c0 + 1;  // every walker between them holds a piece too
+  const int n = c1 - c0 + 1;  // every gang between them holds a piece too
   const int e0 = u0 <= slice(total, G, c0) ? 0 : 1;
   auto piece = [&](int i) {  // workspace row 0 of the unit's piece i
-    return (static_cast<long long>(2 * (c0 + i) + (i == 0 ? e0 : 0)) * p.hg + blockIdx.y) * I::RC;
+    return (static_cast<long long>(2 * (c0 + i) + (i == 0 ? e0 : 0)) * p.kvh + h) * I::RC;
   };
   __shared__ float red_o[4][HD], red_m[4], red_l[4];
   const bool many = n > UNR;

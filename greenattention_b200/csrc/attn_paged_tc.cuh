@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(1024) plan_split_kernel(const __grid_constant_
   }
   if (tid == 0) p.prefix[p.batch] = static_cast<int>(total);
   __syncthreads();
-  const int used = walkers_for(total, G);
+  const int used = gangs_for(total, G);
   for (int g = tid; g < G; g += 1024) {
     const long long g0 = slice(total, used, g), g1 = slice(total, used, g + 1);
     int4 e = make_int4(0, 0, 0, 0);

@@ -111,7 +111,7 @@ int run_tc_split(Launch& a) {
   CUtensorMap maps[2];
   const bool boxes = pool_maps<I>(d, maps);
   const int gangs = a.sm / d.kvh;
-  d.hg = d.kvh, d.groups = 1, d.nrb = 1, d.upr = 1, d.walkers = 1;
+  d.nrb = 1;
   int4* list = reinterpret_cast<int4*>(d.ws_lse + static_cast<size_t>(2 * a.sm) * ga::paged::tc::TM);
   static_assert(ga::paged::SLOT_ROWS >= ga::paged::tc::TM + 16 && I::HD * ga::paged::tc::TM <= ga::paged::SLOT_FLOATS, "workspace");
   GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_split_kernel<I>, dim3(1), dim3(1024), 0, a.st, d, gangs, list));
@@ -149,34 +149,30 @@ template <class I>
 int run(Launch& a) {
   PagedDev& d = a.d;
   static_assert(I::NW * I::RC * I::HD <= ga::paged::SLOT_FLOATS && I::NW * I::RC <= ga::paged::SLOT_ROWS, "slot");
-  d.groups = (d.kvh + I::NW - 1) / I::NW;
-  d.hg = (d.kvh + d.groups - 1) / d.groups;
-  d.walkers = I::NW / d.hg;
+  if (d.kvh > a.sm * I::NW) return fail("%d kv heads: more than a gang can hold", d.kvh);
   const long long rows = static_cast<long long>(d.max_q) * d.gqa;
   if (a.prompt) {
     // a request of n tokens has ceil(n * gqa / RC) row blocks
     const long long blocks = static_cast<long long>(d.total_q) * d.gqa / I::RC + d.batch;
-    const long long grid = (blocks + d.walkers - 1) / d.walkers;
-    if (grid > 0x7fffffffLL || d.groups > 65535) return fail("too many row blocks");
+    const long long grid = (blocks * d.kvh + I::NW - 1) / I::NW;
+    if (grid > 0x7fffffffLL || blocks > 0x7fffffffLL) return fail("too many row blocks");
     d.nrb = 1;
-    d.upr = d.groups;
-    GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 1>, dim3(static_cast<unsigned>(grid), d.groups), dim3(I::NT),
-                                  I::SMEM, a.st, d));
+    GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 1>, dim3(static_cast<unsigned>(grid)), dim3(I::NT), I::SMEM, a.st, d));
     ga::api::launches(1);
     return 0;
   }
   d.nrb = static_cast<int>((rows + I::RC - 1) / I::RC);
-  d.upr = d.groups * d.nrb;
-  const long long units = static_cast<long long>(d.batch) * d.upr;
-  const long long tiles = units * ((a.max_tokens + I::T - 1) / I::T);
-  if (units > 0x7fffffffLL) return fail("too many (request, head group, row block) units");
-  const long long want = (tiles + d.walkers - 1) / d.walkers;
-  const int grid = static_cast<int>(want < a.sm ? (want > 0 ? want : 1) : a.sm);
+  const long long units = static_cast<long long>(d.batch) * d.nrb;
+  if (units > 0x7fffffffLL) return fail("too many (request, row block) units");
+  const long long tiles = units * ((a.max_tokens + I::T - 1) / I::T);  // at most, of each kv head
+  const long long want = (tiles * d.kvh + I::NW - 1) / I::NW;
+  const int least = (d.kvh + I::NW - 1) / I::NW;
+  const int grid = static_cast<int>(want < least ? least : (want < a.sm ? want : a.sm));
   GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 0>, dim3(grid), dim3(I::NT), I::SMEM, a.st, d));
   const int block_rows = rows < I::RC ? static_cast<int>(rows) : I::RC;
-  const unsigned z = combine_shares(units * d.hg, block_rows, a.sm);
-  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_combine<I>, dim3(static_cast<unsigned>(units), d.hg, z),
-                                dim3(128), 0, a.st, d, grid * d.walkers));
+  const unsigned z = combine_shares(units * d.kvh, block_rows, a.sm);
+  GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_combine<I>, dim3(static_cast<unsigned>(units), d.kvh, z), dim3(128), 0, a.st, d,
+                                grid * I::NW / d.kvh));
   ga::api::launches(2);
   return 0;
 }
