@@ -126,12 +126,14 @@ __device__ __forceinline__ long long slice(long long T, int G, int c) {
 // Exclusive prefix over the requests' counts, by the whole CTA (NT threads), and the request that holds item g0[s] for
 // each of the gangs vc0 + s of the CTA's warps. find_b < 0: past the end. `publish`: this CTA writes p.prefix.
 template <int NT, typename CountFn>
-__device__ __forceinline__ long long plan(const PagedDev& p, CountFn count, int mul, long long (*g_of)(long long, int, int),
+__device__ __forceinline__ long long plan(const PagedDev& p, CountFn count_of, int mul, long long (*g_of)(long long, int, int),
                                           int G, int vc0, int gangs, int* find_b, long long* find_pre, bool publish) {
   __shared__ long long wsum[NT / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.batch + NT - 1) / NT;
   const int b0 = min(p.batch, tid * per), b1 = min(p.batch, b0 + per);
+  const int first = b0 < b1 ? count_of(b0) : 0;  // a thread's first request, the only one in most calls, is read once
+  auto count = [&](int b) { return b == b0 ? first : count_of(b); };
   long long mine = 0;
   for (int b = b0; b < b1; ++b) mine += count(b);
   long long incl = mine;
@@ -341,21 +343,23 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
 
   const uint32_t ring = smem_u32(smem_raw) + warp * (I::NST * I::STAGE);
 
-  // Page of this lane's token of the tile the cursor stands on; -1 where no row sees the token (its page-table entry
-  // may be a released page's, or padding) or the page does not exist: such rows are filled with zeros.
+  // Page of this lane's token of the tile the cursor stands on; UNSEEN where no row sees the token (its page-table entry may
+  // be a released page's, or padding). It is looked at when the tile is issued, an iteration later, so that the load has
+  // that long: a check here cost every tile the latency of a load. Unseen rows, and those of pages that do not exist, are
+  // filled with zeros.
+  constexpr int UNSEEN = static_cast<int>(0x80000000);
   auto fetch_pages = [&](const Cursor& c) -> int {
-    if (!c.live || lane >= T) return -1;
+    if (!c.live || lane >= T) return UNSEEN;
     const int n = (c.t < c.r.ns ? c.t : c.r.tlo + c.t - c.r.ns) * T + lane;
-    if (n >= c.r.kend || (n < c.r.lower && n >= p.sinks)) return -1;
-    const int page = p.pt[c.b * p.pt_s0 + (n >> p.page_shift) * p.pt_s1];
-    if (page < 0 || page >= p.num_pages) {
-      atomicExch(p.status, GA_ST_BAD_PAGE);
-      return -1;
-    }
-    return page;
+    if (n >= c.r.kend || (n < c.r.lower && n >= p.sinks)) return UNSEEN;
+    return p.pt[c.b * p.pt_s0 + (n >> p.page_shift) * p.pt_s1];
   };
   auto issue = [&](const Cursor& c, int pages, int stage) {
     if (c.live) {
+      if (static_cast<unsigned>(pages) >= static_cast<unsigned>(p.num_pages)) {
+        if (pages != UNSEEN) atomicExch(p.status, GA_ST_BAD_PAGE);
+        pages = -1;
+      }
       const int n0 = (c.t < c.r.ns ? c.t : c.r.tlo + c.t - c.r.ns) * T;
       const uint32_t dst = ring + stage * I::STAGE;
       constexpr int RPI = 32 / I::CPR;  // rows per instruction
