@@ -7,8 +7,10 @@
 // with integer atomics, whose order does not matter).
 //
 // What bounds it: the bytes of the copied tokens, read once and written once. The decisions (a few integers per row,
-// one count per page) are made by small kernels in front; a copy kernel then moves 16 KB pieces of pages, all layers
-// of all pairs in one launch, with enough CTAs per SM that a piece's chain of descriptor reads hides behind the others'.
+// one count per page) are made by small kernels in front; a copy kernel then moves pieces of pages of up to 16 KB, all
+// layers of all pairs in one launch. A CTA takes a contiguous range of the pieces and one of its threads streams them
+// through shared memory with bulk copies (global to shared, shared to global), up to three loads ahead of the stores, so
+// that the reads of a piece's descriptors hide behind the pieces in flight.
 #pragma once
 
 #include "ga_common.cuh"
@@ -19,7 +21,10 @@ namespace pages {
 enum : int { ST_BAD_PAGE = GA_ST_BAD_PAGE, ST_LEN_RANGE = GA_ST_LEN_RANGE, ST_BAD_INDEX = 7, ST_NO_PAGES = 8, ST_REFS = 9, ST_CLASH = 10 };
 
 constexpr int CHUNK = 16384;      // bytes of a copy item
-constexpr int COPY_THREADS = 256;
+constexpr int COPY_THREADS = 128;
+constexpr int COPY_SLOTS = 4;    // pieces of a CTA in shared memory
+constexpr int COPY_CTAS = 3;     // CTAs per SM
+constexpr int COPY_SMEM = COPY_SLOTS * CHUNK;
 constexpr int PLAN_THREADS = 1024;
 constexpr int SPAN = 16384;       // pages that a CTA looks through at a time (16 per thread)
 
@@ -73,29 +78,87 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
 
 // ------------------------------------------------------------------------------------------------------ copying
 
-// One 16 KB piece (or what `tokens` leaves of it) of one tensor's page.
-__device__ __forceinline__ void copy_piece(const PoolDev& p, int c, int src, int dst, int tokens) {
-  const int t = p.chunk_tensor[c];
-  const long long stride = p.stride[t];
-  const int off = (c - p.chunk_first[t]) * CHUNK;
-  int n = tokens * p.tok_bytes[t] - off;
-  if (n <= 0) return;
-  if (n > CHUNK) n = CHUNK;
-  const uint8_t* base = reinterpret_cast<const uint8_t*>(p.base[t]);
-  const uint4* s = reinterpret_cast<const uint4*>(base + src * stride + off);
-  uint4* d = reinterpret_cast<uint4*>(const_cast<uint8_t*>(base) + dst * stride + off);
-  const int vecs = n >> 4;
-  constexpr int U = CHUNK / 16 / COPY_THREADS;
-  uint4 v[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * COPY_THREADS + threadIdx.x;
-    if (i < vecs) v[u] = __ldcs(s + i);
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, int bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ int pieces(const PoolDev& p, int t, int tokens) { return (tokens * p.tok_bytes[t] + CHUNK - 1) / CHUNK; }
+
+// Pieces [from, to) of the call by one thread. Pair i is `pair(i, src, dst, tokens)`: false for one that is not carried
+// out; its pieces are those of `tokens` tokens of every tensor, tensor by tensor; (i0, skip): the pair that holds piece
+// `from` and how many of its pieces come before. `ring`: COPY_SMEM bytes, `bars`: COPY_SLOTS initialised barriers.
+template <typename Pair>
+__device__ __forceinline__ void copy_pieces(const PoolDev& p, long long from, long long to, int i0, long long skip, Pair pair, uint32_t ring,
+                                            uint32_t bars) {
+  if (from >= to) return;
+  int i = i0, t = 0, src, dst, tokens;
+  bool real = pair(i, src, dst, tokens);
+  int per = pieces(p, 0, tokens);
+  while (skip >= per) {
+    skip -= per;
+    per = pieces(p, ++t, tokens);
   }
+  int c = static_cast<int>(skip);
+  uint8_t* to_at[COPY_SLOTS];
+  int size[COPY_SLOTS];
+  int loads = 0, stores = 0;  // pieces so far
+  bool failed = false;
+  auto store = [&]() {  // the oldest piece that has not been stored; after a wait that ran out pieces are only waited for
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = u * COPY_THREADS + threadIdx.x;
-    if (i < vecs) __stcs(d + i, v[u]);
+    for (int k = 0; k < COPY_SLOTS; ++k)
+      if (k == stores % COPY_SLOTS) {
+        if (!mbar_wait(bars + 8 * k, (stores / COPY_SLOTS) & 1)) {
+          failed = true;
+          flag(p, GA_ST_WAIT_FULL);
+        }
+        if (!failed) bulk_store(to_at[k], ring + k * CHUNK, size[k]);
+      }
+    ++stores;
+  };
+  for (long long at = from; at < to && !failed; ++at) {
+    if (real) {
+      const int off = c * CHUNK;
+      const int n = min(tokens * p.tok_bytes[t] - off, CHUNK);
+      const long long stride = p.stride[t];
+      uint8_t* base = reinterpret_cast<uint8_t*>(p.base[t]) + off;
+      // the slot's last piece was stored two turns ago: at most the store behind it may still be reading
+      if (loads >= COPY_SLOTS) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+#pragma unroll
+      for (int k = 0; k < COPY_SLOTS; ++k)
+        if (k == loads % COPY_SLOTS) {
+          to_at[k] = base + dst * stride;
+          size[k] = n;
+          mbar_expect_tx(bars + 8 * k, n);
+          bulk_load(ring + k * CHUNK, base + src * stride, n, bars + 8 * k);
+        }
+      ++loads;
+      if (loads - stores == COPY_SLOTS - 1) store();
+    }
+    if (++c == per) {
+      c = 0;
+      do {
+        if (++t == p.tensors) {
+          t = 0;
+          if (at + 1 >= to) break;
+          do real = pair(++i, src, dst, tokens);
+          while (tokens <= 0);  // pairs without pieces
+        }
+        per = pieces(p, t, tokens);
+      } while (per == 0);
+    }
+  }
+  while (stores < loads) store();
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+// A CTA's barriers; the thread that copies is thread 0.
+__device__ __forceinline__ void copy_setup(uint32_t bars) {
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < COPY_SLOTS; ++k) mbar_init(bars + 8 * k, 1);
+    mbar_fence_init();
   }
 }
 
@@ -137,14 +200,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) copy_plan_kernel(const __grid_co
 }
 
 __global__ void __launch_bounds__(COPY_THREADS) copy_kernel(const __grid_constant__ PoolDev p, const int2* list, int n) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t bars[COPY_SLOTS];
+  copy_setup(smem_u32(bars));
   grid_dep_wait();
   grid_dep_launch();
-  const long long items = static_cast<long long>(n) * p.chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    const int i = static_cast<int>(it / p.chunks), c = static_cast<int>(it - static_cast<long long>(i) * p.chunks);
-    const int2 pair = list[i];
-    if (pair.x >= 0) copy_piece(p, c, pair.x, pair.y, p.page_size);
-  }
+  if (threadIdx.x != 0) return;
+  const long long all = static_cast<long long>(n) * p.chunks;
+  const long long from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
+  copy_pieces(p, from, to, static_cast<int>(from / p.chunks), from % p.chunks, [&](int i, int& src, int& dst, int& tokens) {
+    const int2 e = list[i];
+    src = e.x, dst = e.y, tokens = p.page_size;
+    return e.x >= 0;
+  }, smem_u32(ring), smem_u32(bars));
 }
 
 // ---------------------------------------------------------------------------------------------------- releasing
@@ -316,11 +384,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) grow_kernel(const __grid_constan
 
 // ------------------------------------------------------------------------------------------------------ forking
 
-// list[i] = (source of the partial last page or -1, its copy, tokens of the parent, 1 if the pair is carried out). A
-// child is an empty row that the call names once; a parent is taken as it was before the call. One CTA; dynamic shared
-// memory: n ints.
+// list[i] = (source of the partial last page or -1, its copy, tokens of the parent, 1 if the pair is carried out), ends[i]
+// = pieces to copy of the pairs up to i. A child is an empty row that the call names once; a parent is taken as it was
+// before the call. One CTA; dynamic shared memory: n ints.
 __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const __grid_constant__ PoolDev p, const void* parents,
-                                                                 const void* children, int is64, int n, int* mark, int4* list) {
+                                                                 const void* children, int is64, int n, int* mark, int4* list,
+                                                                 int* ends) {
   extern __shared__ int incl[];
   __shared__ int tmp[33];
   grid_dep_wait();
@@ -375,42 +444,59 @@ __global__ void __launch_bounds__(PLAN_THREADS) fork_plan_kernel(const __grid_co
     list[i].y = page;
   });
   __syncthreads();
-  for (int i = threadIdx.x; i < n; i += PLAN_THREADS) {
-    int4 e = list[i];
-    if (e.x >= 0 && e.y < 0) {  // no page left for its copy
-      flag(p, ST_NO_PAGES);
-      e = make_int4(-1, -1, 0, 0);
-      list[i] = e;
+  int before_all = 0;
+  for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
+    const int i = i0 + threadIdx.x;
+    int count = 0;
+    if (i < n) {
+      int4 e = list[i];
+      if (e.x >= 0 && e.y < 0) {  // no page left for its copy
+        flag(p, ST_NO_PAGES);
+        e = make_int4(-1, -1, 0, 0);
+        list[i] = e;
+      }
+      if (e.w) p.lens[child_of(i)] = e.z;
+      if (e.x >= 0)
+        for (int t = 0; t < p.tensors; ++t) count += pieces(p, t, e.z & (p.page_size - 1));
     }
-    if (e.w) p.lens[child_of(i)] = e.z;
+    int total;
+    const int before = block_scan<PLAN_THREADS>(count, tmp, total);
+    if (i < n) ends[i] = before_all + before + count;
+    before_all += total;
   }
 }
 
-// Items 0 .. n - 1: the pair's full pages are shared; the rest: pieces of the partial pages.
+// The pairs' full pages are shared (all threads), then the tokens of the partial pages copied.
 __global__ void __launch_bounds__(COPY_THREADS) fork_apply_kernel(const __grid_constant__ PoolDev p, const void* parents,
-                                                                  const void* children, int is64, int n, const int4* list) {
+                                                                  const void* children, int is64, int n, const int4* list,
+                                                                  const int* ends) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t bars[COPY_SLOTS];
+  copy_setup(smem_u32(bars));
   grid_dep_wait();
   grid_dep_launch();
-  const long long items = n + static_cast<long long>(n) * p.chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    if (it < n) {
-      const int i = static_cast<int>(it);
-      const int4 e = list[i];
-      if (!e.w) continue;
-      const int* from = p.table + index_at(parents, is64, i) * p.t_s0;
-      int* to = p.table + index_at(children, is64, i) * p.t_s0;
-      for (int j = threadIdx.x; j < e.z >> p.page_shift; j += COPY_THREADS) {
-        const int page = from[j * p.t_s1];
-        to[j * p.t_s1] = page;
-        if (page >= p.num_pages) flag(p, ST_BAD_PAGE);
-        else if (page >= 0) atomicAdd(p.refs + page, 1);
-      }
-    } else {
-      const int i = static_cast<int>((it - n) / p.chunks), c = static_cast<int>((it - n) - static_cast<long long>(i) * p.chunks);
-      const int4 e = list[i];
-      if (e.x >= 0) copy_piece(p, c, e.x, e.y, e.z & (p.page_size - 1));
+  for (int i = blockIdx.x; i < n; i += gridDim.x) {
+    const int4 e = list[i];
+    if (!e.w) continue;
+    const int* from = p.table + index_at(parents, is64, i) * p.t_s0;
+    int* to = p.table + index_at(children, is64, i) * p.t_s0;
+    for (int j = threadIdx.x; j < e.z >> p.page_shift; j += COPY_THREADS) {
+      const int page = from[j * p.t_s1];
+      to[j * p.t_s1] = page;
+      if (page >= p.num_pages) flag(p, ST_BAD_PAGE);
+      else if (page >= 0) atomicAdd(p.refs + page, 1);
     }
   }
+  if (threadIdx.x != 0) return;
+  const long long all = ends[n - 1];
+  const long long from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
+  if (from >= to) return;
+  const int i0 = holder(ends, n, static_cast<int>(from));
+  copy_pieces(p, from, to, i0, from - (i0 ? ends[i0 - 1] : 0), [&](int i, int& src, int& dst, int& tokens) {
+    const int4 e = list[i];
+    src = e.x, dst = e.y, tokens = e.x >= 0 ? e.z & (p.page_size - 1) : 0;
+    return e.x >= 0;
+  }, smem_u32(ring), smem_u32(bars));
 }
 
 // --------------------------------------------------------------------------------------------------- compacting
@@ -449,11 +535,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_rank_kernel(const __grid
   grid_dep_launch();
   const int tid = threadIdx.x;
   int mine = 0, before = 0;
-  for (int s = tid; s < static_cast<int>(gridDim.x); s += PLAN_THREADS) {
+  for (int s = tid; s < static_cast<int>(gridDim.x) && gridDim.x > 1; s += PLAN_THREADS) {
     mine += counts[s];
     if (s < static_cast<int>(blockIdx.x)) before += counts[s];
   }
   int L, B;
+  if (gridDim.x == 1) mine = __popc(live_bits(p, tid * 16));  // a pool of one span is counted here
   block_scan<PLAN_THREADS>(mine, tmp, L);
   block_scan<PLAN_THREADS>(before, tmp, B);
   if (tid == 0) below = B;
@@ -494,41 +581,44 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_rank_kernel(const __grid
     }
   }
 }
-// Rewrites the page table, moves the counts and copies the pages.
+// Rewrites the page table, moves the counts (all threads), then copies the pages.
 __global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(const __grid_constant__ PoolDev p, int* map, const int* movers,
                                                                      const int* gaps, const int* moved) {
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ __align__(8) uint64_t bars[COPY_SLOTS];
+  copy_setup(smem_u32(bars));
   grid_dep_wait();
   grid_dep_launch();
   const int n = *moved;
-  const long long items = p.rows + static_cast<long long>(n) * p.chunks;
-  for (long long it = blockIdx.x; it < items; it += gridDim.x) {
-    if (it < p.rows) {
-      const int row = static_cast<int>(it);
-      const int held = min(pages_of(p, p.lens[row]), p.cols);
-      int* t = p.table + row * p.t_s0;
-      for (int j = threadIdx.x; j < held; j += COPY_THREADS) {
-        const int page = t[j * p.t_s1];
-        if (page < 0) continue;
-        if (page >= p.num_pages) {
-          flag(p, ST_BAD_PAGE);
-          continue;
-        }
-        const int to = __ldcg(map + page);
-        if (to == -1) flag(p, ST_REFS);  // the books say that the page is free: left alone
-        else if (to <= -2) t[j * p.t_s1] = gaps[-2 - to];
-        else if (to != page) t[j * p.t_s1] = to;
+  for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const int held = min(pages_of(p, p.lens[row]), p.cols);
+    int* t = p.table + row * p.t_s0;
+    for (int j = threadIdx.x; j < held; j += COPY_THREADS) {
+      const int page = t[j * p.t_s1];
+      if (page < 0) continue;
+      if (page >= p.num_pages) {
+        flag(p, ST_BAD_PAGE);
+        continue;
       }
-    } else {
-      const int i = static_cast<int>((it - p.rows) / p.chunks), c = static_cast<int>((it - p.rows) - static_cast<long long>(i) * p.chunks);
-      const int src = movers[i], dst = gaps[i];
-      if (c == 0 && threadIdx.x == 0) {
-        p.refs[dst] = p.refs[src];
-        p.refs[src] = 0;
-        map[src] = dst;
-      }
-      copy_piece(p, c, src, dst, p.page_size);
+      const int to = __ldcg(map + page);
+      if (to == -1) flag(p, ST_REFS);  // the books say that the page is free: left alone
+      else if (to <= -2) t[j * p.t_s1] = gaps[-2 - to];
+      else if (to != page) t[j * p.t_s1] = to;
     }
   }
+  for (int i = blockIdx.x * COPY_THREADS + threadIdx.x; i < n; i += gridDim.x * COPY_THREADS) {
+    const int src = movers[i], dst = gaps[i];
+    p.refs[dst] = p.refs[src];
+    p.refs[src] = 0;
+    map[src] = dst;
+  }
+  if (threadIdx.x != 0) return;
+  const long long all = static_cast<long long>(n) * p.chunks;
+  const long long from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
+  copy_pieces(p, from, to, static_cast<int>(from / p.chunks), from % p.chunks, [&](int i, int& src, int& dst, int& tokens) {
+    src = movers[i], dst = gaps[i], tokens = p.page_size;
+    return true;
+  }, smem_u32(ring), smem_u32(bars));
 }
 
 }  // namespace pages

@@ -54,14 +54,14 @@ int scratch_of(const GaPagePool* a, size_t need, uint8_t** out) {
   return 0;
 }
 
-// CTAs of a copy kernel: eight per SM hold 128 KB of loads in flight.
+// CTAs of a copy kernel for at most so many pieces.
 unsigned copy_grid(long long items, int sm) {
-  const long long most = 8LL * sm;
+  const long long most = static_cast<long long>(COPY_CTAS) * sm;
   return static_cast<unsigned>(items < most ? (items > 0 ? items : 1) : most);
 }
 
 size_t copy_bytes(int pages, int n) { return up(static_cast<size_t>(pages) * 4) + up(static_cast<size_t>(n) * 8); }
-size_t fork_bytes(int rows, int n) { return up(static_cast<size_t>(rows) * 4) + up(static_cast<size_t>(n) * 16); }
+size_t fork_bytes(int rows, int n) { return up(static_cast<size_t>(rows) * 4) + up(static_cast<size_t>(n) * 16) + up(static_cast<size_t>(n) * 4); }
 int spans_of(int pages) { return (pages + SPAN - 1) / SPAN; }
 size_t compact_bytes(int pages) { return up(static_cast<size_t>(spans_of(pages)) * 4) + 2 * up(static_cast<size_t>(pages) * 4) + 256; }
 
@@ -80,6 +80,9 @@ int release(const GaPagePool* a, const void* rows, int is64, int n, int evict, i
 int ga::api::init_pages() {
   GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(grow_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRows * 4));
   GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(fork_plan_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxRows * 4));
+  GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(copy_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, COPY_SMEM));
+  GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(fork_apply_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, COPY_SMEM));
+  GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(compact_apply_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, COPY_SMEM));
   return 0;
 }
 
@@ -104,7 +107,7 @@ int ga_pages_copy(const GaPagePool* a, const void* src, const void* dst, int is6
   int* mark = reinterpret_cast<int*>(s);
   int2* list = reinterpret_cast<int2*>(s + up(static_cast<size_t>(c.d.num_pages) * 4));
   GA_TRY(ga::api::launch_serial(copy_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, c.st, c.d, src, dst, is64, n, mark, list));
-  GA_TRY(ga::api::launch_serial(copy_kernel, dim3(copy_grid(static_cast<long long>(n) * c.d.chunks, c.sm)), dim3(COPY_THREADS), 0, c.st,
+  GA_TRY(ga::api::launch_serial(copy_kernel, dim3(copy_grid(static_cast<long long>(n) * c.d.chunks, c.sm)), dim3(COPY_THREADS), COPY_SMEM, c.st,
                                 c.d, const_cast<const int2*>(list), n));
   return 0;
 }
@@ -140,10 +143,12 @@ int ga_pages_fork(const GaPagePool* a, const void* parents, const void* children
   uint8_t* s;
   if (scratch_of(a, fork_bytes(c.d.rows, n), &s)) return 1;
   int4* list = reinterpret_cast<int4*>(s + up(static_cast<size_t>(c.d.rows) * 4));
+  int* ends = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(list) + up(static_cast<size_t>(n) * 16));
+  if (static_cast<long long>(n) * c.d.chunks > 0x7fffffffLL) return fail("%d forks of %d pieces a page", n, c.d.chunks);
   GA_TRY(ga::api::launch_serial(fork_plan_kernel, dim3(1), dim3(PLAN_THREADS), static_cast<size_t>(n) * 4, c.st, c.d, parents, children,
-                                is64, n, reinterpret_cast<int*>(s), list));
-  GA_TRY(ga::api::launch_serial(fork_apply_kernel, dim3(copy_grid(n + static_cast<long long>(n) * c.d.chunks, c.sm)), dim3(COPY_THREADS), 0,
-                                c.st, c.d, parents, children, is64, n, const_cast<const int4*>(list)));
+                                is64, n, reinterpret_cast<int*>(s), list, ends));
+  GA_TRY(ga::api::launch_serial(fork_apply_kernel, dim3(copy_grid(n + static_cast<long long>(n) * c.d.chunks, c.sm)), dim3(COPY_THREADS),
+                                COPY_SMEM, c.st, c.d, parents, children, is64, n, const_cast<const int4*>(list), const_cast<const int*>(ends)));
   return 0;
 }
 
@@ -158,13 +163,14 @@ int ga_pages_compact(const GaPagePool* a, int32_t* map, int32_t* live, void* str
   int* counts = reinterpret_cast<int*>(s + 256);
   int* movers = reinterpret_cast<int*>(s + 256 + up(static_cast<size_t>(spans) * 4));
   int* gaps = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(movers) + up(static_cast<size_t>(pages) * 4));
-  GA_TRY(ga::api::launch_serial(compact_count_kernel, dim3(spans), dim3(PLAN_THREADS), 0, c.st, c.d, counts));
+  if (spans > 1)
+    GA_TRY(ga::api::launch_serial(compact_count_kernel, dim3(spans), dim3(PLAN_THREADS), 0, c.st, c.d, counts));
   GA_TRY(ga::api::launch_serial(compact_rank_kernel, dim3(spans), dim3(PLAN_THREADS), 0, c.st, c.d, const_cast<const int*>(counts), map,
                                 movers, gaps, live, moved));
   const long long bound = c.d.rows + static_cast<long long>(pages / 2) * c.d.chunks;
-  GA_TRY(ga::api::launch_serial(compact_apply_kernel, dim3(copy_grid(bound, c.sm)), dim3(COPY_THREADS), 0, c.st, c.d, map,
+  GA_TRY(ga::api::launch_serial(compact_apply_kernel, dim3(copy_grid(bound, c.sm)), dim3(COPY_THREADS), COPY_SMEM, c.st, c.d, map,
                                 const_cast<const int*>(movers), const_cast<const int*>(gaps), const_cast<const int*>(moved)));
-  ga::api::launches(3);
+  ga::api::launches(spans > 1 ? 3 : 2);
   return 0;
 }
 
