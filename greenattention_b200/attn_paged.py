@@ -23,13 +23,14 @@ from __future__ import annotations
 
 import ctypes
 import logging
-from typing import Callable, Optional, Union
+from typing import Callable, Union
 
 import torch
 
 from greenattention_b200 import _C, attn_decode, dispatch
 
 HEAD_DIMS = (64, 128, 256)
+MAX_KV_HEADS = 512
 KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 FP8 = torch.float8_e4m3fn
 STATUS_NAMES = {
@@ -73,7 +74,9 @@ def check_status(device: Union[torch.device, int, None] = None, reset: bool = Tr
     return val
 
 
-def _reason(kw: dict) -> Optional[str]:
+def _prepare(kw: dict):
+    """What a call needs at launch, or the reason (a str) why there is no kernel for it: from shapes, types and Python
+    scalars only."""
     more = kw.keys() - _ALLOWED
     for name in more:
         if kw[name] is not None:
@@ -92,18 +95,20 @@ def _reason(kw: dict) -> Optional[str]:
     if len(shape) != 3 or len(kshape) != 4 or kshape != vc.shape:
         return "q or kv rank, or k/v shapes differ"
     total, qh, hd = shape
-    _, page, kvh, khd = kshape
-    if hd not in HEAD_DIMS or khd != hd or not kvh or not qh or qh % kvh:
+    pages, page, kvh, khd = kshape
+    if hd not in HEAD_DIMS or khd != hd or not kvh or not qh or qh % kvh or kvh > MAX_KV_HEADS:
         return f"q shape: no kernel for (head_dim={hd}, q_heads={qh}, kv_heads={kvh})"
     if page <= 0 or page & (page - 1):
         return "page_size not a power of two"
     align = 15 if kv == FP8 else 7  # elements of 16 bytes
     k0, k1, k2, k3 = kc.stride()
     v0, v1, v2, v3 = vc.stride()
-    if k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & align or (kc.data_ptr() | vc.data_ptr()) & 15:
+    kp, vp = kc.data_ptr(), vc.data_ptr()
+    if k3 != 1 or v3 != 1 or (k0 | k1 | k2 | v0 | v1 | v2) & align or (kp | vp) & 15:
         return "kv layout: last stride 1, other strides and the base multiples of 16 bytes"
-    s0, s1, s2 = q.stride()
-    if s2 != 1 or (s0 | s1) & 3 or q.data_ptr() & (3 if qt == FP8 else 7):
+    q0, q1, q2 = q.stride()
+    qp = q.data_ptr()
+    if q2 != 1 or (q0 | q1) & 3 or qp & (3 if qt == FP8 else 7):
         return "q layout: last stride 1, other strides and the base multiples of 4 elements"
     i32 = torch.int32
     ps = pt.shape
@@ -121,28 +126,34 @@ def _reason(kw: dict) -> Optional[str]:
         return "non-causal call with several query tokens"
     if get("softcap"):
         return "softcap"
+    left = -1
     if get("window_size") is not None:
-        window = attn_decode._window_left(kw)
-        if isinstance(window, str):
-            return window
-    sinks = get("sink_tokens")
-    if sinks is not None and (type(sinks) is not int or not 0 <= sinks < 1 << 31):
+        left = attn_decode._window_left(kw)
+        if isinstance(left, str):
+            return left
+        left = min(max(left, -1), 1 << 30)
+    sinks = get("sink_tokens") or 0
+    if type(sinks) is not int or not 0 <= sinks < 1 << 31:
         return f"sink_tokens {sinks} is not a count"
     dev = q.device
     for t in (kc, vc, pt, cs, cu):
         if t.device != dev:
             return f"a tensor is on {t.device}, q on {dev}"
+    scales = []
     for name in ("k_descale", "v_descale"):
         t = get(name)
-        if t is not None:
-            if not isinstance(t, torch.Tensor) or t.device != dev:
-                return f"{name} is on {getattr(t, 'device', None)}, q on {dev}"
-            why = attn_decode._descale_reason(t, batch, kvh, name)
-            if why:
-                return why
+        if t is None:
+            scales += (None, 0, 0)
+            continue
+        if not isinstance(t, torch.Tensor) or t.device != dev:
+            return f"{name} is on {getattr(t, 'device', None)}, q on {dev}"
+        why = attn_decode._descale_reason(t, batch, kvh, name)
+        if why:
+            return why
+        scales += (t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1))
     out = get("out")
+    want = torch.bfloat16 if kv == FP8 else kv
     if out is not None:
-        want = torch.bfloat16 if kv == FP8 else kv
         if not isinstance(out, torch.Tensor) or out.device != dev:
             return "out is not a tensor on q's device"
         if out.dtype != want or out.shape != shape or out.stride(2) != 1:
@@ -152,48 +163,30 @@ def _reason(kw: dict) -> Optional[str]:
             return "out layout: rows must not overlap, strides and the base multiples of 4 elements"
     if dev.type != "cuda":
         return "tensors are on the host: the green kernels have no CPU path"
-    return None
+    scale = get("softmax_scale")
+    head = (KV_TYPES[kv], qp, qt == torch.bfloat16, q0, q1, kp, vp, k0, k1, k2, v0, v1, v2, pages, page, qh, kvh, hd,
+            pt.data_ptr(), *pt.stride(), ps[1], cs.data_ptr(), cu.data_ptr(), *scales)
+    tail = (total, batch, mq, left, sinks, hd**-0.5 if scale is None else scale)
+    return q, out, want, get("return_softmax_lse", False), head, tail
 
 
-def _launch(
-    *, q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, window_size=None, sink_tokens=None,
-    softmax_scale=None, return_softmax_lse=False, out=None, k_descale=None, v_descale=None, **_,
-):
+def _fire(q, out, want, with_lse, head, tail):
     dev = q.device
     index = dev.index
     if index not in _status:
         ensure_ready(dev)
-    total, qh, hd = q.shape
-    kv = k_cache.dtype
+    total, batch = tail[0], tail[1]
     if out is None:
-        out = q.new_empty(q.shape, dtype=torch.bfloat16 if kv == FP8 else kv)
-    lse = q.new_empty((qh, total), dtype=torch.float32) if return_softmax_lse else None
-    pages, page, kvh, _ = k_cache.shape
-    batch, cols = page_table.shape
+        out = q.new_empty(q.shape, dtype=want)
+    o0, o1, _ = out.stride()
+    lse = q.new_empty((q.shape[1], total), dtype=torch.float32) if with_lse else None
     lib = _C.lib()
     nbytes = _workspace_bytes.get((index, batch))
     if nbytes is None:
         nbytes = _workspace_bytes[(index, batch)] = lib.ga_paged_workspace_bytes(index, batch)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
-    q0, q1, _ = q.stride()
-    o0, o1, _ = out.stride()
-    t0, t1 = page_table.stride()
-    kd = vd = None
-    kd0 = kd1 = vd0 = vd1 = 0
-    if k_descale is not None:
-        kd, kd0, kd1 = k_descale.data_ptr(), k_descale.stride(0) if k_descale.shape[0] > 1 else 0, k_descale.stride(1)
-    if v_descale is not None:
-        vd, vd0, vd1 = v_descale.data_ptr(), v_descale.stride(0) if v_descale.shape[0] > 1 else 0, v_descale.stride(1)
-    left = -1 if window_size is None or window_size[0] is None else int(window_size[0])
-    p = _C.GaPagedParams(
-        KV_TYPES[kv], q.data_ptr(), q.dtype == torch.bfloat16, q0, q1, k_cache.data_ptr(), v_cache.data_ptr(),
-        *k_cache.stride()[:3], *v_cache.stride()[:3], pages, page, qh, kvh, hd,
-        page_table.data_ptr(), t0, t1, cols,
-        cache_seqlens.data_ptr(), cu_seqlens_q.data_ptr(), kd, kd0, kd1, vd, vd0, vd1,
-        out.data_ptr(), o0, o1, None if lse is None else lse.data_ptr(), total,
-        batch, max_seqlen_q, min(left, 1 << 30), sink_tokens or 0, hd**-0.5 if softmax_scale is None else softmax_scale,
-        _status[index].data_ptr(), ws.data_ptr(), nbytes,
-    )
+    p = _C.GaPagedParams(*head, out.data_ptr(), o0, o1, lse.data_ptr() if with_lse else None, *tail,
+                         _status[index].data_ptr(), ws.data_ptr(), nbytes)
     if torch.cuda.current_device() == index:
         rc = lib.ga_paged_attend(ctypes.byref(p), _C.raw_stream(index))
     else:
@@ -201,26 +194,26 @@ def _launch(
             rc = lib.ga_paged_attend(ctypes.byref(p), _C.raw_stream(index))
     if rc:
         _C.check(rc, "ga_paged_attend")
-    return (out, lse) if return_softmax_lse else out
+    return (out, lse) if with_lse else out
 
 
 def attend(**kw):
     """Attention over a paged cache (see the module); ``out``, or ``(out, lse)`` with ``return_softmax_lse``. Raises
     ``dispatch.Declined`` with the reason for a call outside what the kernels serve."""
-    why = _reason(kw)
-    if why is not None:
-        raise dispatch.Declined(f"attn_paged: {why}")
-    return _launch(**kw)
+    call = _prepare(kw)
+    if type(call) is str:
+        raise dispatch.Declined(f"attn_paged: {call}")
+    return _fire(*call)
 
 
 def select(kw: dict) -> Union[Callable, str]:
     """The launcher for this call or why there is none, from shapes, types and Python scalars only."""
-    why = _reason(kw)
-    if why is not None:
-        return why
+    call = _prepare(kw)
+    if type(call) is str:
+        return call
     if kw["q"].device.index not in _status:
         return "kernel not prewarmed for this device"
-    return _launch
+    return attend
 
 
 def _select_routed(kw: dict) -> Union[Callable, str]:
