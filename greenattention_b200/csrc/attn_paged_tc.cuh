@@ -156,6 +156,17 @@ __device__ __forceinline__ void wait_or_flag(uint32_t bar, uint32_t parity, bool
   }
 }
 
+// 16 e4m3 values as fp16 into chunks `ch` and ch + 1 of a 128-byte row whose chunks are permuted by `sw`.
+__device__ __forceinline__ void store_e4m3x16(uint32_t row, int ch, int sw, uint4 v, uint32_t flip) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(row + (((ch + k) ^ sw) << 4)), "r"(e4m3x2_to_f16x2(w[2 * k] & 0xffffu) ^ flip),
+                 "r"(e4m3x2_to_f16x2(w[2 * k] >> 16) ^ flip), "r"(e4m3x2_to_f16x2(w[2 * k + 1] & 0xffffu) ^ flip),
+                 "r"(e4m3x2_to_f16x2(w[2 * k + 1] >> 16) ^ flip)
+                 : "memory");
+}
+
 // One warp fills a stage with KEYS keys of CPK 16-byte chunks each, in slabs of eight chunks (128 bytes a key), swizzled by
 // key. n0[u] is the first token of the stage's group u, page[u]
 // the page of its token `lane`, or -1 for a row of zeros. Its own instruction stream is what a stage costs
@@ -234,6 +245,34 @@ __global__ void __launch_bounds__(1024) plan_split_kernel(const __grid_constant_
       e = make_int4(lo, static_cast<int>(g0 - p.prefix[lo]), static_cast<int>(g1 - g0), 0);
     }
     list[g] = e;
+  }
+}
+
+// The same for an e4m3 cache: 16 values of a key a load, converted to fp16 (exact) on the way into the stage. CPK: loads a key.
+template <int CPK, int KEYS>
+__device__ __forceinline__ void gather_e4m3(uint32_t dst, const uint8_t* base, long long s0, long long s1, const int (&n0)[4], int page_mask,
+                                            const int (&page)[4], int lane) {
+  constexpr int KPI = 32 / CPK;  // keys an instruction
+  const int c = lane % CPK, k0 = lane / CPK;
+  base += c * 16;
+  constexpr int U = 4;
+#pragma unroll
+  for (int i0 = 0; i0 < KEYS / KPI; i0 += U) {
+    uint4 v[U];
+    const int u = i0 * KPI / 32;  // a batch of loads lies within a group
+    const long long off = page[u] >= 0 ? page[u] * s0 + ((n0[u] + lane) & page_mask) * s1 : -1;
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const long long o = __shfl_sync(0xffffffffu, off, ((i0 + x) * KPI + k0) & 31);
+      v[x] = make_uint4(0u, 0u, 0u, 0u);
+      if (o >= 0) v[x] = *reinterpret_cast<const uint4*>(base + o);
+    }
+#pragma unroll
+    for (int x = 0; x < U; ++x) {
+      const int key = (i0 + x) * KPI + k0;
+      const uint32_t row = dst + (c >> 2) * (KEYS * 128) + key * 128;
+      store_e4m3x16(row, (c & 3) * 2, key & 7, v[x], 0u);
+    }
   }
 }
 
@@ -468,6 +507,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   if (warp < I::SOFT_WARPS) {
     // ------------------------------------------------------------------------------------------ softmax, epilogue
     regs_up<I::REGS_SOFT>();
+    constexpr int OKV = KV == KV_E4M3 ? KV_BF16 : KV;
     constexpr int SPLIT = I::SPLIT, KEYS = TK / SPLIT, DIMS = HD / SPLIT;
     const int g = warp / (4 * SPLIT), half = (warp >> 2) % SPLIT;  // query tile, part of its keys
     const int row = (warp & 3) * 32 + lane;
@@ -507,7 +547,8 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       const bool any = rr0 < r.nq * p.gqa;  // a warp of padding rows sees nothing and looks at nothing
       w.pmin = any ? r.pos0 + rr0 / p.gqa : -1;
       w.pmax = any ? r.pos0 + (rr0 + 31) / p.gqa : -1;
-      const float sl2 = p.scale_log2;
+      // with a negative descale the queries' signs are flipped as they are gathered; a zero one leaves every score at 0
+      const float sl2 = KV == KV_E4M3 && p.kd ? fmaxf(p.scale_log2 * fabsf(p.kd[b * p.kd_s0 + h * p.kd_s1]), 1e-30f) : p.scale_log2;
       float ref = -INFINITY, sum = 0.f;
       for (int i = 0; i < r.cnt; ++i, n += NQ) {
         const int buf = n & 1;
@@ -586,8 +627,8 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
           for (int k = 0; k < 32; k += 4) {
             uint2 o = make_uint2(0u, 0u);
             if (r.cnt > 0 && sum != 0.f) {
-              o.x = pack16<KV>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
-              o.y = pack16<KV>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
+              o.x = pack16<OKV>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
+              o.y = pack16<OKV>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
             }
             *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = o;
           }
@@ -735,9 +776,9 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
 #pragma unroll
         for (int u = 0; u < MOST; ++u) {
           n0[u] = group_at(r, tile * MOST + (is_v ? part * (KC / GK) : 0) + u);
-          if (u * GK < keys) inside &= n0[u] + GK <= r.kend && (n0[u] >= r.lower || n0[u] + GK <= p.sinks);
+          if (KV != KV_E4M3 && u * GK < keys) inside &= n0[u] + GK <= r.kend && (n0[u] >= r.lower || n0[u] + GK <= p.sinks);
         }
-        if (inside) {  // whole boxes of pages by TMA
+        if (KV != KV_E4M3 && inside) {  // whole boxes of pages by TMA
           const int box = min(p.page_mask + 1, GK), nb = keys / box;
           const int k = lane % nb, slab = lane / nb;
           const int gu = k * box / GK;
@@ -777,6 +818,14 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         const int at = q % NST, turn = q / NST;
         wait_stage(at, turn);
         const uint32_t dst = ring + at * STAGE;
+        if (KV == KV_E4M3) {
+          if (!is_v) gather_e4m3<4, TK>(dst, p.k + h * p.k_s2 + part * 64, p.k_s0, p.k_s1, n0, p.page_mask, page, lane);
+          else gather_e4m3<HD / 16, KC>(dst, p.v + h * p.v_s2, p.v_s0, p.v_s1, n0, p.page_mask, page, lane);
+          pending = q;
+          signal();
+          ++q;
+          return;
+        }
         if (!is_v) gather<8, TK>(dst, p.k + h * p.k_s2 + part * 128, p.k_s0, p.k_s1, n0, p.page_shift, p.page_mask, page, lane);
         else gather<HD / 8, KC>(dst, p.v + h * p.v_s2, p.v_s0, p.v_s1, n0, p.page_shift, p.page_mask, page, lane);
         cp_async_commit();
@@ -824,6 +873,29 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         const int rr = block * I::ROWS + mine, tok = rr / p.gqa;
         const long long off = mine < rows ? static_cast<long long>(r.q0 + tok) * p.q_s0 + static_cast<long long>(h * p.gqa + rr - tok * p.gqa) * p.q_s1 : -1;
         const uint32_t tile = sQ + (part >> 2) * (SLABS * STAGE);
+        if (KV == KV_E4M3) {
+          constexpr int CPR = HD / 16;  // 16 values at a time
+          const uint32_t flip = p.kd && p.kd[seg.b * p.kd_s0 + h * p.kd_s1] < 0.f ? 0x80008000u : 0u;
+#pragma unroll 4
+          for (int it = 0; it < CPR; ++it) {
+            const int e = it * 32 + lane, k = e / CPR, ch = e % CPR;
+            const long long o = __shfl_sync(0xffffffffu, off, k);
+            const int row = (part & 3) * 32 + k;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (o >= 0 && p.q_kind == Q_BF16_TO_E4M3) {
+              const uint4* s = reinterpret_cast<const uint4*>(p.q + (o + ch * 16) * 2);
+              const uint4 a = s[0], b = s[1];
+              auto four = [](uint32_t x, uint32_t y) {
+                return pack_e4m3x4(bf16_bits_to_f32(x & 0xffffu), bf16_bits_to_f32(x >> 16), bf16_bits_to_f32(y & 0xffffu), bf16_bits_to_f32(y >> 16));
+              };
+              v = make_uint4(four(a.x, a.y), four(a.z, a.w), four(b.x, b.y), four(b.z, b.w));
+            } else if (o >= 0) {
+              v = *reinterpret_cast<const uint4*>(p.q + o + ch * 16);
+            }
+            store_e4m3x16(tile + (ch >> 2) * STAGE + row * 128, (ch & 3) * 2, row & 7, v, flip);
+          }
+          continue;
+        }
 #pragma unroll
         for (int it = 0; it < 8; ++it) {
           const int k = it * 4 + (lane >> 3);

@@ -1,6 +1,5 @@
 // C ABI of the attention over 16-bit and e4m3 paged caches with first tokens kept visible (attn_paged.cuh): argument
 // checks, choice of the instance, launches.
-#include <cstdlib>
 #include <mutex>
 #include <vector>
 
@@ -80,7 +79,7 @@ template <class I>
 bool pool_maps(const PagedDev& d, CUtensorMap (&maps)[2]) {
   std::memset(maps, 0, sizeof(maps));
   const int page = d.page_mask + 1;
-  if (page < 8 || d.num_pages <= 0) return false;
+  if (page < 8 || d.num_pages <= 0 || I::KV == ga::paged::KV_E4M3) return false;
   MapKey kk, vk;
   std::memset(&kk, 0, sizeof(kk));
   kk.base = d.k, kk.s_page = d.k_s0, kk.s_tok = d.k_s1, kk.s_head = d.k_s2;
@@ -91,9 +90,13 @@ bool pool_maps(const PagedDev& d, CUtensorMap (&maps)[2]) {
   return pool_map(kk, &maps[0]) && pool_map(vk, &maps[1]);  // not for strides that a map cannot hold
 }
 
-// What the tensor-core kernel takes: its query rows go through 16-byte copies, and it takes the maximum before the scale.
+// What the tensor-core kernel takes: its query rows go through 16-byte copies, and it takes the maximum before the scale
+// (a k_descale comes with e4m3 caches, where the queries can take its sign).
+template <class I>
 bool tc_takes(const PagedDev& d) {
-  return !d.kd && d.scale_log2 > 0.f && d.q_s0 % 8 == 0 && d.q_s1 % 8 == 0 && reinterpret_cast<uintptr_t>(d.q) % 16 == 0;
+  const bool e4m3 = I::KV == ga::paged::KV_E4M3;
+  const int el = e4m3 && d.q_kind == ga::paged::Q_SAME ? 1 : 2;
+  return (!d.kd || e4m3) && d.scale_log2 > 0.f && d.q_s0 * el % 16 == 0 && d.q_s1 * el % 16 == 0 && reinterpret_cast<uintptr_t>(d.q) % 16 == 0;
 }
 
 // Enough CTAs to spread the rows of a small call over the SMs.
@@ -102,12 +105,28 @@ unsigned combine_shares(long long pairs, int rows, int sm) {
   return static_cast<unsigned>(z < 1 ? 1 : (z > rows ? rows : z));
 }
 
+// Whether a call of at most 128 rows per kv head goes to the tensor-core kernel in slices. Both sides measured (bf16,
+// device time, warp-level kernel / tensor-core kernel): 32 x 8192 tokens, 8 kv heads, head_dim 128: 16 rows 174 / 190 us,
+// 20 rows 290 / 191, 128 rows (8 requests more) 298 / 79; head_dim 64: 20 rows 143 / 213, 64 rows 46 / 35 (8 x 2000);
+// head_dim 256 (32 x 4096): 2 rows 273 / 172, 20 rows 544 / 181; pages of one token, 20 rows: 99 / 111; 4 x 300 tokens,
+// head_dim 256: 17 / 24. So: where the warp-level kernel would read the keys more than once (over 32 rows, 16 at
+// head_dim 256); at head_dim 128 from 17 rows and at 256 always, if pages are whole boxes and the call is not a small one.
+template <int KV>
+bool split_on_tensor_cores(const Launch& a, int hd) {
+  const long long rows = static_cast<long long>(a.d.max_q) * a.d.gqa;
+  if (rows > ga::paged::tc::TM) return false;
+  const int once = hd == 256 ? 16 : 32;
+  if (rows > once) return true;
+  const double most_bytes = 4.0 * a.d.batch * a.max_tokens * a.d.kvh * hd;
+  return KV != ga::paged::KV_E4M3 && a.d.page_mask >= 7 && most_bytes >= 8e6 && (hd == 256 || (hd == 128 && rows > 16));
+}
+
 // Verify on the tensor cores (at most 128 rows of a kv head): gangs of kv_heads CTAs, slices of the requests' tiles, and the
 // combine kernel; -1: the call is not one for it.
 template <class I>
 int run_tc_split(Launch& a) {
   PagedDev& d = a.d;
-  if (!tc_takes(d) || d.kvh > a.sm) return -1;
+  if (!tc_takes<I>(d) || d.kvh > a.sm) return -1;
   CUtensorMap maps[2];
   const bool boxes = pool_maps<I>(d, maps);
   const int gangs = a.sm / d.kvh;
@@ -128,7 +147,7 @@ int run_tc_split(Launch& a) {
 template <class I>
 int run_tc(Launch& a, size_t ws_bytes) {
   PagedDev& d = a.d;
-  if (!tc_takes(d)) return -1;
+  if (!tc_takes<I>(d)) return -1;
   const long long blocks = static_cast<long long>(d.total_q) * d.gqa / I::ROWS + d.batch;
   const size_t need = 256 + static_cast<size_t>(blocks) * 16;
   if (need > ws_bytes || blocks * d.kvh > 0x7fffffffLL) return -1;
@@ -203,6 +222,14 @@ int run_kv(Launch& a, int hd) {
 }
 
 template <int KV>
+int route(Launch& a, int hd, size_t ws_bytes) {
+  int rc = -1;
+  if (split_on_tensor_cores<KV>(a, hd)) rc = run_tc_split_kv<KV>(a, hd);
+  else if (a.prompt) rc = run_tc_kv<KV>(a, hd, ws_bytes);
+  return rc >= 0 ? rc : run_kv<KV>(a, hd);
+}
+
+template <int KV>
 int limits_tc_kv() {
   using namespace ga::paged::tc;
   return limits_tc<TcInst<64, KV, true>>() || limits_tc<TcInst<128, KV, true>>() || limits_tc<TcInst<256, KV, true>>() ||
@@ -220,7 +247,7 @@ int limits_kv() {
 
 int ga::api::init_paged() {
   return limits_kv<ga::paged::KV_BF16>() || limits_kv<ga::paged::KV_FP16>() || limits_kv<ga::paged::KV_E4M3>() ||
-         limits_tc_kv<ga::paged::KV_BF16>() || limits_tc_kv<ga::paged::KV_FP16>();
+         limits_tc_kv<ga::paged::KV_BF16>() || limits_tc_kv<ga::paged::KV_FP16>() || limits_tc_kv<ga::paged::KV_E4M3>();
 }
 
 extern "C" {
@@ -299,21 +326,9 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   l.st = static_cast<cudaStream_t>(stream);
   l.max_tokens = static_cast<long long>(a->pt_cols) * a->page_size;
   l.prompt = d.max_q > 16;
-  if (l.prompt && a->kv_type != ga::paged::KV_E4M3) {
-    const int rc = a->kv_type == ga::paged::KV_BF16 ? run_tc_kv<ga::paged::KV_BF16>(l, a->head_dim, a->workspace_bytes)
-                                                    : run_tc_kv<ga::paged::KV_FP16>(l, a->head_dim, a->workspace_bytes);
-    if (rc >= 0) return rc;
-  }
-  const long long rows = static_cast<long long>(d.max_q) * d.gqa;
-  static const int tc_rows = [] { const char* e = std::getenv("GA_TC_ROWS"); return e ? std::atoi(e) : 17; }();
-  if (!l.prompt && a->kv_type != ga::paged::KV_E4M3 && rows >= tc_rows && rows <= ga::paged::tc::TM) {
-    const int rc = a->kv_type == ga::paged::KV_BF16 ? run_tc_split_kv<ga::paged::KV_BF16>(l, a->head_dim)
-                                                    : run_tc_split_kv<ga::paged::KV_FP16>(l, a->head_dim);
-    if (rc >= 0) return rc;
-  }
-  if (a->kv_type == ga::paged::KV_BF16) return run_kv<ga::paged::KV_BF16>(l, a->head_dim);
-  if (a->kv_type == ga::paged::KV_FP16) return run_kv<ga::paged::KV_FP16>(l, a->head_dim);
-  return run_kv<ga::paged::KV_E4M3>(l, a->head_dim);
+  if (a->kv_type == ga::paged::KV_BF16) return route<ga::paged::KV_BF16>(l, a->head_dim, a->workspace_bytes);
+  if (a->kv_type == ga::paged::KV_FP16) return route<ga::paged::KV_FP16>(l, a->head_dim, a->workspace_bytes);
+  return route<ga::paged::KV_E4M3>(l, a->head_dim, a->workspace_bytes);
 }
 
 }  // extern "C"

@@ -311,3 +311,68 @@ def test_through_the_backend_entry(monkeypatch):
         monkeypatch.setattr(dispatch, "KV16", False)
     with pytest.raises(dispatch.Declined, match="softcap"):
         entry(**dict(make(BF16, [9], [1], 16, 8, 2, 128, 30, 4), softcap=30.0))
+
+
+def definition_on_gpu(kw, rows):
+    """The definition in 64 bits on the GPU for some rows of a call: out, sum_j p_j |v_j|, lse of those rows, and how far
+    32-bit scores may be off (see the oracle)."""
+    page, kvh, hd = kw["k_cache"].shape[1:]
+    window, sinks = kw.get("window_size", (-1, 0))[0], kw.get("sink_tokens") or 0
+    cu, lens = kw["cu_seqlens_q"].tolist(), kw["cache_seqlens"].tolist()
+    outs, spreads, lses, offs = [], [], [], []
+    fp8 = kw["k_cache"].dtype == FP8
+    for row in rows:
+        b = max(i for i in range(len(lens)) if cu[i] <= row)
+        p = lens[b] - (cu[b + 1] - cu[b]) + row - cu[b]
+        at = torch.arange(p + 1, device="cuda")
+        if window >= 0:
+            at = at[(at >= p - window) | (at < sinks)]
+        ids = kw["page_table"][b, at // page].long()
+        k, v = (kw[x].view(torch.uint8 if fp8 else torch.int16)[ids, at % page].view(kw[x].dtype).double().transpose(0, 1)
+                for x in ("k_cache", "v_cache"))
+        q = kw["q"][row].to(FP8 if fp8 else kw["q"].dtype).double().view(kvh, -1, hd)
+        kd, vd = (1.0 if kw.get(n) is None else kw[n][b].double()[:, None, None] for n in ("k_descale", "v_descale"))
+        s = q @ k.transpose(1, 2) * hd**-0.5 * kd
+        w = torch.softmax(s, -1)
+        outs.append((w @ v * vd).reshape(-1, hd))
+        spreads.append((w @ v.abs() * vd).reshape(-1, hd))
+        lses.append(torch.logsumexp(s, -1).reshape(-1))
+        offs.append(((q.abs() @ k.abs().transpose(1, 2) * hd**-0.5 * kd).amax() * hd * 2.0**-23 + len(at) * 2.0**-23 + 2.0**-16))
+    return torch.stack(outs), torch.stack(spreads), torch.stack(lses, 1), max(float(x) for x in offs)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("page", [4, 16, 64])
+@pytest.mark.parametrize("new,keys", [(700, 3000), (1500, 1500), (5, 6000), (24, 6000)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (700, 40)])
+def test_many_tiles_and_items(dtype, hd, page, new, keys, window, sinks):
+    """Long enough that every CTA goes through many tiles and several items: rings, buffers and barriers wrap round."""
+    from greenattention_b200 import attn_paged
+
+    g = torch.Generator(device="cuda").manual_seed(hd + new)
+    qh, kvh, batch = 16, 4, 5
+    lens = [keys - 37 * b for b in range(batch)]
+    cols = -(-keys // page)
+    pool = [torch.randn((batch * cols, page, kvh, hd), generator=g, device="cuda").to(dtype) for _ in range(2)]
+    table = torch.randperm(batch * cols, generator=g, device="cuda").view(batch, cols).to(torch.int32)
+    news = [min(new, n) for n in lens]
+    q = torch.randn((sum(news), qh, hd), generator=g, device="cuda").to(BF16)
+    kw = dict(q=q, k_cache=pool[0], v_cache=pool[1], page_table=table, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+              cu_seqlens_q=torch.tensor([0] + news, device="cuda").cumsum(0).to(torch.int32), max_seqlen_q=max(news), causal=True,
+              return_softmax_lse=True)
+    if window >= 0:
+        kw |= dict(window_size=(window, 0), sink_tokens=sinks)
+    if dtype == FP8:
+        kw |= {n: torch.rand((batch, kvh), generator=g, device="cuda") + 0.5 for n in ("k_descale", "v_descale")}
+    out, lse = attn_paged.attend(**kw)
+    again, _ = attn_paged.attend(**kw)
+    assert attn_paged.check_status() == 0
+    assert torch.equal(out, again)
+    rows = sorted({0, len(q) - 1, *torch.randint(0, len(q), (20,), generator=torch.Generator().manual_seed(1)).tolist()})
+    want, spread, want_lse, off = definition_on_gpu(kw, rows)
+    p_step = 2.0**-11 if dtype == FP8 else 2.0**-8
+    # the oracle's bound: half a step of the bf16 output, of P, and the scores' part (twice)
+    bound = (2.0**-8 * want.abs() + (p_step + 2 * off) * spread) * (1 + 2.0**-6) + 2.0**-25
+    assert ((out[rows].double() - want).abs() <= bound).all()
+    assert ((lse[:, rows].double() - want_lse).abs() <= off + 2.0**-20 * (1 + want_lse.abs())).all()
