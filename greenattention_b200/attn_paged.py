@@ -34,6 +34,7 @@ MAX_KV_HEADS = 512
 KV_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float8_e4m3fn: 2}
 FP8 = torch.float8_e4m3fn
 STATUS_NAMES = {
+    1: "a bounded wait for a full stage ran out", 2: "a bounded wait for a free stage ran out", 4: "shared memory was misplaced",
     3: "a page id was out of range (its keys were taken as zeros)",
     5: "a cache_seqlens entry exceeded page_table.shape[1] * page_size",
 }

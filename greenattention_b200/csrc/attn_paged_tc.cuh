@@ -278,7 +278,7 @@ __device__ __forceinline__ void gather_e4m3(uint32_t dst, const uint8_t* base, l
 
 // The call's row blocks: *count = how many, then (request, row block), a request's last block first.
 template <int ROWS>
-__global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constant__ PagedDev p, int* count, int4* blocks) {
+__global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constant__ PagedDev p, int* count, int4* blocks, int cap) {
   __shared__ int wsum[32];
   __shared__ int base;
   grid_dep_wait();
@@ -311,13 +311,14 @@ __global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constan
     // a warp lays out its requests' blocks together
     for (int src = 0; src < 32; ++src) {
       const int m = __shfl_sync(0xffffffffu, n, src), to = __shfl_sync(0xffffffffu, at, src);
-      for (int k = lane; k < m; k += 32) blocks[to + k] = make_int4(b0 + warp * 32 + src, m - 1 - k, 0, 0);
+      // query offsets that do not ascend could ask for more blocks than the list holds: they are left out
+      for (int k = lane; k < m && to + k < cap; k += 32) blocks[to + k] = make_int4(b0 + warp * 32 + src, m - 1 - k, 0, 0);
     }
     __syncthreads();
-    if (tid == 0) base += total;
+    if (tid == 0) base = min(base + total, cap);
     __syncthreads();
   }
-  if (tid == 0) *count = base;
+  if (tid == 0) *count = min(base, cap);
 }
 
 // What a row sees: keys in [lo, pos], and those below `sinks` that are not behind pos. pmin, pmax: positions of the first

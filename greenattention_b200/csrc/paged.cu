@@ -111,12 +111,14 @@ unsigned combine_shares(long long pairs, int rows, int sm) {
 // head_dim 256 (32 x 4096): 2 rows 273 / 172, 20 rows 544 / 181; pages of one token, 20 rows: 99 / 111; 4 x 300 tokens,
 // head_dim 256: 17 / 24. So: where the warp-level kernel would read the keys more than once (over 32 rows, 16 at
 // head_dim 256); at head_dim 128 from 17 rows and at 256 always, if pages are whole boxes and the call is not a small one.
+// An e4m3 cache is converted on the way into the stages, which costs more than reading it again a few times (16 x 8192
+// tokens: head_dim 128 64 rows 243 / 448 us, 128 rows 448 / 463; head_dim 256 64 rows 569 / 877, 128 rows 1101 / 904; head_dim
+// 64 64 rows 141 / 190, 128 rows 264 / 200): from 65 rows on.
 template <int KV>
 bool split_on_tensor_cores(const Launch& a, int hd) {
   const long long rows = static_cast<long long>(a.d.max_q) * a.d.gqa;
   if (rows > ga::paged::tc::TM) return false;
-  const int once = hd == 256 ? 16 : 32;
-  if (rows > once) return true;
+  if (rows > (KV == ga::paged::KV_E4M3 ? 64 : (hd == 256 ? 16 : 32))) return true;
   const double most_bytes = 4.0 * a.d.batch * a.max_tokens * a.d.kvh * hd;
   return KV != ga::paged::KV_E4M3 && a.d.page_mask >= 7 && most_bytes >= 8e6 && (hd == 256 || (hd == 128 && rows > 16));
 }
@@ -156,7 +158,8 @@ int run_tc(Launch& a, size_t ws_bytes) {
   const long long items = blocks * d.kvh;
   CUtensorMap maps[2];
   const bool boxes = pool_maps<I>(d, maps);
-  GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_prompts_kernel<I::ROWS>, dim3(1), dim3(1024), 0, a.st, d, count, list));
+  GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_prompts_kernel<I::ROWS>, dim3(1), dim3(1024), 0, a.st, d, count, list,
+                                static_cast<int>(blocks)));
   GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(static_cast<unsigned>(items < a.sm ? items : a.sm)), dim3(I::NT),
                                 I::SMEM, a.st, d, const_cast<const int*>(count), const_cast<const int4*>(list), maps[0], maps[1],
                                 static_cast<int>(boxes)));
@@ -270,6 +273,7 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   if (a->total_q < 0 || a->total_q > 0x7fffffffLL) return fail("total_q %lld", (long long)a->total_q);
   if (a->max_seqlen_q < 1) return fail("max_seqlen_q %d", a->max_seqlen_q);
   if (a->sink_tokens < 0) return fail("sink_tokens %d", a->sink_tokens);
+  if (a->total_q * (a->q_heads / a->kv_heads) > 0x7fffffffLL) return fail("%lld query rows of a kv head", (long long)a->total_q * (a->q_heads / a->kv_heads));
   if (a->total_q == 0) {
     ga::api::launches(0);
     return 0;

@@ -68,7 +68,7 @@ size_t compact_bytes(int pages) { return up(static_cast<size_t>(spans_of(pages))
 int release(const GaPagePool* a, const void* rows, int is64, int n, int evict, int window, int sinks, void* stream) {
   Call c;
   if (fill(a, stream, &c)) return 1;
-  if (n < 0 || (n > 0 && !rows)) return fail("rows");
+  if (n < 0 || n > kMaxRows || (n > 0 && !rows)) return fail("rows: at most %d entries", kMaxRows);
   ga::api::launches(n > 0);
   if (n == 0) return 0;
   GA_TRY(ga::api::launch_serial(release_kernel, dim3(n), dim3(256), 0, c.st, c.d, rows, is64, n, evict, window, sinks));

@@ -26,8 +26,8 @@ from greenattention_b200 import _C, dispatch
 CHUNK = 16384  # bytes of a copy item of the kernels
 MAX_ROWS = 32768
 STATUS_NAMES = {
-    3: "a page id was out of range", 5: "a length exceeded the row's entries", 7: "a row or page index was out of range",
-    8: "no free page was left", 9: "the page counts did not match the page table",
+    1: "a bounded wait for a copy ran out", 3: "a page id was out of range", 5: "a length exceeded the row's entries",
+    7: "a row or page index was out of range", 8: "no free page was left", 9: "the page counts did not match the page table",
     10: "entries of one call contradict one another, or a forked row was not empty",
 }
 _NO_SCRATCH = ("ga_pages_free", "ga_pages_evict")
@@ -113,6 +113,12 @@ class PagePool:
             _no(f"{name} is not dense")
         return int(t.dtype == torch.int64)
 
+    def _entries(self, rows) -> int:
+        n = rows.shape[0]
+        if n > MAX_ROWS:
+            _no(f"{n} entries in one call, at most {MAX_ROWS}")
+        return n
+
     def _pair(self, a_name: str, a, b_name: str, b) -> int:
         is64 = self._index(a_name, a)
         if self._index(b_name, b) != is64 or a.shape != b.shape:
@@ -164,9 +170,7 @@ class PagePool:
         of a partial last page are copied to the lowest free page (copy on write ahead of the write). A child that is not
         empty or is named before is left alone (status 10), one that finds no free page too (status 8)."""
         is64 = self._pair("parents", parents, "children", children)
-        n = parents.shape[0]
-        if n > MAX_ROWS:
-            _no(f"{n} entries in one call, at most {MAX_ROWS}")
+        n = self._entries(parents)
         if n:
             self._call("ga_pages_fork", n, parents.data_ptr(), children.data_ptr(), is64, n)
 
@@ -175,18 +179,16 @@ class PagePool:
         a smaller length leaves it alone. From the first row on whose pages are not there, rows that need some are left
         as they were (status 8)."""
         is64, lens64 = self._index("rows", rows), self._index("lens", lens)
-        n = rows.shape[0]
+        n = self._entries(rows)
         if lens.shape[0] != n:
             _no("rows and lens differ in length")
-        if n > MAX_ROWS:
-            _no(f"{n} entries in one call, at most {MAX_ROWS}")
         if n:
             self._call("ga_pages_grow", n, rows.data_ptr(), lens.data_ptr(), is64, lens64, n)
 
     def free(self, rows: torch.Tensor) -> None:
         """Releases the rows' pages; their lengths become 0."""
         is64 = self._index("rows", rows)
-        n = rows.shape[0]
+        n = self._entries(rows)
         if n:
             self._call("ga_pages_free", n, rows.data_ptr(), is64, n)
 
@@ -197,7 +199,7 @@ class PagePool:
         for name, v in (("window_left", window_left), ("sink_tokens", sink_tokens)):
             if not isinstance(v, int) or isinstance(v, bool) or not 0 <= v < 1 << 31:
                 _no(f"{name} {v} is not a count")
-        n = rows.shape[0]
+        n = self._entries(rows)
         if n:
             self._call("ga_pages_evict", n, rows.data_ptr(), is64, n, window_left, sink_tokens)
 

@@ -282,12 +282,13 @@ int ga_pages_copy(const GaPagePool* p, const void* src, const void* dst, int is6
 /* Row children[i] (empty) becomes a copy of row parents[i]: full pages are shared, the tokens of a partial last page are
  * copied to a new one. New pages are the lowest free ones, in the entries' order. At most 32768 entries. */
 int ga_pages_fork(const GaPagePool* p, const void* parents, const void* children, int is64, int n, void* stream);
-/* The rows' pages are released and their lengths become 0. */
+/* The rows' pages are released and their lengths become 0. At most 32768 entries. */
 int ga_pages_free(const GaPagePool* p, const void* rows, int is64, int n, void* stream);
 /* Releases the pages whose keys are neither among the first sink_tokens nor in the window [len - window_left, ..] of the
- * row's next query; their entries become -1, the length stays. */
+ * row's next query; their entries become -1, the length stays. At most 32768 entries. */
 int ga_pages_evict(const GaPagePool* p, const void* rows, int is64, int n, int window_left, int sink_tokens, void* stream);
-/* Rows grow to lens[i] tokens (a smaller length leaves a row alone) with the lowest free pages, in the entries' order. */
+/* Rows grow to lens[i] tokens (a smaller length leaves a row alone) with the lowest free pages, in the entries' order.
+ * At most 32768 entries. */
 int ga_pages_grow(const GaPagePool* p, const void* rows, const void* lens, int is64, int lens64, int n, void* stream);
 /* The *live held pages move below id *live: those at or above it, in order, into the free ids below. The table and the
  * counts follow; map[page] is a page's new id, -1 for a free one. */

@@ -81,3 +81,22 @@ def test_pool_has_no_cpu_path():
 
     with pytest.raises(_C.GreenAttentionError, match="no CPU path"):
         pool()
+
+
+def test_struct_layouts_match_the_header():
+    """Field names and order of the ctypes mirrors follow the C structs."""
+    import os
+    import re
+
+    from greenattention_b200 import _C
+
+    with open(os.path.join(os.path.dirname(os.path.dirname(__file__)), "include", "green_attention.h")) as f:
+        header = f.read()
+    for name, mirror in (("GaPagedParams", _C.GaPagedParams), ("GaPagePool", _C.GaPagePool)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), header, flags=re.S).group(1)
+        fields = []
+        for decl in re.sub(r"/\*.*?\*/", "", body, flags=re.S).split(";"):
+            parts = [x.strip() for x in decl.strip().split(",")]
+            if parts[0]:
+                fields += [re.split(r"[\s*]+", parts[0])[-1]] + [x.lstrip("*").strip() for x in parts[1:]]
+        assert fields == [n for n, _ in mirror._fields_], name

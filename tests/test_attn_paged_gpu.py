@@ -376,3 +376,19 @@ def test_many_tiles_and_items(dtype, hd, page, new, keys, window, sinks):
     bound = (2.0**-8 * want.abs() + (p_step + 2 * off) * spread) * (1 + 2.0**-6) + 2.0**-25
     assert ((out[rows].double() - want).abs() <= bound).all()
     assert ((lse[:, rows].double() - want_lse).abs() <= off + 2.0**-20 * (1 + want_lse.abs())).all()
+
+
+@pytest.mark.parametrize("new", [40, 400])
+def test_query_offsets_that_do_not_ascend_stay_in_bounds(new):
+    """Malformed offsets ask for more rows than there are: nothing is written outside, the rest of the call is served."""
+    from greenattention_b200 import attn_paged
+
+    kw = make(BF16, [500, 500, 500], [new, new, new], 16, 8, 2, 64, seed=4)
+    kw["cu_seqlens_q"] = torch.tensor([0, 3 * new, 0, 9 * new], dtype=torch.int32, device="cuda")
+    guard = torch.full((3 * new + 64, 8, 64), 3.0, dtype=BF16, device="cuda")
+    kw["out"] = guard[32:32 + 3 * new]
+    attn_paged.attend(**kw)
+    torch.cuda.synchronize()
+    assert (guard[:32] == 3).all() and (guard[32 + 3 * new:] == 3).all()
+    attn_paged.check_status()
+    check(make(BF16, [50, 60], [40, 40], 16, 8, 2, 64, seed=6))
