@@ -1,27 +1,36 @@
-// Prompts over paged 16-bit caches on the tensor cores (tcgen05, kind::f16, accumulators in tensor memory): the same
-// mathematics as attn_paged.cuh, for calls with enough query rows to fill 128-row tiles.
+// Prompts and verify over paged caches on the tensor cores (tcgen05, kind::f16, accumulators in tensor memory): the same
+// mathematics as attn_paged.cuh. Prompts are cut into row blocks; verify (SPLIT_KV: at most 128 rows of a kv head) along
+// the keys, with the pieces folded by attn_paged_combine.
 //
 // A persistent CTA takes work items of NQ tiles of 128 query rows (row = token * GQA + head, one kv head) against tiles of
-// 128 keys. Roles: a softmax group of four warps per query tile (a thread owns one row), one warp whose elected lane
-// issues every MMA, four warps that gather K and V, two that gather Q.
+// 128 keys. Roles: softmax warps (two threads a row, each with half of the keys; four in verify at head_dim 128), one or two
+// lanes that issue the MMAs, four or five warps that gather K and V, one to four that gather Q.
 //   * S = Q K^T into one of two 128-column score buffers, softmax in place, P as 16-bit pairs over the front half of the
 //     buffer it came from, O += P V with P as the A operand from tensor memory and V as an MN-major B operand, i.e. the
 //     page's [token, dim] layout as it is. Score buffers alternate job by job; a job is (key tile, query tile): at
 //     head_dim <= 128 two query tiles share every K and V tile (NQ = 2), at 256 one query tile (O alone takes half of
 //     tensor memory) has two key tiles in flight.
-//   * The MMAs of a job are issued in an order that needs few barriers: PV(n), then QK(n + 2) into the same buffer. One
-//     thread issues them all and the pipe runs them in order, so scores that are ready say that the PV two jobs before is.
+//   * The MMAs are issued in an order that needs few barriers: PV(n), then QK(n + 2) into the same buffer. With NQ 2 one
+//     lane issues them all and the pipe runs them in order; with NQ 1 a second lane issues the QK MMAs and waits for the PV
+//     two jobs before. Either way scores that are ready say that the PV two jobs before is done.
 //   * The row's reference maximum moves only when a tile exceeds it by more than 2^8 (P stays below 256, exact in the
 //     sums; the 16-bit rounding of P is relative), so O is rescaled in tensor memory in few tiles.
 //   * K and V come through one ring of 16 KB stages in the order in which the MMAs use them: a K stage is 128 keys x 64
 //     dims, a V stage 8192 / head_dim keys x all dims, in the 128-byte swizzle that the MMA descriptors name. Where every
 //     key of a stage is seen by some query, TMA boxes of up to a page each fill it (pages of 8 tokens and more); edges of
 //     what is seen and smaller pages are filled with 16-byte cp.async, rows no query of the item sees (released pages
-//     among them) with zeros.
+//     among them) with zeros. Values of an e4m3 cache go through registers, converted to fp16.
 // Keys are taken in groups of 32: the sinks' groups, then those of the run that ends with the item's last visible key (Req);
 // a tile is the next four, so a few first tokens cost 32 keys of a tile and not one of their own. Items come from a list that a
 // small kernel lays out, later row blocks of a request first (they see more keys), all kv heads of a block side by side
 // (they share pages).
+//
+// What bounds it: a key tile is 2 x 1024 tensor cycles at head_dim 256 and takes about 4600, because scores, softmax, P and
+// PV follow one another over two score buffers, and the QK MMAs (both operands from shared memory) use all of its 128
+// bytes a clock. Measured (bf16): 4 causal prompts of 4096 tokens, head_dim 256, 16 heads 662 us = 830 TFLOP/s, head_dim 128,
+// 32 heads 824 us = 667; 8 x 2048 tokens on 16k, head_dim 256, window 1024 and 4 first tokens 442 us; verify in slices, 32 x
+// 8192 tokens, 20 rows of 8 kv heads (1.07 GB) 191 us = 5.6 TB/s (299 on the warp-level kernel). Over an e4m3 cache the
+// gathering warps convert (exactly, to fp16), which bounds it: the windowed extend takes 1170 us.
 #pragma once
 
 #include "attn_paged.cuh"
