@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   regs_down<I::REGS_REST>();
   if (warp < KV_WARP) {
     // ------------------------------------------------------------------------------------------------- MMA issue
-    // NQ 2: one lane issues for both query tiles in turn (a lane for each measured 10 % slower). NQ 1: one lane for the QK
+    // NQ 2: one lane issues for both query tiles in turn (a lane for each: 4 x 4096 causal tokens 1064 us instead of 897). NQ 1: one lane for the QK
     // MMAs, one for the PV MMAs; a QK waits for the PV two tiles before, whose P it overwrites.
     const int role = warp - MMA_WARP;
     if (lane == 0 && (NQ == 1 || role == 0)) {
