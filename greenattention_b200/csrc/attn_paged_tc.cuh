@@ -27,10 +27,10 @@
 //
 // What bounds it: a key tile is 2 x 1024 tensor cycles at head_dim 256 and takes about 4600, because scores, softmax, P and
 // PV follow one another over two score buffers, and the QK MMAs (both operands from shared memory) use all of its 128
-// bytes a clock. Measured (bf16): 4 causal prompts of 4096 tokens, head_dim 256, 16 heads 662 us = 830 TFLOP/s, head_dim 128,
-// 32 heads 824 us = 667; 8 x 2048 tokens on 16k, head_dim 256, window 1024 and 4 first tokens 442 us; verify in slices, 32 x
+// bytes a clock. Measured (bf16): 4 causal prompts of 4096 tokens, head_dim 256, 16 heads 652 us = 842 TFLOP/s, head_dim 128,
+// 32 heads 802 us = 685; 8 x 2048 tokens on 16k, head_dim 256, window 1024 and 4 first tokens 431 us; verify in slices, 32 x
 // 8192 tokens, 20 rows of 8 kv heads (1.07 GB) 191 us = 5.6 TB/s (299 on the warp-level kernel). Over an e4m3 cache the
-// gathering warps convert (exactly, to fp16), which bounds it: the windowed extend takes 1170 us.
+// gathering warps convert (exactly, to fp16), which bounds it: the windowed extend takes 1110 us.
 #pragma once
 
 #include "attn_paged.cuh"
@@ -72,7 +72,7 @@ struct TcInst {
   // Registers a thread: what the block is launched with (limit of the launch bounds), and its split between the softmax
   // warps and the others. The shares add up to no more than the launch's.
   static constexpr int REGS = SOFT_WARPS == 16 ? 80 : 96;
-  static constexpr int REGS_SOFT = SOFT_WARPS == 16 ? 96 : 128, REGS_REST = SOFT_WARPS == 16 ? 48 : 72;
+  static constexpr int REGS_SOFT = SOFT_WARPS == 16 ? 88 : 120, REGS_REST = SOFT_WARPS == 16 ? 64 : 80;
   static_assert(SOFT_WARPS * REGS_SOFT + (WARPS - SOFT_WARPS) * REGS_REST <= WARPS * REGS, "register split");
   // Row maxima that the halves of a row exchange: at NQ 1 two jobs' in turn; at NQ 2 a query tile's next scores are ready
   // only after both halves are done with the job before.
@@ -330,6 +330,22 @@ __global__ void __launch_bounds__(1024) plan_prompts_kernel(const __grid_constan
   if (tid == 0) *count = min(base, cap);
 }
 
+// Two products and sums, two sums an instruction: the exponential pass issues 5 instructions for two scores instead of 7
+// (full causal head_dim 256 680 -> 652 us, head_dim 128 816 -> 802).
+__device__ __forceinline__ float2 fma2(float x, float y, float s, float t) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+      "fma.rn.f32x2 a, a, b, c;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(x), "f"(y), "f"(s), "f"(t));
+  return r;
+}
+__device__ __forceinline__ void add2(float& x, float& y, float a, float b) {
+  asm("{\n\t.reg .b64 p, q;\n\tmov.b64 p, {%0, %1};\n\tmov.b64 q, {%2, %3};\n\tadd.rn.f32x2 p, p, q;\n\tmov.b64 {%0, %1}, p;\n\t}"
+      : "+f"(x), "+f"(y)
+      : "f"(a), "f"(b));
+}
+
 // What a row sees: keys in [lo, pos], and those below `sinks` that are not behind pos. pmin, pmax: positions of the first
 // and the last row of the thread's warp, which decide for 32 keys at a time whether any row has to look at them.
 struct View {
@@ -392,9 +408,9 @@ __device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, cons
       }
 #pragma unroll
       for (int k = 0; k < 32; k += 2) {
-        const float e0 = ex2(fmaf(__uint_as_float(v[k]), sl2, -mu)), e1 = ex2(fmaf(__uint_as_float(v[k + 1]), sl2, -mu));
-        part[k & 2] += e0;
-        part[(k & 2) + 1] += e1;
+        const float2 a = fma2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]), sl2, -mu);
+        const float e0 = ex2(a.x), e1 = ex2(a.y);
+        add2(part[k & 2], part[(k & 2) + 1], e0, e1);
         out[k / 2] = pack16<KV>(e0, e1);
       }
     }
