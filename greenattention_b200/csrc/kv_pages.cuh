@@ -546,11 +546,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) compact_rank_kernel(const __grid
   block_scan<PLAN_THREADS>(mine, tmp, L);
   block_scan<PLAN_THREADS>(before, tmp, B);
   if (tid == 0) below = B;
-  // live pages below L: the spans before L's and the part of L's own
-  const int ls = L / SPAN;
+  // live pages below L: the spans before L's, whose counts are there if there are several, and the part of the one L lies in
+  const int ls = gridDim.x == 1 ? 0 : L / SPAN;
   int low = 0;
   for (int s = tid; s < ls; s += PLAN_THREADS) low += counts[s];
-  if (L % SPAN) {
+  if (L > ls * SPAN) {
     const int at = ls * SPAN + tid * 16;
     unsigned bits = live_bits(p, at);
     if (at + 16 > L) bits &= at >= L ? 0u : (1u << (L - at)) - 1;
@@ -591,7 +591,12 @@ __global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(const __gri
   copy_setup(smem_u32(bars));
   grid_dep_wait();
   grid_dep_launch();
-  const int n = *moved;
+  // at most half of the pages move; pairs that do not name two pages of the pool are left alone whatever the books say
+  const int n = min(*moved, p.num_pages / 2);
+  auto pair = [&](int i, int& src, int& dst) {
+    src = movers[i], dst = gaps[i];
+    return static_cast<unsigned>(src) < static_cast<unsigned>(p.num_pages) && static_cast<unsigned>(dst) < static_cast<unsigned>(p.num_pages);
+  };
   for (int row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const int held = min(pages_of(p, p.lens[row]), p.cols);
     int* t = p.table + row * p.t_s0;
@@ -604,12 +609,14 @@ __global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(const __gri
       }
       const int to = __ldcg(map + page);
       if (to == -1) flag(p, ST_REFS);  // the books say that the page is free: left alone
-      else if (to <= -2) t[j * p.t_s1] = gaps[-2 - to];
+      else if (to <= -2 && -2 - to < n) t[j * p.t_s1] = gaps[-2 - to];
+      else if (to <= -2) flag(p, ST_REFS);
       else if (to != page) t[j * p.t_s1] = to;
     }
   }
   for (int i = blockIdx.x * COPY_THREADS + threadIdx.x; i < n; i += gridDim.x * COPY_THREADS) {
-    const int src = movers[i], dst = gaps[i];
+    int src, dst;
+    if (!pair(i, src, dst)) continue;
     p.refs[dst] = p.refs[src];
     p.refs[src] = 0;
     map[src] = dst;
@@ -618,8 +625,8 @@ __global__ void __launch_bounds__(COPY_THREADS) compact_apply_kernel(const __gri
   const long long all = static_cast<long long>(n) * p.chunks;
   const long long from = all * blockIdx.x / gridDim.x, to = all * (blockIdx.x + 1) / gridDim.x;
   copy_pieces(p, from, to, static_cast<int>(from / p.chunks), from % p.chunks, [&](int i, int& src, int& dst, int& tokens) {
-    src = movers[i], dst = gaps[i], tokens = p.page_size;
-    return true;
+    tokens = p.page_size;
+    return pair(i, src, dst);
   }, smem_u32(ring), smem_u32(bars));
 }
 

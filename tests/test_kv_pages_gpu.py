@@ -286,3 +286,38 @@ def test_serving_run(dtype):
     step([1, 0, 2, 4], [1, 50, 1, 1])
     pool.free(ints(list(range(rows))))
     assert (refs == 0).all() and (lens == 0).all() and pool.check_status() == 0 and attn_paged.check_status() == 0
+
+
+@pytest.mark.parametrize("pages", [1, 15, 16383, 16384, 16385, 32768])
+@pytest.mark.parametrize("left", [0, -1, 7])
+@pytest.mark.parametrize("hole", [None, 0, -1])
+def test_compact_of_a_full_pool(pages, left, hole):
+    """Every page held, or all but the first or last: whatever words the scratch holds before the call, nothing but the
+    page into the hole moves."""
+    import ctypes
+
+    from greenattention_b200 import _C, kv_pages
+
+    held = [i for i in range(pages) if hole is None or i != hole % pages]
+    refs = torch.full((pages,), 2, dtype=torch.int32, device="cuda")
+    if hole is not None:
+        refs[hole] = 0
+    cache = torch.arange(pages, dtype=torch.int32, device="cuda").view(-1, 1, 1).expand(pages, 1, 4).contiguous()
+    table = ints([held or [-1]])
+    pool = kv_pages.PagePool([cache], table, ints([len(held)]), refs)
+    lib = _C.lib()
+    p = _C.GaPagePool.from_buffer_copy(pool._p)
+    nbytes = lib.ga_pages_scratch_bytes(ctypes.byref(p), 0)
+    scratch = torch.full((nbytes // 4,), left, dtype=torch.int32, device="cuda")
+    p.scratch, p.scratch_bytes = scratch.data_ptr(), nbytes
+    to, live = torch.full((pages,), -9, dtype=torch.int32, device="cuda"), ints([-9])
+    _C.check(lib.ga_pages_compact(ctypes.byref(p), to.data_ptr(), live.data_ptr(), _C.raw_stream(pool.device.index)), "compact")
+    n = len(held)
+    want = [-1] * pages
+    for i in held:
+        want[i] = i if i < n else hole % pages
+    assert live.item() == n and to.tolist() == want and pool.check_status() == 0
+    assert refs.tolist() == [2] * n + [0] * (pages - n)
+    if n:
+        assert table[0].tolist() == [want[i] for i in held]
+        assert torch.equal(cache[table[0].long(), 0, 0].long(), torch.tensor(held, device="cuda"))
