@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(256) release_kernel(const __grid_constant__ Po
     first = (sinks >> p.page_shift) + ((sinks & (p.page_size - 1)) != 0);
     const int gone = len > window ? (len - window) >> p.page_shift : 0;
     last = gone < held ? gone : held;
+    first = min(first, last);  // so that no thread's index passes 32 bits
   }
   int* t = p.table + row * p.t_s0;
   for (int j = first + threadIdx.x; j < last; j += blockDim.x) {

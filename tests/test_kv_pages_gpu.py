@@ -321,3 +321,12 @@ def test_compact_of_a_full_pool(pages, left, hole):
     if n:
         assert table[0].tolist() == [want[i] for i in held]
         assert torch.equal(cache[table[0].long(), 0, 0].long(), torch.tensor(held, device="cuda"))
+
+
+@pytest.mark.parametrize("page", [1, 2, 16])
+@pytest.mark.parametrize("window,sinks", [(0, (1 << 31) - 1), ((1 << 31) - 1, 0), ((1 << 31) - 1, (1 << 31) - 1), (0, (1 << 31) - 257), (3, 5)])
+def test_evict_with_the_largest_window_and_first_tokens(page, window, sinks):
+    pool, books = setup(400, page, 3, 300 // page + 1)
+    both(pool, books, "grow", [0, 1, 2], [290, 0, 7])
+    both(pool, books, "evict", [0, 1, 2], window_left=window, sink_tokens=sinks)
+    same(pool, books)
