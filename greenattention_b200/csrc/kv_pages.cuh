@@ -49,30 +49,30 @@ struct PoolDev {
 __device__ __forceinline__ int pages_of(const PoolDev& p, int len) { return len <= 0 ? 0 : (len - 1) / p.page_size + 1; }
 __device__ __forceinline__ void flag(const PoolDev& p, int what) { atomicExch(p.status, what); }
 
-// Exclusive prefix of `v` over the CTA's threads, and the sum. `tmp`: 33 ints of shared memory.
-template <int NT>
-__device__ __forceinline__ int block_scan(int v, int* tmp, int& total) {
+// Exclusive prefix of `v` over the CTA's threads, and the sum. `tmp`: 33 numbers of shared memory.
+template <int NT, typename N>
+__device__ __forceinline__ N block_scan(N v, N* tmp, N& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int incl = v;
+  N incl = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int o = __shfl_up_sync(0xffffffffu, incl, d);
+    const N o = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += o;
   }
   if (lane == 31) tmp[warp] = incl;
   __syncthreads();
   if (warp == 0) {
-    int w = lane < NT / 32 ? tmp[lane] : 0, wi = w;
+    N w = lane < NT / 32 ? tmp[lane] : 0, wi = w;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, wi, d);
+      const N o = __shfl_up_sync(0xffffffffu, wi, d);
       if (lane >= d) wi += o;
     }
     if (lane < NT / 32) tmp[lane] = wi - w;
     if (lane == NT / 32 - 1) tmp[32] = wi;
   }
   __syncthreads();
-  const int before = tmp[warp] + incl - v;
+  const N before = tmp[warp] + incl - v;
   total = tmp[32];
   __syncthreads();
   return before;
@@ -324,19 +324,23 @@ __device__ __forceinline__ void mark_first(int n, int* mark, RowOf row_of) {
 }
 
 // Rows grow to the given lengths with the lowest free pages, in the call's order. From the first row on whose pages
-// are not there, rows that need some are left as they were (flagged). One CTA; dynamic shared memory: n ints.
+// are not there, rows that need some are left as they were (flagged). One CTA; dynamic shared memory: n ints, the inclusive
+// prefix of the needs, cut where it is past every page (rows times columns may pass 32 bits).
 __global__ void __launch_bounds__(PLAN_THREADS) grow_kernel(const __grid_constant__ PoolDev p, const void* rows,
                                                             const void* to, int is64, int to64, int n, int* mark) {
   extern __shared__ int incl[];
-  __shared__ int tmp[33];
+  __shared__ long long tmp[33];
+  __shared__ int found[33];
   grid_dep_wait();
   grid_dep_launch();
   auto row_of = [&](int i) {
     const long long r = index_at(rows, is64, i);
     return r >= 0 && r < p.rows ? static_cast<int>(r) : -1;
   };
+  const long long most = static_cast<long long>(p.cols) << p.page_shift;  // tokens of a row
+  const long long all = p.num_pages + 1LL;
   mark_first(n, mark, row_of);
-  int sum = 0;
+  long long sum = 0;
   for (int i0 = 0; i0 < n; i0 += PLAN_THREADS) {
     const int i = i0 + threadIdx.x;
     int need = 0;
@@ -348,17 +352,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) grow_kernel(const __grid_constan
         flag(p, ST_CLASH);
       } else {
         const long long want = index_at(to, to64, i);
-        if (want > (static_cast<long long>(p.cols) << p.page_shift)) flag(p, ST_LEN_RANGE);
+        if (want > most) flag(p, ST_LEN_RANGE);
         else need = max(0, pages_of(p, static_cast<int>(want < 0 ? 0 : want)) - pages_of(p, p.lens[r]));
       }
     }
-    int total;
-    const int before = block_scan<PLAN_THREADS>(need, tmp, total);
-    if (i < n) incl[i] = sum + before + need;
+    long long total;
+    const long long before = block_scan<PLAN_THREADS>(static_cast<long long>(need), tmp, total);
+    if (i < n) incl[i] = static_cast<int>(min(sum + before + need, all));
     sum += total;
   }
   __syncthreads();
-  const int got = hand_out(p, sum, tmp, [&](int rank, int page) {
+  const int got = hand_out(p, static_cast<int>(min(sum, all)), found, [&](int rank, int page) {
     const int i = holder(incl, n, rank);
     const int r = row_of(i), j = pages_of(p, p.lens[r]) + rank - (i ? incl[i - 1] : 0);
     p.table[r * p.t_s0 + j * p.t_s1] = page;
@@ -380,8 +384,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) grow_kernel(const __grid_constan
     const int r = row_of(i);
     if (r < 0 || __ldcg(mark + r) != i) continue;
     const long long want = index_at(to, to64, i);
-    const bool fits = incl[i] == (i ? incl[i - 1] : 0) || incl[i] <= got;
-    if (fits && want > p.lens[r] && want <= (static_cast<long long>(p.cols) << p.page_shift)) p.lens[r] = static_cast<int>(want);
+    if (want <= p.lens[r] || want > most) continue;
+    if (incl[i] <= got || pages_of(p, static_cast<int>(want)) <= pages_of(p, p.lens[r])) p.lens[r] = static_cast<int>(want);
   }
 }
 

@@ -330,3 +330,30 @@ def test_evict_with_the_largest_window_and_first_tokens(page, window, sinks):
     both(pool, books, "grow", [0, 1, 2], [290, 0, 7])
     both(pool, books, "evict", [0, 1, 2], window_left=window, sink_tokens=sinks)
     same(pool, books)
+
+
+def test_grow_past_32_bits_of_pages():
+    """All rows of a wide table ask for all columns: more pages than an int counts. None are there for any row."""
+    from greenattention_b200 import kv_pages
+
+    rows, cols, pages = 32768, 65537, 100
+    cache = torch.zeros((pages, 1, 16), dtype=torch.uint8, device="cuda")
+    table = torch.full((rows, cols), -1, dtype=torch.int32, device="cuda")  # 8.6 GB
+    lens, refs = torch.zeros(rows, dtype=torch.int32, device="cuda"), torch.zeros(pages, dtype=torch.int32, device="cuda")
+    pool = kv_pages.PagePool([cache], table, lens, refs)
+    every = torch.arange(rows, dtype=torch.int32, device="cuda")
+    pool.grow(every, torch.full_like(every, cols))
+    assert pool.check_status() == 8
+    assert not lens.any() and not refs.any() and (table[:, :200] == -1).all()
+    some = torch.full_like(every, cols)
+    some[0], some[-1] = 60, 0  # the first row fits; no other does
+    pool.grow(every, some)
+    assert pool.check_status() == 8
+    assert lens[0] == 60 and lens.sum() == 60 and refs.sum() == 60 and (table[1:, :200] == -1).all()
+    assert table[0, :60].tolist() == list(range(60))
+    some[1:] = 0  # rows that need no page, in the shadow of one that finds none
+    some[0], some[1], some[5] = 60, cols, 0
+    lens[7] = 3
+    some[7] = 2
+    pool.grow(every, some)
+    assert pool.check_status() == 8 and lens[0] == 60 and lens[7] == 3 and lens.sum() == 63
