@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) grow_kernel(const __grid_constan
     const long long r = index_at(rows, is64, i);
     return r >= 0 && r < p.rows ? static_cast<int>(r) : -1;
   };
-  const long long most = static_cast<long long>(p.cols) << p.page_shift;  // tokens of a row
+  const long long most = min(static_cast<long long>(p.cols) << p.page_shift, 0x7fffffffLL);  // tokens of a row
   const long long all = p.num_pages + 1LL;
   mark_first(n, mark, row_of);
   long long sum = 0;

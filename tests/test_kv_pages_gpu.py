@@ -357,3 +357,20 @@ def test_grow_past_32_bits_of_pages():
     some[7] = 2
     pool.grow(every, some)
     assert pool.check_status() == 8 and lens[0] == 60 and lens[7] == 3 and lens.sum() == 63
+
+
+@pytest.mark.parametrize("want", [(1 << 31) - 1, 1 << 31, (1 << 31) + 5, (1 << 32) + 7, (1 << 62)])
+def test_grow_to_lengths_that_no_int_holds(want):
+    from greenattention_b200 import kv_pages
+
+    page, cols = 4096, 1 << 20  # 2^32 tokens a row
+    cache = torch.zeros((3, page, 16), dtype=torch.uint8, device="cuda")
+    table = torch.full((2, cols), -1, dtype=torch.int32, device="cuda")
+    pool = kv_pages.PagePool([cache], table, ints([0, 0]), ints([0, 0, 0]))
+    pool.grow(ints([0, 1], torch.int64), ints([want, 5000], torch.int64))
+    first = pool.check_status()
+    assert first == (8 if want < 1 << 31 else 5)
+    if want < 1 << 31:  # asks for 2^19 pages; the row behind it is left as it was
+        assert pool.seqlens.tolist() == [0, 0] and pool.refs.tolist() == [0, 0, 0]
+    else:
+        assert pool.seqlens.tolist() == [0, 5000] and pool.refs.tolist() == [1, 1, 0] and table[1, :2].tolist() == [0, 1]
