@@ -15,6 +15,7 @@ struct Call {
 };
 
 constexpr int kMaxRows = 32768;  // entries of one fork / grow call: their prefix sums lie in shared memory
+constexpr int kMaxPages = 0x7fffffff - 2 * SPAN;  // a kernel's running page, a span further, is still an int
 
 size_t up(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -24,6 +25,7 @@ int fill(const GaPagePool* a, void* stream, Call* c) {
   if (!a) return fail("null pool");
   if (a->tensors <= 0 || a->chunks <= 0 || a->num_pages <= 0 || a->page_size <= 0 || (a->page_size & (a->page_size - 1)))
     return fail("pool of %d tensors, %d chunks, %d pages of %d tokens", a->tensors, a->chunks, a->num_pages, a->page_size);
+  if (a->num_pages > kMaxPages) return fail("%d pages, at most %d", a->num_pages, kMaxPages);
   if (a->rows < 0 || a->cols < 0) return fail("page table of %d x %d", a->rows, a->cols);
   if (!a->base || !a->page_stride || !a->tok_bytes || !a->chunk_tensor || !a->chunk_first || !a->page_table || !a->seqlens ||
       !a->refs || !a->status)

@@ -25,6 +25,7 @@ from greenattention_b200 import _C, dispatch
 
 CHUNK = 16384  # bytes of a copy item of the kernels
 MAX_ROWS = 32768
+MAX_PAGES = (1 << 31) - 1 - 32768
 STATUS_NAMES = {
     1: "a bounded wait for a copy ran out", 3: "a page id was out of range", 5: "a length exceeded the row's entries",
     7: "a row or page index was out of range", 8: "no free page was left", 9: "the page counts did not match the page table",
@@ -57,6 +58,8 @@ class PagePool:
             _no("seqlens and refs are dense, seqlens as long as the page table")
         if (rows > 1 and page_table.stride(0) < cols * max(1, page_table.stride(1))) or (cols > 1 and page_table.stride(1) < 1):
             _no("page_table rows overlap")
+        if pages > MAX_PAGES:
+            _no(f"{pages} pages, at most {MAX_PAGES}")
         page_size = caches[0].shape[1] if caches[0].dim() >= 2 else 0
         if page_size < 1 or page_size & (page_size - 1):
             _no(f"page_size {page_size} is not a power of two")

@@ -100,3 +100,11 @@ def test_struct_layouts_match_the_header():
             if parts[0]:
                 fields += [re.split(r"[\s*]+", parts[0])[-1]] + [x.lstrip("*").strip() for x in parts[1:]]
         assert fields == [n for n, _ in mirror._fields_], name
+
+
+def test_pool_of_more_pages_than_the_kernels_count():
+    n = (1 << 31) - 32768
+    m = dict(dtype=torch.int32, device="meta")
+    for pages, needle in ((n, "at most"), (n - 1, "no CPU path")):
+        with pytest.raises(Exception, match=needle):
+            kv_pages.PagePool([torch.zeros(pages, 1, 4, **m)], torch.zeros(1, 4, **m), torch.zeros(1, **m), torch.zeros(pages, **m))
