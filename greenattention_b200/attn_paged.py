@@ -36,7 +36,7 @@ FP8 = torch.float8_e4m3fn
 STATUS_NAMES = {
     1: "a bounded wait for a full stage ran out", 2: "a bounded wait for a free stage ran out", 4: "shared memory was misplaced",
     3: "a page id was out of range (its keys were taken as zeros)",
-    5: "a cache_seqlens entry exceeded page_table.shape[1] * page_size",
+    5: "a cache_seqlens entry exceeded page_table.shape[1] * page_size, or 2^30",
 }
 _ALLOWED = attn_decode._ALLOWED | {"sink_tokens"}
 logger = logging.getLogger(__name__)

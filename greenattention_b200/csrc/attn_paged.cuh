@@ -40,6 +40,7 @@ enum : int { KV_BF16 = 0, KV_FP16 = 1, KV_E4M3 = 2 };
 enum : int { Q_SAME = 0, Q_BF16_TO_E4M3 = 1 };
 
 constexpr int MAX_WARPS = 8;
+constexpr int MAX_KEYS = 1 << 30;   // keys of a request: sums of two positions, and a tile behind the last, stay ints
 constexpr int SLOT_FLOATS = 32768;  // O floats of a CTA's workspace slot: warps x rows x head_dim of every instance
 constexpr int SLOT_ROWS = 256;      // rows of a CTA's workspace slot, at most
 
@@ -93,7 +94,7 @@ template <int T>
 __device__ __forceinline__ Req req_info(const PagedDev& p, int b, int t0, int nt) {
   Req r;
   int L = p.seqlens[b];
-  const long long cap = static_cast<long long>(p.pt_cols) << p.page_shift;
+  const long long cap = min(static_cast<long long>(p.pt_cols) << p.page_shift, static_cast<long long>(MAX_KEYS));
   if (L > cap) {
     L = static_cast<int>(cap);
     atomicExch(p.status, GA_ST_LEN_RANGE);

@@ -1,5 +1,6 @@
 // C ABI of the attention over 16-bit and e4m3 paged caches with first tokens kept visible (attn_paged.cuh): argument
 // checks, choice of the instance, launches.
+#include <algorithm>
 #include <mutex>
 #include <vector>
 
@@ -318,7 +319,7 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   d.total_q = static_cast<int>(a->total_q);
   d.batch = a->batch;
   d.max_q = a->max_seqlen_q < d.total_q ? a->max_seqlen_q : d.total_q;
-  constexpr int kFar = 1 << 30;  // no position is further away
+  constexpr int kFar = ga::paged::MAX_KEYS;  // no position is further away
   d.window = a->window_left < 0 ? -1 : (a->window_left < kFar ? a->window_left : kFar);
   d.sinks = d.window < 0 ? 0 : (a->sink_tokens < kFar ? a->sink_tokens : kFar);
   d.scale_log2 = a->softmax_scale * 1.4426950408889634f;
@@ -328,7 +329,7 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   d.ws_lse = reinterpret_cast<float*>(ws + prefix_bytes(a->batch));
   d.ws_o = d.ws_lse + static_cast<size_t>(2 * l.sm) * ga::paged::SLOT_ROWS;
   l.st = static_cast<cudaStream_t>(stream);
-  l.max_tokens = static_cast<long long>(a->pt_cols) * a->page_size;
+  l.max_tokens = std::min<long long>(static_cast<long long>(a->pt_cols) * a->page_size, kFar);
   l.prompt = d.max_q > 16;
   if (a->kv_type == ga::paged::KV_BF16) return route<ga::paged::KV_BF16>(l, a->head_dim, a->workspace_bytes);
   if (a->kv_type == ga::paged::KV_FP16) return route<ga::paged::KV_FP16>(l, a->head_dim, a->workspace_bytes);

@@ -194,7 +194,7 @@ typedef struct GaPagedParams {
   const int32_t* page_table;    /* [batch, pt_cols] */
   int64_t pt_stride_row, pt_stride_col;
   int32_t pt_cols;
-  const int32_t* cache_seqlens; /* [batch] keys per request, new tokens included; cut to pt_cols * page_size (status 5) */
+  const int32_t* cache_seqlens; /* [batch] keys per request, new tokens included; cut to pt_cols * page_size and 2^30 (status 5) */
   const int32_t* cu_seqlens_q;  /* [batch + 1] */
   const float* k_descale;       /* [batch | 1, kv_heads] or NULL (= 1) */
   int64_t kd_stride_b, kd_stride_h;

@@ -392,3 +392,27 @@ def test_query_offsets_that_do_not_ascend_stay_in_bounds(new):
     assert (guard[:32] == 3).all() and (guard[32 + 3 * new:] == 3).all()
     attn_paged.check_status()
     check(make(BF16, [50, 60], [40, 40], 16, 8, 2, 64, seed=6))
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF16, 128), (FP8, 256)])
+@pytest.mark.parametrize("new", [1, 20, 200])
+def test_lengths_up_to_the_largest(dtype, hd, new):
+    """The last keys of a request of 2^30 tokens, and lengths beyond, which a wide table would address: cut to 2^30."""
+    from greenattention_b200 import attn_paged
+
+    page, cols, most = 4096, 1 << 20, 1 << 30
+    g = torch.Generator(device="cuda").manual_seed(new)
+    kc, vc = (torch.randn((2, page, 2, hd), generator=g, device="cuda").to(dtype) for _ in range(2))
+    table = torch.full((2, cols), -1, dtype=torch.int32, device="cuda")
+    table[0, most // page - 1], table[0, 0], table[1, 0] = 1, 0, 0
+    kw = dict(q=torch.randn((2 * new, 4, hd), generator=g, device="cuda").to(BF16), k_cache=kc, v_cache=vc, page_table=table,
+              cu_seqlens_q=torch.tensor([0, new, 2 * new], dtype=torch.int32, device="cuda"), max_seqlen_q=new, causal=True,
+              window_size=(300, 0), sink_tokens=5, return_softmax_lse=True)
+    near = dict(kw, page_table=torch.tensor([[0, 1], [0, -1]], dtype=torch.int32, device="cuda"),
+                cache_seqlens=torch.tensor([2 * page, 1000], dtype=torch.int32, device="cuda"))
+    want = paged_oracle.attend(near)
+    for n in (most, most + 1, (1 << 31) - 1):
+        out, lse = attn_paged.attend(**kw, cache_seqlens=torch.tensor([n, 1000], dtype=torch.int32, device="cuda"))
+        assert attn_paged.check_status() == (0 if n == most else 5)
+        assert ((out.cpu().double() - want["out"]).abs() <= want["out_tol"]).all()
+        assert ((lse.cpu().double() - want["lse"]).abs() <= want["lse_tol"]).all()
