@@ -7,9 +7,11 @@
 // evaluated in one pass with the running maximum m and sum l of the row (log2 domain):
 //     m' = max(m, max_j s_ij),  l' = l 2^(m - m') + sum_j 2^(s_ij - m'),  O' = O 2^(m - m') + sum_j 2^(s_ij - m') v_j.
 // Products run on the warp-level 16-bit tensor path with 32-bit accumulators; m, l, O and the partial results are
-// 32 bits. P is rounded to the cache's 16-bit type before P V (bf16 2^-9, fp16 2^-12 of each probability, below the
-// half step 2^-9 / 2^-12 of the output's own rounding); an e4m3 value is an exact fp16 value, so an e4m3 cache runs on
-// the fp16 path with P in fp16. Queries beside an e4m3 cache are e4m3, or bf16 rounded to e4m3 (the contract of the
+// 32 bits. P is rounded to the cache's 16-bit type before P V, by at most 2^-8 (bf16) or 2^-11 (fp16) of each probability:
+// as much again as the rounding of a 16-bit output. fp16 P are taken up to 2^15 (P_TOP), which the sum and the LSE take
+// back: they are subnormal only from 2^-29 of the row's largest down, and a key loses at most 2^-40 of it (2^-25 with P up
+// to 1, so that a long flat tail under one dominant key was lost). An e4m3 value is an exact fp16 value, so an e4m3 cache
+// runs on the fp16 path with P in fp16. Queries beside an e4m3 cache are e4m3, or bf16 rounded to e4m3 (the contract of the
 // FP8 kernels next to this one).
 //
 // What bounds it: the cache's bytes. A warp owns one kv head and a private ring of tiles in shared memory that it fills
@@ -212,6 +214,9 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
+// log2 of the largest P.
+template <int KV>
+constexpr float P_TOP = KV == KV_BF16 ? 0.f : 15.f;
 // Two e4m3 values (the low 16 bits) as two fp16 values: exact.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t v) {
   uint32_t r;
@@ -543,7 +548,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
           }
         }
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) mu[hf] = m[mt][hf] == -INFINITY ? 0.f : m[mt][hf];
+        for (int hf = 0; hf < 2; ++hf) mu[hf] = m[mt][hf] == -INFINITY ? 0.f : m[mt][hf] - P_TOP<KV>;
 #pragma unroll
         for (int j = 0; j < T / 8; ++j)
 #pragma unroll
@@ -609,7 +614,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
           const int row = mt * 16 + hf * 8 + g;
           if (row >= rows) continue;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + lg2(sum);
+          const float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + (lg2(sum) - P_TOP<KV>);
           if (MODE == 0 && !cc.whole) {
             const long long wr = (static_cast<long long>(slot) * p.kvh + h) * I::RC + row;
             float* w = p.ws_o + wr * HD;

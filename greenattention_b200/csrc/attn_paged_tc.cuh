@@ -13,8 +13,9 @@
 //   * The MMAs are issued in an order that needs few barriers: PV(n), then QK(n + 2) into the same buffer. With NQ 2 one
 //     lane issues them all and the pipe runs them in order; with NQ 1 a second lane issues the QK MMAs and waits for the PV
 //     two jobs before. Either way scores that are ready say that the PV two jobs before is done.
-//   * The row's reference maximum moves only when a tile exceeds it by more than 2^8 (P stays below 256, exact in the
-//     sums; the 16-bit rounding of P is relative), so O is rescaled in tensor memory in few tiles.
+//   * The row's reference maximum moves only when a tile exceeds it by more than 2^8 (the lazy rescaling of online softmax),
+//     so O is rescaled in tensor memory in few tiles. At the reference fp16 P are 2^7, so that they stay within 2^15 and a
+//     key loses at most 2^-32 of the row's largest to subnormals; the 16-bit rounding of P is relative otherwise.
 //   * K and V come through one ring of 16 KB stages in the order in which the MMAs use them: a K stage is 128 keys x 64
 //     dims, a V stage 8192 / head_dim keys x all dims, in the 128-byte swizzle that the MMA descriptors name. Where every
 //     key of a stage is seen by some query, TMA boxes of up to a page each fill it (pages of 8 tokens and more); edges of
@@ -44,6 +45,8 @@ constexpr int TK = 128;          // keys of a tile
 constexpr int GK = 32;           // keys of a group
 constexpr int STAGE = 16384;
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
+template <int KV>
+constexpr float P_REF = KV == KV_BF16 ? 0.f : P_TOP<KV> - RISE;  // log2 of P at the reference
 
 // SPLIT_KV: at most 128 rows of each (request, kv head), its keys cut over CTAs (verify). Else row blocks of prompts.
 template <int HD_, int KV_, bool SPLIT_KV_>
@@ -613,7 +616,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             tmem_st32(tO + c * 32, v);
           }
         }
-        sum += part_exp<KV, KEYS>(tS, sl2, ref == -INFINITY ? 0.f : ref, base, w);
+        sum += part_exp<KV, KEYS>(tS, sl2, ref == -INFINITY ? 0.f : ref - P_REF<KV>, base, w);
         wait_st();
         fence_before();
         __syncwarp();
@@ -661,9 +664,9 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         }
       }
       if (I::SPLIT_KV && seg.slot >= 0) {
-        if (real && half == 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = sum == 0.f ? -INFINITY : ref + lg2(sum);
+        if (real && half == 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = sum == 0.f ? -INFINITY : ref + (lg2(sum) - P_REF<KV>);
       } else if (real && half == 0 && p.lse)
-        p.lse[static_cast<long long>(qh) * p.total_q + qrow] = sum == 0.f ? -INFINITY : (ref + lg2(sum)) * 0.6931471805599453f;
+        p.lse[static_cast<long long>(qh) * p.total_q + qrow] = sum == 0.f ? -INFINITY : (ref + (lg2(sum) - P_REF<KV>)) * 0.6931471805599453f;
       if (r.cnt > 0) {
         fence_before();
         __syncwarp();

@@ -15,7 +15,8 @@ def attend(kw: dict) -> dict:
     """``out``, ``lse`` and how far a right kernel may be from them, from the definition, in 64 bits.
 
     ``out_tol``: half a step of the output's type for its rounding; half a step of P's 16-bit type (fp16 beside an e4m3
-    cache) for every probability, i.e. that share of ``sum_j p_j |v_j|``; the fp16 subnormal step where P or out are fp16;
+    cache) for every probability, i.e. that share of ``sum_j p_j |v_j|``; half the fp16 subnormal step where out is fp16, and
+    2^-32 of the row's largest probability for every key where P is (fp16 P are taken up to 2^7 and more);
     and the 32-bit scores: a dot product of ``hd`` terms is off by at most ``hd 2^-23 sum |q_d k_d|`` in any order of
     summation with truncation, which changes every probability by that factor twice (numerator and sum). ``lse_tol``: the
     scores' part, ``n 2^-23`` for the sum of n terms and 2^-20 for the exponentials and the logarithm."""
@@ -65,8 +66,8 @@ def attend(kw: dict) -> dict:
                 out[row, heads] = o
                 e = HALF_STEP[out_type] * o.abs() + (HALF_STEP[p_type] + 2 * off[:, None] + (len(keys) + 64) * 2.0**-23) * spread
                 if p_type == torch.float16:
-                    # P is taken relative to the largest probability so far: its smallest fp16 step, over the sum
-                    e = e + 2.0**-25 * v[:, h].abs().sum(0) * abs(vs) * w.amax(-1)[:, None]
+                    # P is 2^7 at least at the largest probability: half its smallest fp16 step, over the sum
+                    e = e + 2.0**-32 * v[:, h].abs().sum(0) * abs(vs) * w.amax(-1)[:, None]
                 if out_type == torch.float16:
                     e = e + 2.0**-25
                 tol[row, heads] = e * (1 + 2.0**-6)  # products of two of these terms

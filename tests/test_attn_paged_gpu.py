@@ -416,3 +416,45 @@ def test_lengths_up_to_the_largest(dtype, hd, new):
         assert attn_paged.check_status() == (0 if n == most else 5)
         assert ((out.cpu().double() - want["out"]).abs() <= want["out_tol"]).all()
         assert ((lse.cpu().double() - want["lse"]).abs() <= want["lse_tol"]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 5, 17, 300])
+def test_a_long_flat_tail_under_one_dominant_key(dtype, hd, new):
+    """Key 3 scores 18 above all others and its value is 0: what comes out is the tail's share, n e^-18 / (1 + n e^-18), of
+    values of 1, each probability of it 2^-26. The bound is the oracle's: half a step of the output and of P (relative), the
+    32-bit scores and sums, and 2^-32 a key where fp16 P are subnormal."""
+    from greenattention_b200 import attn_paged
+
+    page, kvh, gqa, batch, keys = 64, 2, 4, 3, 20000
+    cols = -(-keys // page)
+    g = torch.Generator().manual_seed(new)
+    table = torch.randperm(batch * cols, generator=g).view(batch, cols).to(torch.int32).cuda()
+    kc, vc = (torch.zeros((batch * cols, page, kvh, hd), device="cuda") for _ in range(2))
+    vc += 1
+    q = torch.zeros((batch * new, kvh * gqa, hd), device="cuda")
+    q[..., 7] = 12
+    first = table[:, 0].long()
+    kc[first, 3, :, 7], vc[first, 3] = 12, 0
+    q_type = BF16 if dtype == FP8 else dtype
+    kw = dict(q=q.to(q_type), k_cache=kc.to(dtype), v_cache=vc.to(dtype), page_table=table,
+              cache_seqlens=torch.full((batch,), keys, dtype=torch.int32, device="cuda"),
+              cu_seqlens_q=torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new, max_seqlen_q=new, causal=True,
+              return_softmax_lse=True, softmax_scale=0.125)
+    out, lse = attn_paged.attend(**kw)
+    assert attn_paged.check_status() == 0
+    n = (keys - new + torch.arange(new, device="cuda").repeat(batch)).double()
+    tail = n * torch.exp(torch.tensor(-18.0, dtype=torch.float64, device="cuda"))
+    want = (tail / (1 + tail))[:, None, None].expand(out.shape)
+    off = hd * 2.0**-23 * 18 + 18 * 2.0**-22
+    p_step, o_step = (2.0**-8 if dtype == BF16 else 2.0**-11), (2.0**-11 if dtype == FP16 else 2.0**-8)
+    bound = (o_step + p_step + 2 * off + (keys + 64) * 2.0**-23) * want * (1 + 2.0**-6)
+    if dtype != BF16:
+        bound = bound + 2.0**-32 * n[:, None, None]
+    if dtype == FP16:
+        bound = bound + 2.0**-25
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), f"{(err / bound).max()} of the bound"
+    z = (18 + torch.log1p(tail)).expand(lse.shape)
+    assert ((lse.double() - z).abs() <= off + keys * 2.0**-23 + 2.0**-20 * (1 + z)).all()
