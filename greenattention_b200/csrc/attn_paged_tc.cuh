@@ -576,8 +576,13 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       const bool any = rr0 < r.nq * p.gqa;  // a warp of padding rows sees nothing and looks at nothing
       w.pmin = any ? r.pos0 + rr0 / p.gqa : -1;
       w.pmax = any ? r.pos0 + (rr0 + 31) / p.gqa : -1;
-      // with a negative descale the queries' signs are flipped as they are gathered; a zero one leaves every score at 0
-      const float sl2 = KV == KV_E4M3 && p.kd ? fmaxf(p.scale_log2 * fabsf(p.kd[b * p.kd_s0 + h * p.kd_s1]), 1e-30f) : p.scale_log2;
+      // with a negative descale the queries' signs are flipped as they are gathered; a zero one leaves every score at 0 (the
+      // masked ones stay below it), one that is no number makes every score none
+      float sl2 = p.scale_log2;
+      if (KV == KV_E4M3 && p.kd) {
+        sl2 *= fabsf(p.kd[b * p.kd_s0 + h * p.kd_s1]);
+        if (sl2 == 0.f) sl2 = 1e-30f;
+      }
       float ref = -INFINITY, sum = 0.f;
       for (int i = 0; i < r.cnt; ++i, n += NQ) {
         const int buf = n & 1;

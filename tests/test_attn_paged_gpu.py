@@ -458,3 +458,21 @@ def test_a_long_flat_tail_under_one_dominant_key(dtype, hd, new):
     assert (err <= bound).all(), f"{(err / bound).max()} of the bound"
     z = (18 + torch.log1p(tail)).expand(lse.shape)
     assert ((lse.double() - z).abs() <= off + keys * 2.0**-23 + 2.0**-20 * (1 + z)).all()
+
+
+@pytest.mark.parametrize("qh,new", [(8, 1), (8, 5), (32, 6), (8, 100)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (40, 3)])
+def test_descales_of_zero_below_it_and_no_number(qh, new, window, sinks):
+    """The same pattern of numbers and NaN whichever kernel the count of rows selects (warp level, slices, prompts)."""
+    from greenattention_b200 import attn_paged
+
+    kw = make(FP8, [200, 130, 160], [new] * 3, 16, qh, 2, 128, window, sinks, seed=new, descale=True)
+    kw["k_descale"].copy_(torch.tensor([[0.0, -0.7], [float("nan"), -0.0], [1.0, 0.25]]))
+    kw["v_descale"].copy_(torch.tensor([[-1.5, 1.0], [1.0, 0.5], [0.0, float("nan")]]))
+    out, lse = attn_paged.attend(**kw)
+    want = paged_oracle.attend(kw)
+    assert torch.equal(out.cpu().isnan(), want["out"].isnan()) and torch.equal(lse.cpu().isnan(), want["lse"].isnan())
+    fine, zfine = ~want["out"].isnan(), ~want["lse"].isnan()
+    assert ((out.cpu().double() - want["out"]).abs() <= want["out_tol"])[fine].all()
+    assert ((lse.cpu().double() - want["lse"]).abs() <= want["lse_tol"])[zfine].all()
+    assert attn_paged.check_status() == 0
