@@ -476,3 +476,74 @@ def test_descales_of_zero_below_it_and_no_number(qh, new, window, sinks):
     assert ((out.cpu().double() - want["out"]).abs() <= want["out_tol"])[fine].all()
     assert ((lse.cpu().double() - want["lse"]).abs() <= want["lse_tol"])[zfine].all()
     assert attn_paged.check_status() == 0
+
+
+def narrow(kw):
+    """The call with query and output rows at multiples of 4 elements that are not multiples of 8: no 16-byte loads."""
+    total, qh, hd = kw["q"].shape
+    q = torch.zeros((total, qh, hd + 4), dtype=kw["q"].dtype, device="cuda")
+    q[..., :hd] = kw["q"]
+    out = torch.full((total, qh, hd + 4), 7.0, dtype=BF16 if kw["k_cache"].dtype == FP8 else kw["k_cache"].dtype, device="cuda")
+    return dict(kw, q=q[..., :hd], out=out[..., :hd])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("qh,kvh,hd,page", [(8, 2, 128, 16), (5, 5, 64, 1), (6, 2, 256, 64)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (50, 7)])
+@pytest.mark.parametrize("new", [1, 5, 90])
+def test_queries_that_only_allow_loads_of_four_elements(dtype, qh, kvh, hd, page, window, sinks, new):
+    kw = narrow(make(dtype, [130, 257, 40, 300], [new, new, 40 if new > 16 else new, 0], page, qh, kvh, hd, window, sinks, seed=hd,
+                     descale=dtype == FP8))
+    check(kw)
+    assert (kw["out"]._base[..., hd:] == 7).all()
+    if dtype == FP8:
+        q = torch.zeros(kw["q"]._base.shape, dtype=FP8, device="cuda")
+        q[..., :hd] = kw["q"].to(FP8)
+        check(dict(kw, q=q[..., :hd], out=None))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("qh,new", [(8, 1), (8, 5), (32, 6), (8, 100)])
+@pytest.mark.parametrize("scale", [0.03, 0.5, 0.0, -0.1])
+def test_given_scales(dtype, qh, new, scale):
+    check(make(dtype, [200, 130, 90], [new, new, min(new, 90)], 16, qh, 2, 128, 60, 4, seed=new, scale=scale, descale=dtype == FP8))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("qh,new", [(8, 1), (8, 5), (32, 6), (8, 100)])
+def test_descales_beside_16_bit_caches(dtype, qh, new):
+    kw = make(dtype, [200, 130, 90], [new, new, min(new, 90)], 16, qh, 2, 128, 60, 4, seed=new, descale=True)
+    kw["k_descale"].copy_(torch.tensor([[0.0, -0.7], [0.4, -0.0], [1.0, 0.25]]))
+    kw["v_descale"].copy_(torch.tensor([[-1.5, 1.0], [1.0, 0.5], [0.0, 3.0]]))
+    check(kw)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("page", [1, 64])
+@pytest.mark.parametrize("new,keys", [(700, 3000), (5, 6000), (24, 6000)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (700, 40)])
+def test_many_tiles_and_items_fp16(hd, page, new, keys, window, sinks):
+    """As above with queries, keys and values in half precision."""
+    from greenattention_b200 import attn_paged
+
+    g = torch.Generator(device="cuda").manual_seed(hd + new)
+    qh, kvh, batch = 16, 4, 5
+    lens = [keys - 37 * b for b in range(batch)]
+    cols = -(-keys // page)
+    pool = [torch.randn((batch * cols, page, kvh, hd), generator=g, device="cuda").to(FP16) for _ in range(2)]
+    table = torch.randperm(batch * cols, generator=g, device="cuda").view(batch, cols).to(torch.int32)
+    q = torch.randn((batch * new, qh, hd), generator=g, device="cuda").to(FP16)
+    kw = dict(q=q, k_cache=pool[0], v_cache=pool[1], page_table=table, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+              cu_seqlens_q=torch.arange(batch + 1, dtype=torch.int32, device="cuda") * new, max_seqlen_q=new, causal=True,
+              return_softmax_lse=True)
+    if window >= 0:
+        kw |= dict(window_size=(window, 0), sink_tokens=sinks)
+    out, lse = attn_paged.attend(**kw)
+    assert attn_paged.check_status() == 0
+    rows = sorted({0, len(q) - 1, *torch.randint(0, len(q), (20,), generator=torch.Generator().manual_seed(1)).tolist()})
+    want, spread, want_lse, off = definition_on_gpu(kw, rows)
+    seen = keys if window < 0 else window + 1 + sinks
+    # the oracle's bound; subnormal P: |v| is below 8, so a key loses at most 2^-32 * 8
+    bound = (2.0**-11 * want.abs() + (2.0**-11 + 2 * off) * spread) * (1 + 2.0**-6) + 2.0**-25 + seen * 2.0**-29
+    assert ((out[rows].double() - want).abs() <= bound).all()
+    assert ((lse[:, rows].double() - want_lse).abs() <= off + 2.0**-20 * (1 + want_lse.abs())).all()
