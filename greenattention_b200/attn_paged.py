@@ -160,7 +160,8 @@ def _prepare(kw: dict):
         if out.dtype != want or out.shape != shape or out.stride(2) != 1:
             return f"out must be {want} of q's shape with last stride 1"
         s0, s1, _ = out.stride()
-        if (s0 | s1) & 3 or out.data_ptr() & 7 or (qh > 1 and s1 < hd) or (total > 1 and s0 < hd):
+        if (s0 | s1) & 3 or out.data_ptr() & 7 or (qh > 1 and s1 < hd) or (total > 1 and s0 < hd) or (
+                qh > 1 and total > 1 and s0 < (qh - 1) * s1 + hd and s1 < (total - 1) * s0 + hd):
             return "out layout: rows must not overlap, strides and the base multiples of 4 elements"
     if dev.type != "cuda":
         return "tensors are on the host: the green kernels have no CPU path"

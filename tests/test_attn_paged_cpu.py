@@ -108,3 +108,13 @@ def test_pool_of_more_pages_than_the_kernels_count():
     for pages, needle in ((n, "at most"), (n - 1, "no CPU path")):
         with pytest.raises(Exception, match=needle):
             kv_pages.PagePool([torch.zeros(pages, 1, 4, **m)], torch.zeros(1, 4, **m), torch.zeros(1, **m), torch.zeros(pages, **m))
+
+
+@pytest.mark.parametrize("strides,ok", [
+    ((1024, 128, 1), True), ((128, 512, 1), True), ((1028, 128, 1), True), ((128, 516, 1), True), ((1152, 144, 1), True),
+    ((128, 128, 1), False), ((1020, 128, 1), False), ((128, 508, 1), False), ((256, 128, 1), False), ((128, 384, 1), False),
+])
+def test_rows_of_out_that_overlap_are_refused(strides, ok):
+    out = torch.empty_strided((4, 8, 128), strides, dtype=BF16, device="meta")
+    why = attn_paged.select(call(out=out))
+    assert ("on the host" if ok else "overlap") in why
