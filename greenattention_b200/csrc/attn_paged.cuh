@@ -45,6 +45,7 @@ constexpr int MAX_WARPS = 8;
 constexpr int MAX_KEYS = 1 << 30;   // keys of a request: sums of two positions, and a tile behind the last, stay ints
 constexpr int SLOT_FLOATS = 32768;  // O floats of a CTA's workspace slot: warps x rows x head_dim of every instance
 constexpr int SLOT_ROWS = 256;      // rows of a CTA's workspace slot, at most
+constexpr int SEG_FLOATS = 512;     // softmax threads of a CTA of the tensor-core kernel, at most
 
 struct PagedDev {
   const uint8_t* q;
@@ -74,6 +75,7 @@ struct PagedDev {
   int* prefix;
   float* ws_o;
   float* ws_lse;
+  float* ws_seg;  // tensor-core kernel: LSE of an item's segments before, a float for each softmax thread
 };
 
 // What the query tokens [t0, t0 + nt) of request b see: tiles of T tokens, the sinks' first, then one run that ends

@@ -16,6 +16,9 @@
 //   * The row's reference maximum moves only when a tile exceeds it by more than 2^8 (the lazy rescaling of online softmax),
 //     so O is rescaled in tensor memory in few tiles. At the reference fp16 P are 2^7, so that they stay within 2^15 and a
 //     key loses at most 2^-32 of the row's largest to subnormals; the 16-bit rounding of P is relative otherwise.
+//   * An item's tiles come in segments of at most 256 (32768 keys): O and the sum are read out, normalised and folded with the
+//     segments before in 32 bits. The tensor cores cut every product to the accumulator's last place, so that over 2^20 keys of
+//     equal weight a single accumulator lost 0.4 % of O (2.3 % over 2^22); and no wait lasts longer than a segment.
 //   * K and V come through one ring of 16 KB stages in the order in which the MMAs use them: a K stage is 128 keys x 64
 //     dims, a V stage 8192 / head_dim keys x all dims, in the 128-byte swizzle that the MMA descriptors name. Where every
 //     key of a stage is seen by some query, TMA boxes of up to a page each fill it (pages of 8 tokens and more); edges of
@@ -44,6 +47,7 @@ constexpr int TM = 128;          // query rows of a tile = tensor memory lanes
 constexpr int TK = 128;          // keys of a tile
 constexpr int GK = 32;           // keys of a group
 constexpr int STAGE = 16384;
+constexpr int SEG_TILES = 256;   // tiles of a segment, at most
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
 template <int KV>
 constexpr float P_REF = KV == KV_BF16 ? 0.f : P_TOP<KV> - RISE;  // log2 of P at the reference
@@ -473,20 +477,24 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   grid_dep_launch();
 
   bool failed = false;
-  // The CTA's segments: a row block of a prompt with all its tiles, or what its gang's slice holds of a request.
+  // The CTA's segments: parts of a row block of a prompt, or of what its gang's slice holds of a request. What the softmax warps
+  // need behind a segment's tiles follows from few numbers (opens, last): they have no registers to spare.
   struct Seg {
     int b, block, h;
-    int i0;    // first tile
-    int slot;  // < 0: the rows' final result; >= 0: a piece, into this workspace slot
-    Req r;     // r.cnt: tiles of the segment
+    int i0, i1;  // tiles of the segment
+    int slot;    // split: workspace slot of the piece, or -1 - the one that a whole request's piece would have gone to
+    bool first;  // split: the piece's first segment
+    Req r;       // r.cnt = i1 - i0
   };
   struct Work {
     int x, end;                 // prompts: item and their number
-    int b, off, rem, gang, h;   // split: place in the slice
+    int b, rem, gang, h, slot;  // split: request and place in the slice, slot of the piece
+    int off, left;              // first tile of the item's next segment, 0 behind its last; split: tiles left of the piece
     bool first;
   };
   auto begin = [&]() {
     Work w;
+    w.off = w.left = 0;
     if (I::SPLIT_KV) {
       w.gang = blockIdx.x / p.kvh;
       w.h = blockIdx.x - w.gang * p.kvh;
@@ -501,35 +509,49 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   };
   auto next = [&](Work& w, Seg& s) {
     if (I::SPLIT_KV) {
-      if (w.rem <= 0) return false;
-      s.r = I::req(p, w.b);
-      while (s.r.cnt == 0) {  // requests without visible keys
-        if (++w.b >= p.batch) return false;
+      s.first = w.left == 0;
+      if (s.first) {  // the next request of the slice
+        if (w.rem <= 0) return false;
+        s.r = I::req(p, w.b);
+        while (s.r.cnt == 0) {  // requests without visible keys
+          if (++w.b >= p.batch) return false;
+          s.r = I::req(p, w.b);
+        }
+        w.left = min(s.r.cnt - w.off, w.rem);
+        w.rem -= w.left;
+        w.slot = (2 * w.gang + (w.first ? 0 : 1)) * p.kvh + w.h;
+        if (w.left == s.r.cnt) w.slot = -1 - w.slot;
+        w.first = false;
+      } else {
         s.r = I::req(p, w.b);
       }
-      const int all = s.r.cnt;
-      const int n = min(all - w.off, w.rem);
       s.b = w.b, s.block = 0, s.h = w.h;
-      s.i0 = w.off;
-      s.slot = n == all ? -1 : (2 * w.gang + (w.first ? 0 : 1)) * p.kvh + w.h;
-      s.r.cnt = n;
-      w.rem -= n;
-      w.off = 0;
-      w.first = false;
-      return ++w.b < p.batch || (w.rem = 0, true);
+      s.slot = w.slot;
+      s.i0 = w.off, s.i1 = w.off + min(w.left, SEG_TILES);
+      w.left -= s.i1 - s.i0;
+      w.off = s.i1;
+      if (w.left == 0) {
+        w.off = 0;
+        if (++w.b >= p.batch) w.rem = 0;
+      }
+    } else {
+      if (w.x >= w.end) return false;
+      const int k = w.x / p.kvh;
+      s.h = w.x - k * p.kvh;
+      const int4 e = list[k];
+      s.b = e.x, s.block = e.y;
+      const int t0 = s.block * I::ROWS / p.gqa, t1 = (s.block * I::ROWS + I::ROWS - 1) / p.gqa;
+      s.r = req_info<GK>(p, s.b, t0, t1 - t0 + 1);
+      const int all = (s.r.cnt + TK / GK - 1) / (TK / GK);
+      s.i0 = w.off, s.i1 = min(all, w.off + SEG_TILES);
+      w.off = s.i1;
+      if (s.i1 == all) w.off = 0, w.x += gridDim.x;
     }
-    if (w.x >= w.end) return false;
-    const int k = w.x / p.kvh;
-    s.h = w.x - k * p.kvh;
-    const int4 e = list[k];
-    s.b = e.x, s.block = e.y;
-    const int t0 = s.block * I::ROWS / p.gqa, t1 = (s.block * I::ROWS + I::ROWS - 1) / p.gqa;
-    s.r = req_info<GK>(p, s.b, t0, t1 - t0 + 1);
-    s.r.cnt = (s.r.cnt + TK / GK - 1) / (TK / GK);
-    s.i0 = 0, s.slot = -1;
-    w.x += gridDim.x;
+    s.r.cnt = s.i1 - s.i0;
     return true;
   };
+  auto opens = [&](const Seg& s) { return I::SPLIT_KV ? s.first : s.i1 <= SEG_TILES; };
+  auto last = [&](const Work& w) { return (I::SPLIT_KV ? w.left : w.off) == 0; };
   // first token of a group; groups behind the last one lie past every visible key
   auto group_at = [](const Req& r, int i) { return (i < r.ns ? i : r.tlo + i - r.ns) * GK; };
 
@@ -544,7 +566,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
     const uint32_t tO = tmem + lanes + I::O_COL + g * HD + half * DIMS;  // this thread's part of the output dims
     const uint32_t xm = sX + (g * 2 * TM + row) * 4;                         // [turn or query tile][half][row]
     int n = NQ == 2 ? g : 0;  // running job
-    int done = 0;             // items with jobs so far
+    int done = 0;             // segments with jobs so far
     uint32_t turn = 0;
     auto exchange = [&](float mine, bool add) {  // maximum or sum over the threads that have the row's parts
       const uint32_t at = xm + turn * (SPLIT * TM * 4);
@@ -584,7 +606,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         if (sl2 == 0.f) sl2 = 1e-30f;
       }
       float ref = -INFINITY, sum = 0.f;
-      for (int i = 0; i < r.cnt; ++i, n += NQ) {
+      for (int i = seg.i0; i < seg.i1; ++i, n += NQ) {
         const int buf = n & 1;
         const uint32_t tS = tmem + lanes + buf * TK + half * KEYS;
         wait_or_flag(b_s + 8 * buf, (n >> 1) & 1, failed, p.status, GA_ST_WAIT_FULL);
@@ -592,7 +614,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         fence_after();
         int base[KEYS / GK];
 #pragma unroll
-        for (int c = 0; c < KEYS / GK; ++c) base[c] = group_at(r, (seg.i0 + i) * (TK / GK) + half * (KEYS / GK) + c);
+        for (int c = 0; c < KEYS / GK; ++c) base[c] = group_at(r, i * (TK / GK) + half * (KEYS / GK) + c);
         float mx = part_max<KEYS>(tS, base, w);
         mx = exchange(mx, false) * sl2;
         bool scale = false;
@@ -633,9 +655,27 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       const int qrow = r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
       uint8_t* dst = static_cast<uint8_t*>(p.out) +
                      (static_cast<long long>(qrow) * p.o_s0 + static_cast<long long>(qh) * p.o_s1 + half * DIMS) * 2;
-      const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
-      const float inv = sum == 0.f ? 0.f : vds / sum;
-      if (r.cnt > 0) {
+      // O of the segments before, and their log2 LSE (each thread's own): in the piece's slot, or the CTA's room
+      const int room = !I::SPLIT_KV ? static_cast<int>(blockIdx.x) : (seg.slot < 0 ? -1 - seg.slot : seg.slot);
+      float* ws = p.ws_o + (static_cast<long long>(room) * I::ROWS + g * TM + row) * HD + half * DIMS;
+      float* ws_before = p.ws_seg + static_cast<long long>(blockIdx.x) * (SPLIT * NQ * TM) + tid;
+      const bool has = seg.i1 > 0;
+      const bool piece = !last(work) || (I::SPLIT_KV && seg.slot >= 0);
+      const float before = opens(seg) ? -INFINITY : *ws_before;
+      // what is added of this segment's O and of the one before: their shares, and 1 / sum
+      const bool some = sum != 0.f, more = before != -INFINITY;
+      const float vds = !piece && p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
+      float lse2 = some ? ref + (lg2(sum) - P_REF<KV>) : -INFINITY, mine = vds / sum, theirs = vds;
+      if (more && some) {
+        const float top = fmaxf(before, lse2), wb = ex2(before - top), wm = ex2(lse2 - top), one = 1.f / (wb + wm);
+        mine *= wm * one;
+        theirs *= wb * one;
+        lse2 = top + lg2(wb + wm);
+      } else if (more) {
+        lse2 = before;
+      }
+      if (!last(work)) *ws_before = lse2;
+      if (has) {
         wait_or_flag(b_ofull + 8 * g, done & 1, failed, p.status, GA_ST_WAIT_FULL);
         __syncwarp();
         fence_after();
@@ -643,36 +683,47 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
 #pragma unroll 1
       for (int c = 0; c < DIMS / 32; ++c) {
         uint32_t v[32];
-        if (r.cnt > 0) {
+        if (has) {
           tmem_ld32(tO + c * 32, v);
           wait_ld();
         }
-        if (I::SPLIT_KV && seg.slot >= 0) {
-          const float one = sum == 0.f ? 0.f : 1.f / sum;
-          float* ws = p.ws_o + (static_cast<long long>(seg.slot) * TM + row) * HD + half * DIMS + c * 32;
-          if (real) {
-#pragma unroll
-            for (int k = 0; k < 32; k += 4)
-              *reinterpret_cast<float4*>(ws + k) = make_float4(__uint_as_float(v[k]) * one, __uint_as_float(v[k + 1]) * one,
-                                                               __uint_as_float(v[k + 2]) * one, __uint_as_float(v[k + 3]) * one);
-          }
-        } else if (real) {
+        if (real && !piece && !more) {
 #pragma unroll
           for (int k = 0; k < 32; k += 4) {
             uint2 o = make_uint2(0u, 0u);
-            if (r.cnt > 0 && sum != 0.f) {
-              o.x = pack16<OKV>(__uint_as_float(v[k]) * inv, __uint_as_float(v[k + 1]) * inv);
-              o.y = pack16<OKV>(__uint_as_float(v[k + 2]) * inv, __uint_as_float(v[k + 3]) * inv);
+            if (some) {
+              o.x = pack16<OKV>(__uint_as_float(v[k]) * mine, __uint_as_float(v[k + 1]) * mine);
+              o.y = pack16<OKV>(__uint_as_float(v[k + 2]) * mine, __uint_as_float(v[k + 3]) * mine);
             }
             *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = o;
           }
+        } else if (real && !more) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            *reinterpret_cast<float4*>(ws + c * 32 + k) =
+                some ? make_float4(__uint_as_float(v[k]) * mine, __uint_as_float(v[k + 1]) * mine, __uint_as_float(v[k + 2]) * mine,
+                                   __uint_as_float(v[k + 3]) * mine)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        } else if (real) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4) {
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (some)
+              o = make_float4(__uint_as_float(v[k]) * mine, __uint_as_float(v[k + 1]) * mine, __uint_as_float(v[k + 2]) * mine,
+                              __uint_as_float(v[k + 3]) * mine);
+            float4* at = reinterpret_cast<float4*>(ws + c * 32 + k);
+            const float4 w = *at;
+            o.x += w.x * theirs, o.y += w.y * theirs, o.z += w.z * theirs, o.w += w.w * theirs;
+            if (piece) *at = o;
+            else *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = make_uint2(pack16<OKV>(o.x, o.y), pack16<OKV>(o.z, o.w));
+          }
         }
       }
-      if (I::SPLIT_KV && seg.slot >= 0) {
-        if (real && half == 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = sum == 0.f ? -INFINITY : ref + (lg2(sum) - P_REF<KV>);
-      } else if (real && half == 0 && p.lse)
-        p.lse[static_cast<long long>(qh) * p.total_q + qrow] = sum == 0.f ? -INFINITY : (ref + (lg2(sum) - P_REF<KV>)) * 0.6931471805599453f;
-      if (r.cnt > 0) {
+      if (real && half == 0 && last(work)) {
+        if (I::SPLIT_KV && seg.slot >= 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = lse2;
+        else if (p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
+      }
+      if (has) {
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(b_ofree + 8 * g);

@@ -23,7 +23,9 @@ struct Launch {
 };
 
 size_t prefix_bytes(int batch) { return (static_cast<size_t>(batch) + 1 + 63) / 64 * 256; }
-size_t slots_bytes(int sm) { return static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) * 4; }
+size_t slots_bytes(int sm) {
+  return (static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) + static_cast<size_t>(sm) * ga::paged::SEG_FLOATS) * 4;
+}
 
 template <class I>
 int limits() {
@@ -135,7 +137,8 @@ int run_tc_split(Launch& a) {
   const int gangs = a.sm / d.kvh;
   d.nrb = 1;
   int4* list = reinterpret_cast<int4*>(d.ws_lse + static_cast<size_t>(2 * a.sm) * ga::paged::tc::TM);
-  static_assert(ga::paged::SLOT_ROWS >= ga::paged::tc::TM + 16 && I::HD * ga::paged::tc::TM <= ga::paged::SLOT_FLOATS, "workspace");
+  static_assert(ga::paged::SLOT_ROWS >= ga::paged::tc::TM + 16 && I::HD * ga::paged::tc::TM <= ga::paged::SLOT_FLOATS &&
+                    I::SOFT_WARPS * 32 <= ga::paged::SEG_FLOATS, "workspace");
   GA_TRY(ga::api::launch_serial(ga::paged::tc::plan_split_kernel<I>, dim3(1), dim3(1024), 0, a.st, d, gangs, list));
   GA_TRY(ga::api::launch_serial(ga::paged::tc::attn_paged_tc_kernel<I>, dim3(gangs * d.kvh), dim3(I::NT), I::SMEM, a.st, d,
                                 static_cast<const int*>(nullptr), const_cast<const int4*>(list), maps[0], maps[1], static_cast<int>(boxes)));
@@ -148,12 +151,16 @@ int run_tc_split(Launch& a) {
 
 // Prompts on the tensor cores; -1: the call is not one for them.
 template <class I>
-int run_tc(Launch& a, size_t ws_bytes) {
+int run_tc(Launch& a) {
   PagedDev& d = a.d;
   if (!tc_takes<I>(d)) return -1;
   const long long blocks = static_cast<long long>(d.total_q) * d.gqa / I::ROWS + d.batch;
+  // the list in front, O of the segments before (one slot a CTA) in the back half of the slots
+  float* room = d.ws_o + static_cast<size_t>(a.sm) * ga::paged::SLOT_FLOATS;
+  static_assert(I::ROWS * I::HD <= ga::paged::SLOT_FLOATS && I::SOFT_WARPS * 32 <= ga::paged::SEG_FLOATS, "workspace");
   const size_t need = 256 + static_cast<size_t>(blocks) * 16;
-  if (need > ws_bytes || blocks * d.kvh > 0x7fffffffLL) return -1;
+  if (need > static_cast<size_t>(reinterpret_cast<uint8_t*>(room) - reinterpret_cast<uint8_t*>(d.prefix)) || blocks * d.kvh > 0x7fffffffLL) return -1;
+  d.ws_o = room;
   int* count = d.prefix;
   int4* list = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(d.prefix) + 256);
   const long long items = blocks * d.kvh;
@@ -201,11 +208,11 @@ int run(Launch& a) {
 }
 
 template <int KV>
-int run_tc_kv(Launch& a, int hd, size_t ws_bytes) {
+int run_tc_kv(Launch& a, int hd) {
   using namespace ga::paged::tc;
-  if (hd == 64) return run_tc<TcInst<64, KV, false>>(a, ws_bytes);
-  if (hd == 128) return run_tc<TcInst<128, KV, false>>(a, ws_bytes);
-  return run_tc<TcInst<256, KV, false>>(a, ws_bytes);
+  if (hd == 64) return run_tc<TcInst<64, KV, false>>(a);
+  if (hd == 128) return run_tc<TcInst<128, KV, false>>(a);
+  return run_tc<TcInst<256, KV, false>>(a);
 }
 
 template <int KV>
@@ -226,10 +233,10 @@ int run_kv(Launch& a, int hd) {
 }
 
 template <int KV>
-int route(Launch& a, int hd, size_t ws_bytes) {
+int route(Launch& a, int hd) {
   int rc = -1;
   if (split_on_tensor_cores<KV>(a, hd)) rc = run_tc_split_kv<KV>(a, hd);
-  else if (a.prompt) rc = run_tc_kv<KV>(a, hd, ws_bytes);
+  else if (a.prompt) rc = run_tc_kv<KV>(a, hd);
   return rc >= 0 ? rc : run_kv<KV>(a, hd);
 }
 
@@ -328,12 +335,13 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   d.prefix = reinterpret_cast<int*>(ws);
   d.ws_lse = reinterpret_cast<float*>(ws + prefix_bytes(a->batch));
   d.ws_o = d.ws_lse + static_cast<size_t>(2 * l.sm) * ga::paged::SLOT_ROWS;
+  d.ws_seg = d.ws_o + static_cast<size_t>(2 * l.sm) * ga::paged::SLOT_FLOATS;
   l.st = static_cast<cudaStream_t>(stream);
   l.max_tokens = std::min<long long>(static_cast<long long>(a->pt_cols) * a->page_size, kFar);
   l.prompt = d.max_q > 16;
-  if (a->kv_type == ga::paged::KV_BF16) return route<ga::paged::KV_BF16>(l, a->head_dim, a->workspace_bytes);
-  if (a->kv_type == ga::paged::KV_FP16) return route<ga::paged::KV_FP16>(l, a->head_dim, a->workspace_bytes);
-  return route<ga::paged::KV_E4M3>(l, a->head_dim, a->workspace_bytes);
+  if (a->kv_type == ga::paged::KV_BF16) return route<ga::paged::KV_BF16>(l, a->head_dim);
+  if (a->kv_type == ga::paged::KV_FP16) return route<ga::paged::KV_FP16>(l, a->head_dim);
+  return route<ga::paged::KV_E4M3>(l, a->head_dim);
 }
 
 }  // extern "C"

@@ -547,3 +547,84 @@ def test_many_tiles_and_items_fp16(hd, page, new, keys, window, sinks):
     bound = (2.0**-11 * want.abs() + (2.0**-11 + 2 * off) * spread) * (1 + 2.0**-6) + 2.0**-25 + seen * 2.0**-29
     assert ((out[rows].double() - want).abs() <= bound).all()
     assert ((lse[:, rows].double() - want_lse).abs() <= off + 2.0**-20 * (1 + want_lse.abs())).all()
+
+
+def repeated(dtype, hd, kvh, gqa, lens, new, seed):
+    """A call over requests whose page tables go round 8 pages of 128 tokens, values between 0.5 and 1.5."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    page, pages = 128, 8
+    kc = (torch.randn((pages, page, kvh, hd), generator=g, device="cuda") * 0.3).to(dtype)
+    vc = (torch.rand((pages, page, kvh, hd), generator=g, device="cuda") + 0.5).to(dtype)
+    cols = -(-max(lens) // page)
+    table = ((torch.arange(cols, device="cuda") + torch.arange(len(lens), device="cuda")[:, None]) % pages).to(torch.int32)
+    news = [min(new, n) for n in lens]
+    q = torch.randn((sum(news), kvh * gqa, hd), generator=g, device="cuda").to(BF16 if dtype == FP8 else dtype)
+    return dict(q=q, k_cache=kc, v_cache=vc, page_table=table, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                cu_seqlens_q=torch.tensor([0] + news, device="cuda").cumsum(0).to(torch.int32), max_seqlen_q=max(news), causal=True,
+                return_softmax_lse=True)
+
+
+def check_repeated(kw, rows, fold=32768):
+    """Some rows against the definition in 64 bits, every token of the pool weighed by how often the row sees it. The bound is
+    the oracle's, with the 32-bit sums (a product cut to the accumulator's last place, at most 2^-23 of it) over `fold` keys:
+    behind so many the sum is put aside. Values are positive, so sum_j p_j |v_j| is the output."""
+    from greenattention_b200 import attn_paged
+
+    out, lse = attn_paged.attend(**kw)
+    again, _ = attn_paged.attend(**kw)
+    assert attn_paged.check_status() == 0 and torch.equal(out, again)
+    page, kvh, hd = kw["k_cache"].shape[1:]
+    dtype, cu, lens = kw["k_cache"].dtype, kw["cu_seqlens_q"].tolist(), kw["cache_seqlens"].tolist()
+    p_step, o_step = (2.0**-8 if dtype == BF16 else 2.0**-11), (2.0**-11 if dtype == FP16 else 2.0**-8)
+    k, v = (kw[x].double().flatten(0, 1).transpose(0, 1) for x in ("k_cache", "v_cache"))
+    for row in rows:
+        b = max(i for i in range(len(lens)) if cu[i] <= row)
+        n = lens[b] - (cu[b + 1] - cu[b]) + row - cu[b] + 1
+        full = torch.bincount(kw["page_table"][b, : n // page].long(), minlength=len(kw["k_cache"])).repeat_interleave(page)
+        if n % page:
+            full[kw["page_table"][b, n // page].long() * page:][: n % page] += 1
+        q = kw["q"][row].to(dtype).double().view(kvh, -1, hd)
+        s = q @ k.transpose(1, 2) * hd**-0.5
+        off = hd * 2.0**-23 * float((q.abs() @ k.abs().transpose(1, 2)).amax()) * hd**-0.5 + float(s.abs().amax()) * 2.0**-22
+        z = torch.logsumexp(s + full.double().log(), -1)
+        want = (torch.exp(s - z[..., None]) * full) @ v
+        bound = (o_step + (p_step + 2 * off + (min(n, fold) + 64) * 2.0**-23)) * want * (1 + 2.0**-6)
+        err = (out[row].double().view(want.shape) - want).abs()
+        assert (err <= bound).all(), f"row {row}, {n} keys: {(err / bound).max()} of the bound"
+        zerr = (lse[:, row].double().view(z.shape) - z).abs()
+        assert (zerr <= off + (min(n, fold) + 64) * 2.0**-23 + 2.0**-20 * (1 + z)).all()
+
+
+LONG = [1 << 21, 70000, 33000, 5, 90000, 131072, 32768, 32769, 65537, 200, 40000]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("kvh,gqa,new", [(100, 2, 40), (2, 2, 100)])
+def test_sums_over_many_keys(dtype, hd, kvh, gqa, new):
+    """Few gangs with long slices (warp level, split prompts' kernel), and prompts: segments end inside requests and with them."""
+    kw = repeated(dtype, hd, kvh, gqa, LONG, new, hd + new)
+    cu = kw["cu_seqlens_q"].tolist()
+    check_repeated(kw, sorted({x for a, b in zip(cu, cu[1:]) for x in (a, b - 1)}))
+
+
+def test_an_item_that_lasts_seconds():
+    """A prompt on 2^27 keys (one page, named by every entry) in front of more items than SMs: the queries of the item behind
+    it wait that long. Keys are 0 and values 1, so every output is 1 and the LSE is the logarithm of the count."""
+    from greenattention_b200 import attn_paged
+
+    page, new, gqa, hd, keys, others = 1024, 20, 8, 64, 1 << 27, 320
+    kc = torch.zeros((1, page, 1, hd), dtype=BF16, device="cuda")
+    lens = torch.tensor([keys] + [100 + i for i in range(others)], dtype=torch.int32, device="cuda")
+    table = torch.zeros((others + 1, keys // page), dtype=torch.int32, device="cuda")
+    total = (others + 1) * new
+    q = torch.randn((total, gqa, hd), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(BF16)
+    out, lse = attn_paged.attend(q=q, k_cache=kc, v_cache=torch.ones_like(kc), page_table=table, cache_seqlens=lens,
+                                 cu_seqlens_q=torch.arange(others + 2, dtype=torch.int32, device="cuda") * new, max_seqlen_q=new,
+                                 causal=True, return_softmax_lse=True)
+    assert attn_paged.check_status() == 0
+    seen = (lens[:, None] - new + 1 + torch.arange(new, device="cuda")).flatten().double()
+    # sums of at most 32768 equal numbers are exact; each of the folds behind rounds the shares and the LSE a few times
+    folds = (seen / 32768).ceil()
+    assert ((out.double() - 1).abs() <= (2.0**-8 + folds * 2.0**-22)[:, None, None]).all()
+    assert ((lse.double() - seen.log()).abs() <= (2.0**-20 + folds * 2.0**-22) * (1 + seen.log())).all()
