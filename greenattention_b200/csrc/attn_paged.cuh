@@ -43,6 +43,11 @@ enum : int { Q_SAME = 0, Q_BF16_TO_E4M3 = 1 };
 
 constexpr int MAX_WARPS = 8;
 constexpr int MAX_KEYS = 1 << 30;   // keys of a request: sums of two positions, and a tile behind the last, stay ints
+// Keys after which O and the sum are put aside, normalised, and begun anew: the tensor cores cut every product to the last place
+// of the accumulator that it goes into, so that over 2^20 keys of equal weight a single accumulator lost 0.4 % of O (2.3 % over
+// 2^22). Rounding every 16 keys' products into O instead (as MODE 1 does, which has no workspace) made decode 3 % slower and
+// 32-row blocks 16 %.
+constexpr int FOLD_KEYS = 32768;
 constexpr int SLOT_FLOATS = 32768;  // O floats of a CTA's workspace slot: warps x rows x head_dim of every instance
 constexpr int SLOT_ROWS = 256;      // rows of a CTA's workspace slot, at most
 constexpr int SEG_FLOATS = 512;     // softmax threads of a CTA of the tensor-core kernel, at most
@@ -207,6 +212,18 @@ __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uin
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same for O. APART: the sum of the 16 products is rounded to nearest on its way into d.
+template <int KV, bool APART>
+__device__ __forceinline__ void pv16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (!APART) {
+    mma16<KV>(d, a, b0, b1);
+  } else {
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+    mma16<KV>(c, a, b0, b1);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) d[e] += c[e];
+  }
+}
 template <int KV>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if (KV == KV_BF16) {
@@ -268,24 +285,33 @@ struct Cursor {
   Req r;
   int t, t_end;    // tiles of the current segment
   long long rem;   // tiles of the slice after this segment
-  bool live, whole, first;
+  bool live, first;
+  bool whole;      // the slice holds all of the unit
+  bool more;       // the unit's segments before were put aside
 };
 
+// A segment of tiles of the current unit from t_off on; at most FOLD_KEYS of them where there is a workspace for what is put aside.
 template <class I, int MODE>
-__device__ __forceinline__ void open_segment(const PagedDev& p, Cursor& c, int t_off) {
+__device__ __forceinline__ void open_segment(const PagedDev& p, Cursor& c, int t_off, bool more) {
   const long long left = c.r.cnt - t_off;
-  const long long n = left < c.rem ? left : c.rem;
+  long long n = left < c.rem ? left : c.rem;
+  if (!more) c.whole = t_off == 0 && n == left;
+  c.more = more;
+  if (MODE == 0 && n > FOLD_KEYS / I::T) n = FOLD_KEYS / I::T;
   c.t = t_off;
   c.t_end = t_off + static_cast<int>(n);
   c.rem -= n;
-  c.whole = t_off == 0 && c.t_end == c.r.cnt;
 }
-// To the next tile; to the next unit behind the segment's last one.
+// To the next tile; to the next segment behind the last one.
 template <class I, int MODE>
 __device__ __forceinline__ void advance(const PagedDev& p, Cursor& c) {
   if (++c.t < c.t_end) return;
   if (MODE == 1 || c.rem <= 0) {
     c.live = false;
+    return;
+  }
+  if (c.t < c.r.cnt) {
+    open_segment<I, MODE>(p, c, c.t, true);
     return;
   }
   c.first = false;
@@ -299,7 +325,7 @@ __device__ __forceinline__ void advance(const PagedDev& p, Cursor& c) {
       c.r = req_info<I::T>(p, c.b, 0, p.max_q);
     } while (c.r.cnt == 0);
   }
-  open_segment<I, MODE>(p, c, 0);
+  open_segment<I, MODE>(p, c, 0, false);
 }
 
 // MODE 0: the tile stream cut evenly over all gangs (decode, verify). MODE 1: a gang takes one row block with the tiles that
@@ -338,7 +364,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
     ci.block = unit;
     ci.rem = g1 - g0;
     ci.live = ci.first = true;
-    open_segment<I, MODE>(p, ci, static_cast<int>(in - static_cast<long long>(unit) * ci.r.cnt));
+    open_segment<I, MODE>(p, ci, static_cast<int>(in - static_cast<long long>(unit) * ci.r.cnt), false);
   } else {
     auto blocks = [&](int b) {
       int q0;
@@ -353,7 +379,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
     ci.r = req_info<T>(p, ci.b, t0, t1 - t0 + 1);
     ci.rem = ci.r.cnt;
     ci.live = ci.r.cnt > 0;
-    open_segment<I, MODE>(p, ci, 0);
+    open_segment<I, MODE>(p, ci, 0, false);
   }
 
   const uint32_t ring = smem_u32(smem_raw) + warp * (I::NST * I::STAGE);
@@ -578,8 +604,8 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
             ldsm_x4_trans(va + swz<RB>(row, d * 2 + cx), r0, r1, r2, r3);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma16<KV>(o[mt][2 * d], a[mt], r0, r1);
-              mma16<KV>(o[mt][2 * d + 1], a[mt], r2, r3);
+              pv16<KV, MODE == 1>(o[mt][2 * d], a[mt], r0, r1);
+              pv16<KV, MODE == 1>(o[mt][2 * d + 1], a[mt], r2, r3);
             }
           }
         } else {
@@ -593,8 +619,8 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
               const uint32_t o0 = e4m3x2_to_f16x2(prmt(r[2 * i], 0, 0x4431)), o1 = e4m3x2_to_f16x2(prmt(r[2 * i + 1], 0, 0x4431));
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
-                mma16<KV>(o[mt][4 * d + 2 * i], a[mt], e0, e1);
-                mma16<KV>(o[mt][4 * d + 2 * i + 1], a[mt], o0, o1);
+                pv16<KV, MODE == 1>(o[mt][4 * d + 2 * i], a[mt], e0, e1);
+                pv16<KV, MODE == 1>(o[mt][4 * d + 2 * i + 1], a[mt], o0, o1);
               }
             }
           }
@@ -606,47 +632,113 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
     if (last) {
       const float vds = p.vd ? p.vd[cc.b * p.vd_s0 + h * p.vd_s1] : 1.f;
       const int slot = 2 * vc + (cc.first ? 0 : 1);
+      const bool on = MODE == 0 && cc.t_end < cc.r.cnt && cc.rem > 0;  // the unit goes on in this slice
+      if (MODE == 0 && (cc.more || on)) {
+        // One of several segments of a unit: what there is so far goes where the unit's piece goes or would have gone.
+        const bool piece = on || !cc.whole;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          float sum = l[mt][hf];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          const int row = mt * 16 + hf * 8 + g;
-          if (row >= rows) continue;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          const float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + (lg2(sum) - P_TOP<KV>);
-          if (MODE == 0 && !cc.whole) {
+          for (int hf = 0; hf < 2; ++hf) {
+            float sum = l[mt][hf];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int row = mt * 16 + hf * 8 + g;
+            if (row >= rows) continue;
             const long long wr = (static_cast<long long>(slot) * p.kvh + h) * I::RC + row;
             float* w = p.ws_o + wr * HD;
-#pragma unroll
-            for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
-              if (KV != KV_E4M3) {
-                *reinterpret_cast<float2*>(w + j * 8 + tq * 2) = make_float2(o[mt][j][hf * 2] * inv, o[mt][j][hf * 2 + 1] * inv);
+            const float one = piece ? 1.f : vds;
+            float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + (lg2(sum) - P_TOP<KV>);
+            float f = one / sum, theirs = one;
+            if (cc.more) {
+              const float before = __ldcg(p.ws_lse + wr);
+              if (sum == 0.f) {
+                lse2 = before;
               } else {
-                *reinterpret_cast<float4*>(w + j * 8 + tq * 4) =
-                    make_float4(o[mt][j][hf * 2] * inv, o[mt][j + 1][hf * 2] * inv, o[mt][j][hf * 2 + 1] * inv, o[mt][j + 1][hf * 2 + 1] * inv);
+                const float top = fmaxf(before, lse2), wb = before == -INFINITY ? 0.f : ex2(before - top), wm = ex2(lse2 - top);
+                f *= wm / (wb + wm);
+                theirs *= wb / (wb + wm);
+                lse2 = top + lg2(wb + wm);
               }
             }
-            if (tq == 0) p.ws_lse[wr] = lse2;
-          } else {
-            const int rr = block * I::RC + row, tok = rr / p.gqa;
-            const int qrow = cc.r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
-            uint8_t* dst = static_cast<uint8_t*>(p.out) + (qrow * p.o_s0 + qh * p.o_s1) * 2;
-            const float f = sum == 0.f ? 0.f : inv * vds;
+            // columns of n8 tiles j and, beside an e4m3 cache, j + 1: this thread's two or four dims
 #pragma unroll
             for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
+              float v[4];
               if (KV != KV_E4M3) {
-                *reinterpret_cast<uint32_t*>(dst + (j * 8 + tq * 2) * 2) = pack16<KV>(o[mt][j][hf * 2] * f, o[mt][j][hf * 2 + 1] * f);
+                v[0] = o[mt][j][hf * 2], v[1] = o[mt][j][hf * 2 + 1];
               } else {
-                uint2 w;
-                w.x = pack16<KV_BF16>(o[mt][j][hf * 2] * f, o[mt][j + 1][hf * 2] * f);
-                w.y = pack16<KV_BF16>(o[mt][j][hf * 2 + 1] * f, o[mt][j + 1][hf * 2 + 1] * f);
-                *reinterpret_cast<uint2*>(dst + (j * 8 + tq * 4) * 2) = w;
+                v[0] = o[mt][j][hf * 2], v[1] = o[mt][j + 1][hf * 2], v[2] = o[mt][j][hf * 2 + 1], v[3] = o[mt][j + 1][hf * 2 + 1];
+              }
+              constexpr int N = KV == KV_E4M3 ? 4 : 2;
+              const int at = j * 8 + tq * N;
+#pragma unroll
+              for (int e = 0; e < N; ++e) v[e] = sum == 0.f ? 0.f : v[e] * f;
+              if (cc.more) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) v[e] += w[at + e] * theirs;
+              }
+              if (piece) {
+                if (KV != KV_E4M3) *reinterpret_cast<float2*>(w + at) = make_float2(v[0], v[1]);
+                else *reinterpret_cast<float4*>(w + at) = make_float4(v[0], v[1], v[2], v[3]);
+              } else {
+                const int rr = block * I::RC + row, tok = rr / p.gqa;
+                uint8_t* dst = static_cast<uint8_t*>(p.out) + ((cc.r.q0 + tok) * p.o_s0 + (h * p.gqa + rr - tok * p.gqa) * p.o_s1 + at) * 2;
+                if (KV != KV_E4M3) *reinterpret_cast<uint32_t*>(dst) = pack16<KV>(v[0], v[1]);
+                else *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<KV_BF16>(v[0], v[1]), pack16<KV_BF16>(v[2], v[3]));
               }
             }
-            if (tq == 0 && p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
+            if (tq == 0) {
+              const int rr = block * I::RC + row, tok = rr / p.gqa, qh = h * p.gqa + rr - tok * p.gqa;
+              if (piece) p.ws_lse[wr] = lse2;
+              else if (p.lse) p.lse[static_cast<long long>(qh) * p.total_q + cc.r.q0 + tok] = lse2 * 0.6931471805599453f;
+            }
+          }
+        }
+        __syncwarp();  // a row's LSE is written by one lane and read by four
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            float sum = l[mt][hf];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int row = mt * 16 + hf * 8 + g;
+            if (row >= rows) continue;
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const float lse2 = sum == 0.f ? -INFINITY : m[mt][hf] + (lg2(sum) - P_TOP<KV>);
+            if (MODE == 0 && !cc.whole) {
+              const long long wr = (static_cast<long long>(slot) * p.kvh + h) * I::RC + row;
+              float* w = p.ws_o + wr * HD;
+#pragma unroll
+              for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
+                if (KV != KV_E4M3) {
+                  *reinterpret_cast<float2*>(w + j * 8 + tq * 2) = make_float2(o[mt][j][hf * 2] * inv, o[mt][j][hf * 2 + 1] * inv);
+                } else {
+                  *reinterpret_cast<float4*>(w + j * 8 + tq * 4) =
+                      make_float4(o[mt][j][hf * 2] * inv, o[mt][j + 1][hf * 2] * inv, o[mt][j][hf * 2 + 1] * inv, o[mt][j + 1][hf * 2 + 1] * inv);
+                }
+              }
+              if (tq == 0) p.ws_lse[wr] = lse2;
+            } else {
+              const int rr = block * I::RC + row, tok = rr / p.gqa;
+              const int qrow = cc.r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
+              uint8_t* dst = static_cast<uint8_t*>(p.out) + (qrow * p.o_s0 + qh * p.o_s1) * 2;
+              const float f = sum == 0.f ? 0.f : inv * vds;
+#pragma unroll
+              for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
+                if (KV != KV_E4M3) {
+                  *reinterpret_cast<uint32_t*>(dst + (j * 8 + tq * 2) * 2) = pack16<KV>(o[mt][j][hf * 2] * f, o[mt][j][hf * 2 + 1] * f);
+                } else {
+                  uint2 w;
+                  w.x = pack16<KV_BF16>(o[mt][j][hf * 2] * f, o[mt][j + 1][hf * 2] * f);
+                  w.y = pack16<KV_BF16>(o[mt][j][hf * 2 + 1] * f, o[mt][j + 1][hf * 2 + 1] * f);
+                  *reinterpret_cast<uint2*>(dst + (j * 8 + tq * 4) * 2) = w;
+                }
+              }
+              if (tq == 0 && p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
+            }
           }
         }
       }

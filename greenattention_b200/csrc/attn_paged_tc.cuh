@@ -47,7 +47,7 @@ constexpr int TM = 128;          // query rows of a tile = tensor memory lanes
 constexpr int TK = 128;          // keys of a tile
 constexpr int GK = 32;           // keys of a group
 constexpr int STAGE = 16384;
-constexpr int SEG_TILES = 256;   // tiles of a segment, at most
+constexpr int SEG_TILES = FOLD_KEYS / TK;  // tiles of a segment, at most
 constexpr float RISE = 8.f;      // log2: how far a row's maximum may exceed the reference before O is rescaled
 template <int KV>
 constexpr float P_REF = KV == KV_BF16 ? 0.f : P_TOP<KV> - RISE;  // log2 of P at the reference

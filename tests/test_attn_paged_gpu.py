@@ -600,10 +600,18 @@ LONG = [1 << 21, 70000, 33000, 5, 90000, 131072, 32768, 32769, 65537, 200, 40000
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
 @pytest.mark.parametrize("hd", [64, 128, 256])
-@pytest.mark.parametrize("kvh,gqa,new", [(100, 2, 40), (2, 2, 100)])
+@pytest.mark.parametrize("kvh,gqa,new", [(512, 1, 1), (100, 2, 40), (2, 2, 100)])
 def test_sums_over_many_keys(dtype, hd, kvh, gqa, new):
     """Few gangs with long slices (warp level, split prompts' kernel), and prompts: segments end inside requests and with them."""
     kw = repeated(dtype, hd, kvh, gqa, LONG, new, hd + new)
+    cu = kw["cu_seqlens_q"].tolist()
+    check_repeated(kw, sorted({x for a, b in zip(cu, cu[1:]) for x in (a, b - 1)}))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_sums_over_many_keys_without_16_byte_queries(dtype, hd):
+    kw = narrow(repeated(dtype, hd, 2, 2, [1 << 20, 70000, 90], 50, hd))
     cu = kw["cu_seqlens_q"].tolist()
     check_repeated(kw, sorted({x for a, b in zip(cu, cu[1:]) for x in (a, b - 1)}))
 
