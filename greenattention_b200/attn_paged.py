@@ -9,8 +9,8 @@ The call contract is that of ``attn_decode`` (same names, layouts, causal and wi
   request's first ``S`` keys. The pages between the first tokens and the window are never read, so their page-table
   entries may be those of released pages (``kv_pages.PagePool.evict``) and the lengths go on counting;
 * a row that sees no key gets zeros and an LSE of -inf; rows of ``out`` and ``lse`` behind the last request's are left
-  as they were. Non-finite values count where they are visible; a K or V row that no query of the call's request sees
-  is not read. (Among the new tokens of one request a later token's non-finite V row reaches the earlier rows.)
+  as they were. Non-finite values count where they are visible, and reach no row that does not see them; a K or V row
+  that no query of the call's request sees is not read.
 
 Every call brings its own scratch (from torch's caching allocator, on the current stream), so calls on several streams
 and captured graphs do not share any. What the kernels cannot serve is declined with a reason (``dispatch.Declined``).

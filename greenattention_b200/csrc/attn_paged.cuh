@@ -80,6 +80,7 @@ struct PagedDev {
   int* prefix;
   float* ws_o;
   float* ws_lse;
+  int* ws_spoilt;  // MODE 1: whether a result is no number
   float* ws_seg;  // tensor-core kernel: LSE of an item's segments before, a float for each softmax thread
 };
 
@@ -251,6 +252,174 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// ------------------------------------------------------------------------------------------- values that are no numbers
+
+// P of a key that a row does not see is 0, and 0 times an infinity or NaN is NaN: a V row with such values spoils, in a matrix
+// product, rows that do not see it. So the results of calls with several new tokens are looked at, by the kernel behind or (prompts)
+// as they are written; where one is no number the kernel behind finds the V rows with such values that only some rows of the
+// block see, and computes the rows anew that do not see all of them. (Looking at every such V row ahead of the product instead
+// cost prompts 3 to 20 %.)
+
+// The places of a word that hold infinities or NaN, as bits 15 and 31 (16-bit types) or 7, 15, 23 and 31 (e4m3, NaN).
+template <int KV>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t EXP = KV == KV_BF16 ? 0x7f807f80u : (KV == KV_FP16 ? 0x7c007c00u : 0x7f7f7f7fu);
+  constexpr uint32_t ONE = KV == KV_BF16 ? 0x00800080u : (KV == KV_FP16 ? 0x04000400u : 0x01010101u);
+  return ((w & EXP) + ONE) & (KV == KV_E4M3 ? 0x80808080u : 0x80008000u);
+}
+// Products of two words' 16-bit values with 0, added up: no number once one of them was none.
+template <int KV>
+__device__ __forceinline__ void look_at(uint32_t& acc, uint32_t x, uint32_t y) {
+  if (KV == KV_FP16)
+    asm("fma.rn.f16x2 %0, %1, %3, %0;\n\tfma.rn.f16x2 %0, %2, %3, %0;" : "+r"(acc) : "r"(x), "r"(y), "r"(0u));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %3, %0;\n\tfma.rn.bf16x2 %0, %2, %3, %0;" : "+r"(acc) : "r"(x), "r"(y), "r"(0u));
+}
+// Value `d` of a row of the cache.
+template <int KV>
+__device__ __forceinline__ float value_at(const uint8_t* row, int d) {
+  if (KV == KV_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[d]);
+  if (KV == KV_FP16) return __half2float(reinterpret_cast<const __half*>(row)[d]);
+  const uint32_t two = e4m3x2_to_f16x2(row[d]);
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(two)));
+}
+
+constexpr int MEND_KEYS = 64;
+template <int HD, int NW>
+struct MendSmem {
+  float q[NW][HD];       // a warp's query row
+  int keys[MEND_KEYS];   // V rows that are no numbers
+  int n;
+};
+// By the NW first warps of a CTA, which meet in `sync`: request b's rows row0 .. row0 + n of kv head h (row = token * GQA + head), of
+// which a warp takes first, first + step, ...; `r`: what the block's tiles were made of.
+template <int KV, int HD, int NW, typename Sync>
+__device__ __forceinline__ void mend(const PagedDev& p, const Req& r, int b, int h, int row0, int n, int first, int step, MendSmem<HD, NW>& sm,
+                                     Sync sync) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pmin = r.pos0 + row0 / p.gqa, pmax = r.pos0 + (row0 + n - 1) / p.gqa;
+  auto rows_of = [&](int key, const uint8_t*& k, const uint8_t*& v) {  // null: a page that does not exist
+    const int page = p.pt[b * p.pt_s0 + (key >> p.page_shift) * p.pt_s1];
+    const bool real = page >= 0 && page < p.num_pages;
+    k = real ? p.k + page * p.k_s0 + (key & p.page_mask) * p.k_s1 + h * p.k_s2 : nullptr;
+    v = real ? p.v + page * p.v_s0 + (key & p.page_mask) * p.v_s1 + h * p.v_s2 : nullptr;
+  };
+  sync();
+  if (threadIdx.x == 0) sm.n = 0;
+  sync();
+  // keys that are seen, but not by all rows: new tokens, and those that the window leaves behind
+  auto look = [&](int from, int to, int least) {
+#pragma unroll 1
+    for (int key = max(from, 0) + threadIdx.x; key < to; key += NW * 32) {
+      const uint8_t *k, *v;
+      if (key < least) continue;
+      rows_of(key, k, v);
+      uint32_t any = 0;
+      if (v) {
+#pragma unroll 1
+        for (int c = 0; c < HD * (KV == KV_E4M3 ? 1 : 2) / 16; ++c) {
+          const uint4 w = reinterpret_cast<const uint4*>(v)[c];
+          any |= not_finite<KV>(w.x) | not_finite<KV>(w.y) | not_finite<KV>(w.z) | not_finite<KV>(w.w);
+        }
+      }
+      if (any) {
+        const int at = atomicAdd(&sm.n, 1);
+        if (at < MEND_KEYS) sm.keys[at] = key;
+      }
+    }
+  };
+  look(pmin + 1, r.kend, 0);
+  if (p.window >= 0) look(r.lower, min(pmax - p.window, pmin + 1), p.sinks);
+  sync();
+  const int found = sm.n;
+  if (found == 0) return;
+  const float sl2 = p.scale_log2 * (p.kd ? p.kd[b * p.kd_s0 + h * p.kd_s1] : 1.f);
+  const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
+#pragma unroll 1
+  for (int row = first; row < n; row += step) {
+    const int rr = row0 + row, tok = rr / p.gqa, head = h * p.gqa + rr - tok * p.gqa, pos = r.pos0 + tok;
+    uint8_t* out = static_cast<uint8_t*>(p.out) + ((r.q0 + tok) * p.o_s0 + head * p.o_s1) * 2;
+    constexpr int OKV = KV == KV_E4M3 ? KV_BF16 : KV;
+    bool odd = found > MEND_KEYS;  // some value that the row does not see, and one of its own that is no number
+    for (int i = lane; i < found && i < MEND_KEYS; i += 32) {
+      const int key = sm.keys[i];
+      odd |= key > pos || (p.window >= 0 && key < pos - p.window && key >= p.sinks);
+    }
+    bool none = false;
+    for (int d = lane * 2; d < HD; d += 64) none |= not_finite<OKV>(*reinterpret_cast<const uint32_t*>(out + d * 2)) != 0;
+    if (!__any_sync(0xffffffffu, odd) || !__any_sync(0xffffffffu, none)) continue;
+    // the row anew: a lane a key for the scores, lanes over the dims for O
+    const uint8_t* q = p.q + ((r.q0 + tok) * p.q_s0 + head * p.q_s1) * (KV == KV_E4M3 && p.q_kind == Q_SAME ? 1 : 2);
+    __syncwarp();
+    for (int d = lane; d < HD; d += 32) {
+      float x;
+      if (KV == KV_E4M3 && p.q_kind == Q_BF16_TO_E4M3) {
+        const uint32_t two = e4m3x2_to_f16x2(pack_e4m3x2(value_at<KV_BF16>(q, d), 0.f));
+        x = __half2float(__ushort_as_half(static_cast<unsigned short>(two)));
+      } else {
+        x = value_at<KV>(q, d);
+      }
+      sm.q[warp][d] = x;
+    }
+    __syncwarp();
+    float o[HD / 32], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int x = 0; x < HD / 32; ++x) o[x] = 0.f;
+    const int low = p.window >= 0 ? max(0, pos - p.window) : 0, sinks = min(p.sinks, low);
+    const int seen = pos < 0 ? 0 : sinks + pos + 1 - low;
+#pragma unroll 1
+    for (int i0 = 0; i0 < seen; i0 += 32) {
+      const int i = i0 + lane;
+      const uint8_t *k = nullptr, *v = nullptr;
+      float s = -INFINITY;
+      if (i < seen) {
+        rows_of(i < sinks ? i : low + i - sinks, k, v);
+        s = 0.f;
+        if (k)
+#pragma unroll 4
+          for (int d = 0; d < HD; ++d) s += value_at<KV>(k, d) * sm.q[warp][d];
+        s *= sl2;
+      }
+      float top = s;
+#pragma unroll
+      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      top = fmaxf(top, m);
+      const float f = top == -INFINITY ? 1.f : ex2(m - top), e = i < seen ? ex2(s - (top == -INFINITY ? 0.f : top)) : 0.f;
+      m = top;
+      l = l * f + e;
+#pragma unroll
+      for (int x = 0; x < HD / 32; ++x) o[x] *= f;
+#pragma unroll 1
+      for (int x = 0; x < 32 && i0 + x < seen; ++x) {
+        const float w = __shfl_sync(0xffffffffu, e, x);
+        const uint8_t* row_v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), x));
+        if (row_v)
+#pragma unroll
+          for (int y = 0; y < HD / 32; ++y) {
+            const float u = value_at<KV>(row_v, y * 32 + lane);
+            o[y] += fabsf(u) <= 3.4028234663852886e38f ? w * u : u + w;  // (w: its score may be no number)
+          }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+    const float one = l == 0.f ? 0.f : vds / l;
+#pragma unroll
+    for (int y = 0; y < HD / 32; ++y) {
+      const float u = l == 0.f ? 0.f : o[y] * one;
+      if (OKV == KV_FP16) reinterpret_cast<__half*>(out)[y * 32 + lane] = __float2half_rn(u);
+      else reinterpret_cast<__nv_bfloat16*>(out)[y * 32 + lane] = __float2bfloat16_rn(u);
+    }
+  }
+}
+
+// The same by a CTA of four warps, as a call: it is rare, and the kernel around it short.
+template <int KV, int HD>
+__device__ __noinline__ void mend_call(const PagedDev& p, const Req& r, int b, int h, int row0, int n, int first, int step) {
+  __shared__ MendSmem<HD, 4> sm;
+  mend<KV, HD, 4>(p, r, b, h, row0, n, first, step, sm, [] { __syncthreads(); });
+}
+
 // Byte offset of 16-byte chunk `c` of row `r` in a tile whose rows hold RB bytes: rows lie one after the other in
 // 128-byte lines, and the chunks of a line are permuted so that eight rows' chunks c fall into different banks.
 template <int RB>
@@ -273,6 +442,7 @@ struct Inst {
   static constexpr int NST = STAGE <= 4096 ? 6 : 3;        // stages of a warp's ring: 192 KB of shared memory in all
   static constexpr int SMEM = NW * NST * STAGE;
   static constexpr int RC = 16 * MT;                       // rows of a unit
+  static constexpr bool LOOKS = false;                     // whether the kernel looks at the results that it writes itself
   static constexpr int NT = NW * 32;
   static __device__ __forceinline__ Req req(const PagedDev& p, int b) { return req_info<T>(p, b, 0, p.max_q); }
 };
@@ -726,17 +896,22 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
               const int qrow = cc.r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
               uint8_t* dst = static_cast<uint8_t*>(p.out) + (qrow * p.o_s0 + qh * p.o_s1) * 2;
               const float f = sum == 0.f ? 0.f : inv * vds;
+              uint32_t acc = 0;
 #pragma unroll
               for (int j = 0; j < HD / 8; j += (KV == KV_E4M3 ? 2 : 1)) {
                 if (KV != KV_E4M3) {
-                  *reinterpret_cast<uint32_t*>(dst + (j * 8 + tq * 2) * 2) = pack16<KV>(o[mt][j][hf * 2] * f, o[mt][j][hf * 2 + 1] * f);
+                  const uint32_t w = pack16<KV>(o[mt][j][hf * 2] * f, o[mt][j][hf * 2 + 1] * f);
+                  *reinterpret_cast<uint32_t*>(dst + (j * 8 + tq * 2) * 2) = w;
+                  if (MODE == 1) look_at<KV>(acc, w, 0u);
                 } else {
                   uint2 w;
                   w.x = pack16<KV_BF16>(o[mt][j][hf * 2] * f, o[mt][j + 1][hf * 2] * f);
                   w.y = pack16<KV_BF16>(o[mt][j][hf * 2 + 1] * f, o[mt][j + 1][hf * 2 + 1] * f);
                   *reinterpret_cast<uint2*>(dst + (j * 8 + tq * 4) * 2) = w;
+                  if (MODE == 1) look_at<KV_BF16>(acc, w.x, w.y);
                 }
               }
+              if (MODE == 1 && not_finite<KV == KV_E4M3 ? KV_BF16 : KV>(acc)) *p.ws_spoilt = 1;
               if (tq == 0 && p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
             }
           }
@@ -748,6 +923,29 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
     advance<I, MODE>(p, cc);
   }
   cp_async_wait<0>();
+}
+
+// Behind the kernels that write every row themselves (prompts): nothing, unless a result is no number. RC: rows of their blocks.
+template <int KV, int HD, int RC>
+__global__ void __launch_bounds__(128) attn_paged_mend(const __grid_constant__ PagedDev p) {
+  grid_dep_wait();
+  grid_dep_launch();
+  if (__ldcg(p.ws_spoilt) == 0) return;
+  long long before = 0;  // (block, kv head) items of the requests before
+  for (int b = 0; b < p.batch; ++b) {
+    int q0;
+    const int ql = new_tokens(p, b, q0);
+    const long long rows = ql > 0 ? static_cast<long long>(min(ql, p.max_q)) * p.gqa : 0;
+    const long long n = (rows + RC - 1) / RC * p.kvh;
+    for (long long x = (blockIdx.x + gridDim.x - before % gridDim.x) % gridDim.x; x < n; x += gridDim.x) {
+      const int block = static_cast<int>(x / p.kvh), h = static_cast<int>(x - static_cast<long long>(block) * p.kvh);
+      const int t0 = block * RC / p.gqa, t1 = (block * RC + RC - 1) / p.gqa;
+      const Req r = req_info<32>(p, b, t0, t1 - t0 + 1);
+      mend_call<KV, HD>(p, r, b, h, block * RC, static_cast<int>(min(rows - static_cast<long long>(block) * RC, static_cast<long long>(RC))),
+                        threadIdx.x >> 5, 4);
+    }
+    before += n;
+  }
 }
 
 // Folds the pieces of every unit that the main kernel cut, in slice order, and writes the rows of requests without
@@ -765,13 +963,18 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
   grid_dep_launch();
   if (rows <= 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int OKV = I::KV == KV_E4M3 ? KV_BF16 : I::KV;
+  bool none = false;  // a result is no number
   auto store = [&](int row, const float (&v)[VEC], float f, float lse2) {
     const int rr = block * I::RC + row, tok = rr / p.gqa;
     const int qrow = r.q0 + tok, qh = h * p.gqa + rr - tok * p.gqa;
     uint8_t* dst = static_cast<uint8_t*>(p.out) + (qrow * p.o_s0 + qh * p.o_s1 + lane * VEC) * 2;
-    constexpr int OKV = I::KV == KV_E4M3 ? KV_BF16 : I::KV;
 #pragma unroll
-    for (int i = 0; i < VEC; i += 2) *reinterpret_cast<uint32_t*>(dst + i * 2) = pack16<OKV>(v[i] * f, v[i + 1] * f);
+    for (int i = 0; i < VEC; i += 2) {
+      const uint32_t w = pack16<OKV>(v[i] * f, v[i + 1] * f);
+      *reinterpret_cast<uint32_t*>(dst + i * 2) = w;
+      none |= not_finite<OKV>(w) != 0;
+    }
     if (lane == 0 && p.lse) p.lse[static_cast<long long>(qh) * p.total_q + qrow] = lse2 * 0.6931471805599453f;
   };
   const int share = gridDim.z;
@@ -791,7 +994,21 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
     return static_cast<int>(c);
   };
   const int c0 = owner(u0), c1 = owner(u1 - 1);
-  if (c0 == c1) return;
+  if (c0 == c1) {  // its gang has written the rows
+    if (p.max_q == 1 || I::LOOKS) return;
+    constexpr int LPR = HD / 8;  // lanes a row, 16 bytes each
+    const int row0 = (blockIdx.z * 4 + warp) * (32 / LPR) + lane / LPR;
+    for (int row = row0; row < rows; row += 4 * share * (32 / LPR)) {
+      const int rr = block * I::RC + row, tok = rr / p.gqa;
+      const uint8_t* at = static_cast<const uint8_t*>(p.out) + ((r.q0 + tok) * p.o_s0 + (h * p.gqa + rr - tok * p.gqa) * p.o_s1 + lane % LPR * 8) * 2;
+      const uint2 x = __ldcg(reinterpret_cast<const uint2*>(at)), y = __ldcg(reinterpret_cast<const uint2*>(at + 8));
+      none |= (not_finite<OKV>(x.x) | not_finite<OKV>(x.y) | not_finite<OKV>(y.x) | not_finite<OKV>(y.y)) != 0;
+    }
+    if (__syncthreads_or(none))
+      for (int s = 0; s < 32 / LPR; ++s)
+        mend_call<I::KV, HD>(p, r, b, h, block * I::RC, rows, (blockIdx.z * 4 + warp) * (32 / LPR) + s, 4 * share * (32 / LPR));
+    return;
+  }
   const int n = c1 - c0 + 1;  // every gang between them holds a piece too
   const int e0 = u0 <= slice(total, G, c0) ? 0 : 1;
   auto piece = [&](int i) {  // workspace row 0 of the unit's piece i
@@ -865,6 +1082,8 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
       store(row, acc, den == 0.f ? 0.f : vds / den, den == 0.f ? -INFINITY : mx + lg2(den));
     }
   }
+  if (p.max_q > 1 && __syncthreads_or(none))
+    mend_call<I::KV, HD>(p, r, b, h, block * I::RC, rows, many ? (warp ? rows : blockIdx.z) : blockIdx.z * 4 + warp, many ? share : 4 * share);
 }
 
 }  // namespace paged

@@ -90,6 +90,7 @@ struct TcInst {
   static_assert(NST % EG == 0, "ring");
   static constexpr int O_COL = 256;
   static constexpr int RC = ROWS;  // rows of a unit, for the combine kernel
+  static constexpr bool LOOKS = true;
   static __device__ __forceinline__ Req req(const PagedDev& p, int b) {
     Req r = req_info<GK>(p, b, 0, p.max_q);
     r.cnt = (r.cnt + TK / GK - 1) / (TK / GK);
@@ -445,6 +446,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   const uint32_t b_pv = b_p + 16;                            // NQ 1: PV out of a buffer done
   const uint32_t b_ofull = b_pv + 16, b_ofree = b_ofull + 16; // [2] O complete / read
   const uint32_t slot_at = b_ofree + 16;
+  const uint32_t spoilt = slot_at + 8;                       // [2] a result is no number, a wait of the softmax warps ran out
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int MMA_WARP = I::SOFT_WARPS, KV_WARP = MMA_WARP + 2, Q_WARP = KV_WARP + I::KV_WARPS;
 
@@ -463,6 +465,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       mbar_init(b_ofree + 8 * i, I::SPLIT * 4);
     }
     mbar_fence_init();
+    asm volatile("st.shared.v2.b32 [%0], {%1,%1};" ::"r"(spoilt), "r"(0) : "memory");
   }
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot_at), "r"(512) : "memory");
@@ -682,6 +685,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
       }
 #pragma unroll 1
       for (int c = 0; c < DIMS / 32; ++c) {
+        uint32_t acc = 0;
         uint32_t v[32];
         if (has) {
           tmem_ld32(tO + c * 32, v);
@@ -696,6 +700,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
               o.y = pack16<OKV>(__uint_as_float(v[k + 2]) * mine, __uint_as_float(v[k + 3]) * mine);
             }
             *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = o;
+            look_at<OKV>(acc, o.x, o.y);
           }
         } else if (real && !more) {
 #pragma unroll
@@ -714,10 +719,16 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             float4* at = reinterpret_cast<float4*>(ws + c * 32 + k);
             const float4 w = *at;
             o.x += w.x * theirs, o.y += w.y * theirs, o.z += w.z * theirs, o.w += w.w * theirs;
-            if (piece) *at = o;
-            else *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = make_uint2(pack16<OKV>(o.x, o.y), pack16<OKV>(o.z, o.w));
+            if (piece) {
+              *at = o;
+            } else {
+              const uint2 u = make_uint2(pack16<OKV>(o.x, o.y), pack16<OKV>(o.z, o.w));
+              *reinterpret_cast<uint2*>(dst + (c * 32 + k) * 2) = u;
+              look_at<OKV>(acc, u.x, u.y);
+            }
           }
         }
+        if (not_finite<OKV>(acc)) asm volatile("st.shared.b32 [%0], %1;" ::"r"(spoilt), "r"(1) : "memory");
       }
       if (real && half == 0 && last(work)) {
         if (I::SPLIT_KV && seg.slot >= 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = lse2;
@@ -728,6 +739,22 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(b_ofree + 8 * g);
         ++done;
+      }
+    }
+    // The CTA's blocks, or the requests that it has all of, once more if need be; the operands' shared memory is free.
+    auto sync = [] { named_bar_sync(3, I::SOFT_WARPS * 32); };
+    if (failed) asm volatile("st.shared.b32 [%0], %1;" ::"r"(spoilt + 4), "r"(1) : "memory");
+    sync();
+    uint32_t any, lost;  // (where a wait ran out copies may still be on their way)
+    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(any), "=r"(lost) : "r"(spoilt) : "memory");
+    if (any && !lost) {
+      auto& sm = *reinterpret_cast<MendSmem<HD, I::SOFT_WARPS>*>(smem_raw);
+      Work again = begin();
+      Seg s;
+      while (next(again, s)) {
+        const int row0 = s.block * I::ROWS;
+        if (last(again) && !(I::SPLIT_KV && s.slot >= 0))
+          mend<KV, HD, I::SOFT_WARPS>(p, s.r, s.b, s.h, row0, min(s.r.nq * p.gqa - row0, I::ROWS), warp, I::SOFT_WARPS, sm, sync);
       }
     }
   } else {

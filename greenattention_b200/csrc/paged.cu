@@ -24,7 +24,7 @@ struct Launch {
 
 size_t prefix_bytes(int batch) { return (static_cast<size_t>(batch) + 1 + 63) / 64 * 256; }
 size_t slots_bytes(int sm) {
-  return (static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) + static_cast<size_t>(sm) * ga::paged::SEG_FLOATS) * 4;
+  return (static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) + static_cast<size_t>(sm) * ga::paged::SEG_FLOATS + 64) * 4;
 }
 
 template <class I>
@@ -187,8 +187,10 @@ int run(Launch& a) {
     const long long grid = (blocks * d.kvh + I::NW - 1) / I::NW;
     if (grid > 0x7fffffffLL || blocks > 0x7fffffffLL) return fail("too many row blocks");
     d.nrb = 1;
+    GA_TRY(cudaMemsetAsync(d.ws_spoilt, 0, 4, a.st));
     GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_kernel<I, 1>, dim3(static_cast<unsigned>(grid)), dim3(I::NT), I::SMEM, a.st, d));
-    ga::api::launches(1);
+    GA_TRY(ga::api::launch_serial(ga::paged::attn_paged_mend<I::KV, I::HD, I::RC>, dim3(a.sm), dim3(128), 0, a.st, d));
+    ga::api::launches(2);
     return 0;
   }
   d.nrb = static_cast<int>((rows + I::RC - 1) / I::RC);
@@ -336,6 +338,7 @@ int ga_paged_attend(const GaPagedParams* a, void* stream) {
   d.ws_lse = reinterpret_cast<float*>(ws + prefix_bytes(a->batch));
   d.ws_o = d.ws_lse + static_cast<size_t>(2 * l.sm) * ga::paged::SLOT_ROWS;
   d.ws_seg = d.ws_o + static_cast<size_t>(2 * l.sm) * ga::paged::SLOT_FLOATS;
+  d.ws_spoilt = reinterpret_cast<int*>(d.ws_seg + static_cast<size_t>(l.sm) * ga::paged::SEG_FLOATS);
   l.st = static_cast<cudaStream_t>(stream);
   l.max_tokens = std::min<long long>(static_cast<long long>(a->pt_cols) * a->page_size, kFar);
   l.prompt = d.max_q > 16;

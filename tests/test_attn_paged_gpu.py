@@ -636,3 +636,86 @@ def test_an_item_that_lasts_seconds():
     folds = (seen / 32768).ceil()
     assert ((out.double() - 1).abs() <= (2.0**-8 + folds * 2.0**-22)[:, None, None]).all()
     assert ((lse.double() - seen.log()).abs() <= (2.0**-20 + folds * 2.0**-22) * (1 + seen.log())).all()
+
+
+def poison(kw, where):
+    """Values put into (cache, request, key, head, dim) places."""
+    page = kw["k_cache"].shape[1]
+    table = kw["page_table"].tolist()
+    for cache, b, key, h, d, x in where:
+        kw[cache][table[b][key // page], key % page, h, d] = x
+
+
+def check_with_non_finite(kw):
+    from greenattention_b200 import attn_paged
+
+    out, lse = attn_paged.attend(**kw)
+    assert attn_paged.check_status() == 0
+    want = paged_oracle.attend(kw)
+    got, ref = out.cpu().double(), want["out"]
+    odd = (got.isnan() != ref.isnan()).nonzero()
+    assert len(odd) == 0, f"{odd[:5].tolist()} of {len(odd)}"
+    inf = ref.isinf()
+    odd = ((got.isinf() != inf) | inf & (got != ref)).nonzero()
+    assert len(odd) == 0, f"{odd[:5].tolist()} of {len(odd)}"
+    fin = ref.isfinite()
+    assert ((got - ref).abs() <= want["out_tol"])[fin].all()
+    glse, rlse = lse.cpu().double(), want["lse"]
+    assert torch.equal(glse.isnan(), rlse.isnan()) and torch.equal(glse[rlse == -torch.inf], rlse[rlse == -torch.inf])
+    fin = rlse.isfinite()
+    assert ((glse - rlse).abs() <= want["lse_tol"])[fin].all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP8])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("qh,new", [(8, 2), (8, 16), (40, 6), (8, 90)])
+@pytest.mark.parametrize("window,sinks", [(-1, 0), (50, 7), (3, 130)])
+def test_non_finite_values_that_only_some_rows_see(dtype, hd, qh, new, window, sinks):
+    """Infinities and NaN among the new tokens, around the far edge of the first and the last row's window and among the first
+    tokens: they reach the rows that see them and no others. The last request has more new tokens than keys."""
+    inf, nan = (float("nan") if dtype == FP8 else float("inf")), float("nan")
+    lens = [200, 300, 70, new - 1 or 1]
+    where = []
+    for b, n in enumerate(lens[:3]):
+        at = {n - 1: inf, n - new: nan, n - new // 2: -inf, n - new + 1: inf, 2: inf, 5: nan}
+        if window >= 0:
+            at |= {max(0, n - new - window): -inf, max(0, n - new - window + 1): nan, max(0, n - 1 - window): inf, max(0, n - 2 - window): nan}
+        where += [("v_cache", b, j, i % 2, (5 * i + b) % hd, x) for i, (j, x) in enumerate(at.items()) if 0 <= j < n]
+    where += [("v_cache", 3, lens[3] - 1, 0, 9, nan), ("v_cache", 3, 0, 1, 3, inf), ("k_cache", 1, 300 - new // 2, 1, 4, nan)]
+    kw = make(dtype, lens, [new] * 4, 16, qh, 2, hd, window, sinks, seed=new, descale=dtype == FP8)
+    seen = [(n - new - window if window >= 0 else 0, n) for n in lens]  # what the pool holds pages for
+    poison(kw, [w for w in where if w[2] >= seen[w[1]][0] or w[2] < sinks])
+    check_with_non_finite(kw)
+    if new == 90:
+        check_with_non_finite(narrow(kw))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP8])
+@pytest.mark.parametrize("kvh,gqa,new", [(2, 2, 3), (16, 10, 9), (2, 4, 70)])
+def test_non_finite_values_in_split_requests_and_behind_segments(dtype, kvh, gqa, new):
+    """One long request over many CTAs, and over few, in segments: the new tokens' values lie in its last piece."""
+    kw = repeated(dtype, 64, kvh, gqa, [70000, 33000], new, new)
+    own = [torch.empty_like(kw[n][:1]).expand(4, *kw[n].shape[1:]).contiguous() for n in ("k_cache", "v_cache")]
+    for t, n in zip(own, ("k_cache", "v_cache")):  # the last two pages of each request are its own
+        t.copy_(kw[n][:4])
+        kw[n] = torch.cat([kw[n].view(torch.uint8 if dtype == FP8 else torch.int16), t.view(torch.uint8 if dtype == FP8 else torch.int16)]).view(dtype)
+    for b, n in enumerate((70000, 33000)):
+        last = (n - 1) // 128
+        kw["page_table"][b, last - 1], kw["page_table"][b, last] = 8 + 2 * b, 9 + 2 * b
+    clean = dict(kw, v_cache=kw["v_cache"].clone())
+    poison(kw, [("v_cache", 0, 69999, 0, 3, float("nan")), ("v_cache", 0, 70000 - new + 1, 1, 60, float("nan")),
+                ("v_cache", 1, 33000 - new // 2, 1, 0, float("nan"))])
+    from greenattention_b200 import attn_paged
+
+    out, lse = attn_paged.attend(**kw)
+    want, wlse = attn_paged.attend(**clean)
+    assert attn_paged.check_status() == 0 and torch.equal(lse, wlse)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device="cuda").view(2, new, kvh, gqa, 64)
+    hit[0, new - 1:, 0, :, 3] = True
+    hit[0, 1:, 1, :, 60] = True
+    hit[1, new - new // 2:, 1, :, 0] = True
+    hit = hit.view(out.shape)
+    # rows that are computed anew are rounded elsewhere: both results are within the oracle's bound of the definition
+    bound = 2 * (2.0**-8 + (2.0**-11 if dtype == FP8 else 2.0**-8) + (32768 + 64) * 2.0**-23) * want.double()
+    odd = ((out.isnan() != hit) | ~hit & ((out.double() - want.double()).abs() > bound)).nonzero()
+    assert len(odd) == 0, f"{odd[:5].tolist()} of {len(odd)}"
