@@ -67,11 +67,17 @@ bool pool_map(const MapKey& key, CUtensorMap* out) {
   return true;
 }
 
+// Whether an instance of the tensor-core kernel was built with the registers that its split between the roles draws on. Where
+// a compiler gave it fewer its calls go to the warp-level kernel, and the rest of the library is not concerned.
+template <class I>
+bool g_tc_built = false;
+
 template <class I>
 int limits_tc() {
   cudaFuncAttributes at;
   GA_TRY(cudaFuncGetAttributes(&at, reinterpret_cast<const void*>(ga::paged::tc::attn_paged_tc_kernel<I>)));
-  if (at.numRegs < I::REGS) return fail("attn_paged_tc_kernel: built with %d registers a thread, its split needs %d", at.numRegs, I::REGS);
+  g_tc_built<I> = at.numRegs >= I::REGS;
+  if (!g_tc_built<I>) return 0;
   GA_TRY(cudaFuncSetAttribute(reinterpret_cast<const void*>(ga::paged::tc::attn_paged_tc_kernel<I>),
                               cudaFuncAttributeMaxDynamicSharedMemorySize, I::SMEM));
   return 0;
@@ -99,7 +105,7 @@ template <class I>
 bool tc_takes(const PagedDev& d) {
   const bool e4m3 = I::KV == ga::paged::KV_E4M3;
   const int el = e4m3 && d.q_kind == ga::paged::Q_SAME ? 1 : 2;
-  return (!d.kd || e4m3) && d.scale_log2 > 0.f && d.q_s0 * el % 16 == 0 && d.q_s1 * el % 16 == 0 && reinterpret_cast<uintptr_t>(d.q) % 16 == 0;
+  return g_tc_built<I> && (!d.kd || e4m3) && d.scale_log2 > 0.f && d.q_s0 * el % 16 == 0 && d.q_s1 * el % 16 == 0 && reinterpret_cast<uintptr_t>(d.q) % 16 == 0;
 }
 
 // Enough CTAs to spread the rows of a small call over the SMs.
