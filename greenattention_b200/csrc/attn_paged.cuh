@@ -19,9 +19,8 @@
 // in the grid, whatever CTAs they are in) walk the same tokens, one kv head each, which makes the bytes of a token run
 // contiguous in DRAM within a short window whatever the page size (from one token up), strides and alignment. The call is
 // one stream of tiles ordered by (request, row block), cut evenly over the gangs on the device from the live lengths; a
-// unit that is cut leaves normalised 32-bit partials and their
-// log2 LSE in the workspace, folded in slice order by attn_paged_combine (no atomics: results do not depend on
-// scheduling).
+// unit that is cut leaves normalised 32-bit partials and their log2 LSE in the workspace, folded in slice order by
+// attn_paged_combine (no atomics: results do not depend on scheduling).
 //
 // Tiles of 16 or 32 tokens (8 KB of K and V; 4 or 16 KB where a row is narrow or wide) in three stages: two in flight per
 // warp are 128 KB per SM, three times what latency times bandwidth asks for. Measured: 64 requests of 1k..8k tokens, 64 / 8
@@ -80,7 +79,7 @@ struct PagedDev {
   int* prefix;
   float* ws_o;
   float* ws_lse;
-  int* ws_spoilt;  // MODE 1: whether a result is no number
+  int* ws_spoilt;  // whether a result is no number: a word a CTA of the tensor-core kernel's slices, one in MODE 1
   float* ws_seg;  // tensor-core kernel: LSE of an item's segments before, a float for each softmax thread
 };
 
@@ -256,9 +255,9 @@ __device__ __forceinline__ void cp_async_wait() {
 
 // P of a key that a row does not see is 0, and 0 times an infinity or NaN is NaN: a V row with such values spoils, in a matrix
 // product, rows that do not see it. So the results of calls with several new tokens are looked at, by the kernel behind or (prompts)
-// as they are written; where one is no number the kernel behind finds the V rows with such values that only some rows of the
-// block see, and computes the rows anew that do not see all of them. (Looking at every such V row ahead of the product instead
-// cost prompts 3 to 20 %.)
+// as they are written; where one is no number the V rows with such values that only some rows of the block see are looked for, and
+// the rows that do not see all of them are computed anew. (Looking at every such V row ahead of the product instead cost
+// prompts 3 to 20 %.)
 
 // The places of a word that hold infinities or NaN, as bits 15 and 31 (16-bit types) or 7, 15, 23 and 31 (e4m3, NaN).
 template <int KV>
@@ -284,26 +283,279 @@ __device__ __forceinline__ float value_at(const uint8_t* row, int d) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(two)));
 }
 
+// Whether every query between positions pmin and pmax sees the keys [n0, n0 + n).
+__device__ __forceinline__ bool all_see(const PagedDev& p, int n0, int n, int pmin, int pmax) {
+  return n0 + n - 1 <= pmin && (p.window < 0 || n0 >= pmax - p.window || n0 + n <= p.sinks);
+}
+// Rows of K and V of request b's key in head h; null: a page that does not exist.
+__device__ __forceinline__ void rows_of(const PagedDev& p, int b, int h, int key, const uint8_t*& k, const uint8_t*& v) {
+  const int page = p.pt[b * p.pt_s0 + (key >> p.page_shift) * p.pt_s1];
+  const bool real = page >= 0 && page < p.num_pages;
+  k = real ? p.k + page * p.k_s0 + (key & p.page_mask) * p.k_s1 + h * p.k_s2 : nullptr;
+  v = real ? p.v + page * p.v_s0 + (key & p.page_mask) * p.v_s1 + h * p.v_s2 : nullptr;
+}
+__device__ __forceinline__ const uint8_t* shfl_ptr(const uint8_t* x, int lane) {
+  return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(x), lane));
+}
+
+// By one warp, up to 16 rows of request b and kv head h anew, row i being base + i * step < n of the block that begins at row0: steps
+// of 16 keys whose fragments come straight from global memory. V rows that only some of the rows see go into the product
+// without values that are no numbers; those are added to the rows that see them afterwards.
+template <int KV, int HD>
+__device__ __forceinline__ void redo16(const PagedDev& p, const Req& r, int b, int h, int row0, int base, int step, int n) {
+  constexpr int EB = KV == KV_E4M3 ? 1 : 2, OKV = KV == KV_E4M3 ? KV_BF16 : KV;
+  const int lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+  const int rows = min((n - base + step - 1) / step, 16);
+  const float sl2 = p.scale_log2 * (p.kd ? p.kd[b * p.kd_s0 + h * p.kd_s1] : 1.f);
+  const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
+  auto tok_of = [&](int i) { return (row0 + base + i * step) / p.gqa; };
+  auto head_of = [&](int i) { return h * p.gqa + (row0 + base + i * step) % p.gqa; };
+  auto out_of = [&](int i) { return static_cast<uint8_t*>(p.out) + ((r.q0 + tok_of(i)) * p.o_s0 + head_of(i) * p.o_s1) * 2; };
+  const int pmin = r.pos0 + tok_of(0), pmax = r.pos0 + tok_of(rows - 1);
+  int pos[2];
+  uint32_t qf[HD / 16][4];
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    const int i = hf * 8 + g;
+    const bool real = i < rows;
+    pos[hf] = real ? r.pos0 + tok_of(i) : -1;
+    const bool q8 = KV == KV_E4M3 && p.q_kind == Q_SAME;
+    const uint8_t* q = p.q + (real ? ((r.q0 + tok_of(i)) * p.q_s0 + head_of(i) * p.q_s1) * (q8 ? 1 : 2) : 0);
+#pragma unroll
+    for (int x = 0; x < HD / 8; ++x) {  // dims 8 x + 2 tq, + 1
+      uint32_t w = 0;
+      if (real) {
+        if (q8) {
+          w = e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(q + x * 8 + tq * 2));
+        } else {
+          w = *reinterpret_cast<const uint32_t*>(q + (x * 8 + tq * 2) * 2);
+          if (KV == KV_E4M3) w = e4m3x2_to_f16x2(pack_e4m3x2(bf16_bits_to_f32(w & 0xffffu), bf16_bits_to_f32(w >> 16)));
+        }
+      }
+      qf[x / 2][(x & 1) * 2 + hf] = w;
+    }
+  }
+  float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+  const int low = p.window >= 0 ? max(0, pmin - p.window) : 0, sinks = min(p.sinks, low);
+  const int seen = pmax < 0 ? 0 : sinks + pmax + 1 - low;
+  auto key_at = [&](int i) { return i < sinks ? i : low + i - sinks; };
+#pragma unroll 1
+  for (int i0 = 0; i0 < seen; i0 += 16) {
+    const uint8_t *kp = nullptr, *vp = nullptr;
+    bool part = false;
+    if (lane < 16 && i0 + lane < seen) {
+      const int key = key_at(i0 + lane);
+      rows_of(p, b, h, key, kp, vp);
+      part = !all_see(p, key, 1, pmin, pmax);
+    }
+    const uint32_t parts = __ballot_sync(0xffffffffu, part);
+    float s[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      const uint8_t* k = shfl_ptr(kp, j * 8 + g);
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        uint32_t w[2] = {0u, 0u};
+        if (k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint8_t* at = k + (ks * 16 + x * 8 + tq * 2) * EB;
+            w[x] = KV == KV_E4M3 ? e4m3x2_to_f16x2(*reinterpret_cast<const uint16_t*>(at)) : *reinterpret_cast<const uint32_t*>(at);
+          }
+        mma16<KV>(s[j], qf[ks], w[0], w[1]);
+      }
+    }
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + j * 8 + tq * 2 + (e & 1), key = key_at(i), at = pos[e >> 1];
+        const bool sees = i < seen && key <= at && (p.window < 0 || key >= at - p.window || key < p.sinks);
+        s[j][e] = sees ? s[j][e] * sl2 : -INFINITY;
+        top[e >> 1] = fmaxf(top[e >> 1], s[j][e]);
+      }
+    float mu[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 1));
+      top[hf] = fmaxf(top[hf], __shfl_xor_sync(0xffffffffu, top[hf], 2));
+      const float f = top[hf] == -INFINITY ? 1.f : ex2(m[hf] - top[hf]);
+      m[hf] = top[hf];
+      mu[hf] = top[hf] == -INFINITY ? 0.f : top[hf] - P_TOP<KV>;
+      l[hf] *= f;
+#pragma unroll
+      for (int j = 0; j < HD / 8; ++j) o[j][hf * 2] *= f, o[j][hf * 2 + 1] *= f;
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[j][e] = ex2(s[j][e] - mu[e >> 1]);
+        l[e >> 1] += s[j][e];
+      }
+    const uint32_t a[4] = {pack16<KV>(s[0][0], s[0][1]), pack16<KV>(s[0][2], s[0][3]), pack16<KV>(s[1][0], s[1][1]), pack16<KV>(s[1][2], s[1][3])};
+    const uint8_t* v[4];  // of keys 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9
+    uint32_t keep = 0;    // bits of a word that stay whatever they are: those of keys that all rows see
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int at = tq * 2 + (x & 1) + (x >> 1) * 8;
+      v[x] = shfl_ptr(vp, at);
+      keep |= (parts >> at & 1) ? 0u : 1u << x;
+    }
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) {
+      uint32_t w[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        uint32_t u[2];
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint8_t* row = v[x * 2 + y];
+          u[y] = 0u;
+          if (row) u[y] = KV == KV_E4M3 ? row[j * 8 + g] : reinterpret_cast<const uint16_t*>(row)[j * 8 + g];
+          if (!(keep >> (x * 2 + y) & 1) && (not_finite<KV>(u[y]) & (KV == KV_E4M3 ? 0x80u : 0x8000u))) u[y] = 0u;
+        }
+        w[x] = KV == KV_E4M3 ? e4m3x2_to_f16x2(u[0] | u[1] << 8) : (u[0] | u[1] << 16);
+      }
+      pv16<KV, true>(o[j], a, w[0], w[1]);
+    }
+  }
+#pragma unroll
+  for (int hf = 0; hf < 2; ++hf) {
+    float sum = l[hf];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    const int i = hf * 8 + g;
+    if (i < rows) {
+      uint8_t* out = out_of(i);
+      const float f = vds / sum;
+#pragma unroll
+      for (int j = 0; j < HD / 8; ++j)
+        *reinterpret_cast<uint32_t*>(out + (j * 8 + tq * 2) * 2) = sum == 0.f ? 0u : pack16<OKV>(o[j][hf * 2] * f, o[j][hf * 2 + 1] * f);
+    }
+  }
+  __syncwarp();
+  auto add = [&](int from, int to, int least) {
+#pragma unroll 1
+    for (int key = max(max(from, 0), least); key < to; ++key) {
+      const uint8_t *k, *v;
+      rows_of(p, b, h, key, k, v);
+      if (!v) continue;
+#pragma unroll 1
+      for (int d = lane; d < HD; d += 32) {
+        const float x = value_at<KV>(v, d);
+        if (fabsf(x) <= 3.4028234663852886e38f) continue;
+#pragma unroll 1
+        for (int y = 0; y < rows; ++y) {
+          const int at = r.pos0 + tok_of(y);
+          if (key > at || (p.window >= 0 && key < at - p.window && key >= p.sinks)) continue;
+          if (OKV == KV_FP16) {
+            __half* w = reinterpret_cast<__half*>(out_of(y)) + d;
+            *w = __float2half_rn(__half2float(*w) + x * vds);
+          } else {
+            __nv_bfloat16* w = reinterpret_cast<__nv_bfloat16*>(out_of(y)) + d;
+            *w = __float2bfloat16_rn(__bfloat162float(*w) + x * vds);
+          }
+        }
+      }
+    }
+  };
+  add(pmin + 1, pmax + 1, 0);
+  if (p.window >= 0) add(low, min(pmax - p.window, pmin + 1), p.sinks);
+  __syncwarp();
+}
+
+// By one warp, a row of request b and kv head h anew, with few registers: for the kernels that fold pieces, where blocks are of few
+// rows. `sq`: HD floats of shared memory.
+template <int KV, int HD>
+__device__ __forceinline__ void redo1(const PagedDev& p, const Req& r, int b, int h, int rr, float* sq) {
+  constexpr int OKV = KV == KV_E4M3 ? KV_BF16 : KV;
+  const int lane = threadIdx.x & 31;
+  const int tok = rr / p.gqa, head = h * p.gqa + rr - tok * p.gqa, pos = r.pos0 + tok;
+  uint8_t* out = static_cast<uint8_t*>(p.out) + ((r.q0 + tok) * p.o_s0 + head * p.o_s1) * 2;
+  const float sl2 = p.scale_log2 * (p.kd ? p.kd[b * p.kd_s0 + h * p.kd_s1] : 1.f);
+  const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
+      // the row anew: a lane a key for the scores, lanes over the dims for O
+      const uint8_t* q = p.q + ((r.q0 + tok) * p.q_s0 + head * p.q_s1) * (KV == KV_E4M3 && p.q_kind == Q_SAME ? 1 : 2);
+      __syncwarp();
+      for (int d = lane; d < HD; d += 32) {
+        float x;
+        if (KV == KV_E4M3 && p.q_kind == Q_BF16_TO_E4M3) {
+          const uint32_t two = e4m3x2_to_f16x2(pack_e4m3x2(value_at<KV_BF16>(q, d), 0.f));
+          x = __half2float(__ushort_as_half(static_cast<unsigned short>(two)));
+        } else {
+          x = value_at<KV>(q, d);
+        }
+        sq[d] = x;
+      }
+      __syncwarp();
+      float o[HD / 32], m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int x = 0; x < HD / 32; ++x) o[x] = 0.f;
+      const int low = p.window >= 0 ? max(0, pos - p.window) : 0, sinks = min(p.sinks, low);
+      const int seen = pos < 0 ? 0 : sinks + pos + 1 - low;
+#pragma unroll 1
+      for (int i0 = 0; i0 < seen; i0 += 32) {
+        const int i = i0 + lane;
+        const uint8_t *k = nullptr, *v = nullptr;
+        float s = -INFINITY;
+        if (i < seen) {
+          rows_of(p, b, h, i < sinks ? i : low + i - sinks, k, v);
+          s = 0.f;
+          if (k)
+#pragma unroll 4
+            for (int d = 0; d < HD; ++d) s += value_at<KV>(k, d) * sq[d];
+          s *= sl2;
+        }
+        float top = s;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        top = fmaxf(top, m);
+        const float f = top == -INFINITY ? 1.f : ex2(m - top), e = i < seen ? ex2(s - (top == -INFINITY ? 0.f : top)) : 0.f;
+        m = top;
+        l = l * f + e;
+#pragma unroll
+        for (int x = 0; x < HD / 32; ++x) o[x] *= f;
+#pragma unroll 1
+        for (int x = 0; x < 32 && i0 + x < seen; ++x) {
+          const float w = __shfl_sync(0xffffffffu, e, x);
+          const uint8_t* row_v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), x));
+          if (row_v)
+#pragma unroll
+            for (int y = 0; y < HD / 32; ++y) {
+              const float u = value_at<KV>(row_v, y * 32 + lane);
+              o[y] += fabsf(u) <= 3.4028234663852886e38f ? w * u : u + w;  // (w: its score may be no number)
+            }
+        }
+      }
+#pragma unroll
+      for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+      const float one = l == 0.f ? 0.f : vds / l;
+#pragma unroll
+      for (int y = 0; y < HD / 32; ++y) {
+        const float u = l == 0.f ? 0.f : o[y] * one;
+        if (OKV == KV_FP16) reinterpret_cast<__half*>(out)[y * 32 + lane] = __float2half_rn(u);
+        else reinterpret_cast<__nv_bfloat16*>(out)[y * 32 + lane] = __float2bfloat16_rn(u);
+      }
+}
+
 constexpr int MEND_KEYS = 64;
-template <int HD, int NW>
 struct MendSmem {
-  float q[NW][HD];       // a warp's query row
   int keys[MEND_KEYS];   // V rows that are no numbers
   int n;
+  float q[4][256];       // ROWS 1: a warp's query row
 };
 // By the NW first warps of a CTA, which meet in `sync`: request b's rows row0 .. row0 + n of kv head h (row = token * GQA + head), of
-// which a warp takes first, first + step, ...; `r`: what the block's tiles were made of.
-template <int KV, int HD, int NW, typename Sync>
-__device__ __forceinline__ void mend(const PagedDev& p, const Req& r, int b, int h, int row0, int n, int first, int step, MendSmem<HD, NW>& sm,
-                                     Sync sync) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// which a warp has first, first + step, ..., and takes 16 or one at a time (ROWS); `r`: what the block's tiles were made of.
+template <int KV, int HD, int NW, int ROWS, typename Sync>
+__device__ __forceinline__ void mend(const PagedDev& p, const Req& r, int b, int h, int row0, int n, int first, int step, MendSmem& sm, Sync sync) {
+  constexpr int OKV = KV == KV_E4M3 ? KV_BF16 : KV;
+  const int lane = threadIdx.x & 31;
   const int pmin = r.pos0 + row0 / p.gqa, pmax = r.pos0 + (row0 + n - 1) / p.gqa;
-  auto rows_of = [&](int key, const uint8_t*& k, const uint8_t*& v) {  // null: a page that does not exist
-    const int page = p.pt[b * p.pt_s0 + (key >> p.page_shift) * p.pt_s1];
-    const bool real = page >= 0 && page < p.num_pages;
-    k = real ? p.k + page * p.k_s0 + (key & p.page_mask) * p.k_s1 + h * p.k_s2 : nullptr;
-    v = real ? p.v + page * p.v_s0 + (key & p.page_mask) * p.v_s1 + h * p.v_s2 : nullptr;
-  };
   sync();
   if (threadIdx.x == 0) sm.n = 0;
   sync();
@@ -313,7 +565,7 @@ __device__ __forceinline__ void mend(const PagedDev& p, const Req& r, int b, int
     for (int key = max(from, 0) + threadIdx.x; key < to; key += NW * 32) {
       const uint8_t *k, *v;
       if (key < least) continue;
-      rows_of(key, k, v);
+      rows_of(p, b, h, key, k, v);
       uint32_t any = 0;
       if (v) {
 #pragma unroll 1
@@ -333,91 +585,33 @@ __device__ __forceinline__ void mend(const PagedDev& p, const Req& r, int b, int
   sync();
   const int found = sm.n;
   if (found == 0) return;
-  const float sl2 = p.scale_log2 * (p.kd ? p.kd[b * p.kd_s0 + h * p.kd_s1] : 1.f);
-  const float vds = p.vd ? p.vd[b * p.vd_s0 + h * p.vd_s1] : 1.f;
 #pragma unroll 1
-  for (int row = first; row < n; row += step) {
-    const int rr = row0 + row, tok = rr / p.gqa, head = h * p.gqa + rr - tok * p.gqa, pos = r.pos0 + tok;
-    uint8_t* out = static_cast<uint8_t*>(p.out) + ((r.q0 + tok) * p.o_s0 + head * p.o_s1) * 2;
-    constexpr int OKV = KV == KV_E4M3 ? KV_BF16 : KV;
-    bool odd = found > MEND_KEYS;  // some value that the row does not see, and one of its own that is no number
-    for (int i = lane; i < found && i < MEND_KEYS; i += 32) {
-      const int key = sm.keys[i];
-      odd |= key > pos || (p.window >= 0 && key < pos - p.window && key >= p.sinks);
-    }
-    bool none = false;
-    for (int d = lane * 2; d < HD; d += 64) none |= not_finite<OKV>(*reinterpret_cast<const uint32_t*>(out + d * 2)) != 0;
-    if (!__any_sync(0xffffffffu, odd) || !__any_sync(0xffffffffu, none)) continue;
-    // the row anew: a lane a key for the scores, lanes over the dims for O
-    const uint8_t* q = p.q + ((r.q0 + tok) * p.q_s0 + head * p.q_s1) * (KV == KV_E4M3 && p.q_kind == Q_SAME ? 1 : 2);
-    __syncwarp();
-    for (int d = lane; d < HD; d += 32) {
-      float x;
-      if (KV == KV_E4M3 && p.q_kind == Q_BF16_TO_E4M3) {
-        const uint32_t two = e4m3x2_to_f16x2(pack_e4m3x2(value_at<KV_BF16>(q, d), 0.f));
-        x = __half2float(__ushort_as_half(static_cast<unsigned short>(two)));
-      } else {
-        x = value_at<KV>(q, d);
-      }
-      sm.q[warp][d] = x;
-    }
-    __syncwarp();
-    float o[HD / 32], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int x = 0; x < HD / 32; ++x) o[x] = 0.f;
-    const int low = p.window >= 0 ? max(0, pos - p.window) : 0, sinks = min(p.sinks, low);
-    const int seen = pos < 0 ? 0 : sinks + pos + 1 - low;
+  for (int base = first; base < n; base += ROWS * step) {
+    // whether one of these rows is no number somewhere, and does not see all that was found
+    bool redo = false;
 #pragma unroll 1
-    for (int i0 = 0; i0 < seen; i0 += 32) {
-      const int i = i0 + lane;
-      const uint8_t *k = nullptr, *v = nullptr;
-      float s = -INFINITY;
-      if (i < seen) {
-        rows_of(i < sinks ? i : low + i - sinks, k, v);
-        s = 0.f;
-        if (k)
-#pragma unroll 4
-          for (int d = 0; d < HD; ++d) s += value_at<KV>(k, d) * sm.q[warp][d];
-        s *= sl2;
+    for (int row = base; row < n && row < base + ROWS * step; row += step) {
+      const int rr = row0 + row, tok = rr / p.gqa, pos = r.pos0 + tok;
+      const uint8_t* out = static_cast<const uint8_t*>(p.out) + ((r.q0 + tok) * p.o_s0 + (h * p.gqa + rr - tok * p.gqa) * p.o_s1) * 2;
+      bool odd = found > MEND_KEYS, none = false;
+      for (int i = lane; i < found && i < MEND_KEYS; i += 32) {
+        const int key = sm.keys[i];
+        odd |= key > pos || (p.window >= 0 && key < pos - p.window && key >= p.sinks);
       }
-      float top = s;
-#pragma unroll
-      for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-      top = fmaxf(top, m);
-      const float f = top == -INFINITY ? 1.f : ex2(m - top), e = i < seen ? ex2(s - (top == -INFINITY ? 0.f : top)) : 0.f;
-      m = top;
-      l = l * f + e;
-#pragma unroll
-      for (int x = 0; x < HD / 32; ++x) o[x] *= f;
-#pragma unroll 1
-      for (int x = 0; x < 32 && i0 + x < seen; ++x) {
-        const float w = __shfl_sync(0xffffffffu, e, x);
-        const uint8_t* row_v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v), x));
-        if (row_v)
-#pragma unroll
-          for (int y = 0; y < HD / 32; ++y) {
-            const float u = value_at<KV>(row_v, y * 32 + lane);
-            o[y] += fabsf(u) <= 3.4028234663852886e38f ? w * u : u + w;  // (w: its score may be no number)
-          }
-      }
+      for (int d = lane * 2; d < HD; d += 64) none |= not_finite<OKV>(*reinterpret_cast<const uint32_t*>(out + d * 2)) != 0;
+      redo |= __any_sync(0xffffffffu, odd) && __any_sync(0xffffffffu, none);
     }
-#pragma unroll
-    for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    const float one = l == 0.f ? 0.f : vds / l;
-#pragma unroll
-    for (int y = 0; y < HD / 32; ++y) {
-      const float u = l == 0.f ? 0.f : o[y] * one;
-      if (OKV == KV_FP16) reinterpret_cast<__half*>(out)[y * 32 + lane] = __float2half_rn(u);
-      else reinterpret_cast<__nv_bfloat16*>(out)[y * 32 + lane] = __float2bfloat16_rn(u);
-    }
+    if (!redo) continue;
+    if (ROWS == 16) redo16<KV, HD>(p, r, b, h, row0, base, step, n);
+    else redo1<KV, HD>(p, r, b, h, row0 + base, sm.q[threadIdx.x >> 5]);
   }
 }
 
 // The same by a CTA of four warps, as a call: it is rare, and the kernel around it short.
-template <int KV, int HD>
+template <int KV, int HD, int ROWS>
 __device__ __noinline__ void mend_call(const PagedDev& p, const Req& r, int b, int h, int row0, int n, int first, int step) {
-  __shared__ MendSmem<HD, 4> sm;
-  mend<KV, HD, 4>(p, r, b, h, row0, n, first, step, sm, [] { __syncthreads(); });
+  __shared__ MendSmem sm;
+  mend<KV, HD, 4, ROWS>(p, r, b, h, row0, n, first, step, sm, [] { __syncthreads(); });
 }
 
 // Byte offset of 16-byte chunk `c` of row `r` in a tile whose rows hold RB bytes: rows lie one after the other in
@@ -707,7 +901,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_kernel(const __grid_const
           }
         }
       }
-      const bool open = n0 + T - 1 <= pos_first && (p.window < 0 || n0 >= pos_last - p.window || n0 + T <= p.sinks);
+      const bool open = all_see(p, n0, T, pos_first, pos_last);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float mx[2] = {-INFINITY, -INFINITY};
@@ -941,7 +1135,7 @@ __global__ void __launch_bounds__(128) attn_paged_mend(const __grid_constant__ P
       const int block = static_cast<int>(x / p.kvh), h = static_cast<int>(x - static_cast<long long>(block) * p.kvh);
       const int t0 = block * RC / p.gqa, t1 = (block * RC + RC - 1) / p.gqa;
       const Req r = req_info<32>(p, b, t0, t1 - t0 + 1);
-      mend_call<KV, HD>(p, r, b, h, block * RC, static_cast<int>(min(rows - static_cast<long long>(block) * RC, static_cast<long long>(RC))),
+      mend_call<KV, HD, 16>(p, r, b, h, block * RC, static_cast<int>(min(rows - static_cast<long long>(block) * RC, static_cast<long long>(RC))),
                         threadIdx.x >> 5, 4);
     }
     before += n;
@@ -995,7 +1189,12 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
   };
   const int c0 = owner(u0), c1 = owner(u1 - 1);
   if (c0 == c1) {  // its gang has written the rows
-    if (p.max_q == 1 || I::LOOKS) return;
+    if (p.max_q == 1) return;
+    if (I::LOOKS) {
+      if (__ldcg(p.ws_spoilt + c0 * p.kvh + h))
+        mend_call<I::KV, HD, 1>(p, r, b, h, block * I::RC, rows, blockIdx.z * 4 + warp, 4 * share);
+      return;
+    }
     constexpr int LPR = HD / 8;  // lanes a row, 16 bytes each
     const int row0 = (blockIdx.z * 4 + warp) * (32 / LPR) + lane / LPR;
     for (int row = row0; row < rows; row += 4 * share * (32 / LPR)) {
@@ -1006,7 +1205,7 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
     }
     if (__syncthreads_or(none))
       for (int s = 0; s < 32 / LPR; ++s)
-        mend_call<I::KV, HD>(p, r, b, h, block * I::RC, rows, (blockIdx.z * 4 + warp) * (32 / LPR) + s, 4 * share * (32 / LPR));
+        mend_call<I::KV, HD, 1>(p, r, b, h, block * I::RC, rows, (blockIdx.z * 4 + warp) * (32 / LPR) + s, 4 * share * (32 / LPR));
     return;
   }
   const int n = c1 - c0 + 1;  // every gang between them holds a piece too
@@ -1083,7 +1282,7 @@ __global__ void __launch_bounds__(128) attn_paged_combine(const __grid_constant_
     }
   }
   if (p.max_q > 1 && __syncthreads_or(none))
-    mend_call<I::KV, HD>(p, r, b, h, block * I::RC, rows, many ? (warp ? rows : blockIdx.z) : blockIdx.z * 4 + warp, many ? share : 4 * share);
+    mend_call<I::KV, HD, 1>(p, r, b, h, block * I::RC, rows, many ? (warp ? rows : blockIdx.z) : blockIdx.z * 4 + warp, many ? share : 4 * share);
 }
 
 }  // namespace paged

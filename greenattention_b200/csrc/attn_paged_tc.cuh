@@ -34,7 +34,7 @@
 // bytes a clock. Measured (bf16): 4 causal prompts of 4096 tokens, head_dim 256, 16 heads 652 us = 842 TFLOP/s, head_dim 128,
 // 32 heads 802 us = 685; 8 x 2048 tokens on 16k, head_dim 256, window 1024 and 4 first tokens 431 us; verify in slices, 32 x
 // 8192 tokens, 20 rows of 8 kv heads (1.07 GB) 191 us = 5.6 TB/s (299 on the warp-level kernel). Over an e4m3 cache the
-// gathering warps convert (exactly, to fp16), which bounds it: the windowed extend takes 1110 us.
+// gathering warps convert (exactly, to fp16), which bounds it: the windowed extend takes 1150 us.
 #pragma once
 
 #include "attn_paged.cuh"
@@ -263,6 +263,7 @@ __global__ void __launch_bounds__(1024) plan_split_kernel(const __grid_constant_
     }
     list[g] = e;
   }
+  for (int g = tid; g < G * p.kvh; g += 1024) p.ws_spoilt[g] = 0;
 }
 
 // The same for an e4m3 cache: 16 values of a key a load, converted to fp16 (exact) on the way into the stage. CPK: loads a key.
@@ -427,6 +428,13 @@ __device__ __forceinline__ float part_exp(uint32_t tS, float sl2, float mu, cons
   return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
+// What the softmax warps do when a result is no number: a call, so that it takes no registers from the tiles (in line prompts hd128
+// took 429 us instead of 300; a kernel behind, which finds nothing to do, costs every call 15 us).
+template <class I>
+__device__ __noinline__ void mend_tail(const PagedDev& p, const Req& r, int b, int h, int row0, int n, MendSmem& sm) {
+  mend<I::KV, I::HD, I::SOFT_WARPS, 16>(p, r, b, h, row0, n, threadIdx.x >> 5, I::SOFT_WARPS, sm, [] { named_bar_sync(3, I::SOFT_WARPS * 32); });
+}
+
 template <class I>
 __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_constant__ PagedDev p, const int* count, const int4* list,
                                                                  const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int boxes) {
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
   const uint32_t b_pv = b_p + 16;                            // NQ 1: PV out of a buffer done
   const uint32_t b_ofull = b_pv + 16, b_ofree = b_ofull + 16; // [2] O complete / read
   const uint32_t slot_at = b_ofree + 16;
-  const uint32_t spoilt = slot_at + 8;                       // [2] a result is no number, a wait of the softmax warps ran out
+  const uint32_t spoilt = slot_at + 8;                       // prompts [2]: a result is no number, a wait of the softmax warps ran out
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   constexpr int MMA_WARP = I::SOFT_WARPS, KV_WARP = MMA_WARP + 2, Q_WARP = KV_WARP + I::KV_WARPS;
 
@@ -728,7 +736,10 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
             }
           }
         }
-        if (not_finite<OKV>(acc)) asm volatile("st.shared.b32 [%0], %1;" ::"r"(spoilt), "r"(1) : "memory");
+        if (not_finite<OKV>(acc)) {
+          if (I::SPLIT_KV) p.ws_spoilt[blockIdx.x] = 1;  // for the combine kernel
+          else asm volatile("st.shared.b32 [%0], %1;" ::"r"(spoilt), "r"(1) : "memory");
+        }
       }
       if (real && half == 0 && last(work)) {
         if (I::SPLIT_KV && seg.slot >= 0) p.ws_lse[static_cast<long long>(seg.slot) * TM + row] = lse2;
@@ -741,20 +752,19 @@ __global__ void __launch_bounds__(I::NT, 1) attn_paged_tc_kernel(const __grid_co
         ++done;
       }
     }
-    // The CTA's blocks, or the requests that it has all of, once more if need be; the operands' shared memory is free.
-    auto sync = [] { named_bar_sync(3, I::SOFT_WARPS * 32); };
-    if (failed) asm volatile("st.shared.b32 [%0], %1;" ::"r"(spoilt + 4), "r"(1) : "memory");
-    sync();
-    uint32_t any, lost;  // (where a wait ran out copies may still be on their way)
-    asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(any), "=r"(lost) : "r"(spoilt) : "memory");
-    if (any && !lost) {
-      auto& sm = *reinterpret_cast<MendSmem<HD, I::SOFT_WARPS>*>(smem_raw);
-      Work again = begin();
-      Seg s;
-      while (next(again, s)) {
-        const int row0 = s.block * I::ROWS;
-        if (last(again) && !(I::SPLIT_KV && s.slot >= 0))
-          mend<KV, HD, I::SOFT_WARPS>(p, s.r, s.b, s.h, row0, min(s.r.nq * p.gqa - row0, I::ROWS), warp, I::SOFT_WARPS, sm, sync);
+    if (!I::SPLIT_KV) {  // the CTA's blocks once more if need be; the operands' shared memory is free
+      if (failed) asm volatile("st.shared.b32 [%0], %1;" ::"r"(spoilt + 4), "r"(1) : "memory");
+      named_bar_sync(3, I::SOFT_WARPS * 32);
+      uint32_t any, lost;  // (where a wait ran out copies may still be on their way)
+      asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(any), "=r"(lost) : "r"(spoilt) : "memory");
+      if (any && !lost) {
+        auto& sm = *reinterpret_cast<MendSmem*>(smem_raw);
+        Work again = begin();
+        Seg s;
+        while (next(again, s)) {
+          const int row0 = s.block * I::ROWS;
+          if (last(again)) mend_tail<I>(p, s.r, s.b, s.h, row0, min(s.r.nq * p.gqa - row0, I::ROWS), sm);
+        }
       }
     }
   } else {

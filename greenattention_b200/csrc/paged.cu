@@ -24,7 +24,7 @@ struct Launch {
 
 size_t prefix_bytes(int batch) { return (static_cast<size_t>(batch) + 1 + 63) / 64 * 256; }
 size_t slots_bytes(int sm) {
-  return (static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) + static_cast<size_t>(sm) * ga::paged::SEG_FLOATS + 64) * 4;
+  return (static_cast<size_t>(2 * sm) * (ga::paged::SLOT_FLOATS + ga::paged::SLOT_ROWS) + static_cast<size_t>(sm) * (ga::paged::SEG_FLOATS + 1)) * 4;
 }
 
 template <class I>
@@ -115,14 +115,14 @@ unsigned combine_shares(long long pairs, int rows, int sm) {
 }
 
 // Whether a call of at most 128 rows per kv head goes to the tensor-core kernel in slices. Both sides measured (bf16,
-// device time, warp-level kernel / tensor-core kernel): 32 x 8192 tokens, 8 kv heads, head_dim 128: 16 rows 174 / 190 us,
-// 20 rows 290 / 191, 128 rows (8 requests more) 298 / 79; head_dim 64: 20 rows 143 / 213, 64 rows 46 / 35 (8 x 2000);
-// head_dim 256 (32 x 4096): 2 rows 273 / 172, 20 rows 544 / 181; pages of one token, 20 rows: 99 / 111; 4 x 300 tokens,
-// head_dim 256: 17 / 24. So: where the warp-level kernel would read the keys more than once (over 32 rows, 16 at
+// device time, warp-level kernel / tensor-core kernel): 32 x 8192 tokens, 8 kv heads, head_dim 128: 16 rows 176 / 190 us,
+// 20 rows 294 / 194, 128 rows (8 requests) 297 / 80; head_dim 64: 20 rows 145 / 215, 64 rows 44 / 35 (8 x 2000);
+// head_dim 256 (32 x 4096): 2 rows 265 / 174, 20 rows 527 / 183; pages of one token (32 x 4096), 20 rows: 161 / 201; 4 x 300
+// tokens, head_dim 256: 27 / 28, both bound by the host. So: where the warp-level kernel would read the keys more than once (over 32 rows, 16 at
 // head_dim 256); at head_dim 128 from 17 rows and at 256 always, if pages are whole boxes and the call is not a small one.
 // An e4m3 cache is converted on the way into the stages, which costs more than reading it again a few times (16 x 8192
-// tokens: head_dim 128 64 rows 243 / 448 us, 128 rows 448 / 463; head_dim 256 64 rows 569 / 877, 128 rows 1101 / 904; head_dim
-// 64 64 rows 141 / 190, 128 rows 264 / 200): from 65 rows on.
+// tokens: head_dim 128 64 rows 260 / 384 us, 128 rows 475 / 403; head_dim 256 64 rows 564 / 886, 128 rows 1088 / 911; head_dim
+// 64 64 rows 143 / 223, 128 rows 266 / 233): from 65 rows on.
 template <int KV>
 bool split_on_tensor_cores(const Launch& a, int hd) {
   const long long rows = static_cast<long long>(a.d.max_q) * a.d.gqa;

@@ -161,7 +161,7 @@ class PagePool:
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor) -> None:
         """Page ``dst[i]`` becomes a copy of page ``src[i]`` in every tensor; counts and table stay. Of entries with one
-        destination the last counts. An entry whose source another entry writes is left out (status 10): what it would
+        destination the last counts; one that copies a page onto itself says nothing. An entry whose source another entry writes is left out (status 10): what it would
         copy depends on the order. Entries that name no page are left out (status 7)."""
         is64 = self._pair("src", src, "dst", dst)
         n = src.shape[0]

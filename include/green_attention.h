@@ -178,7 +178,8 @@ typedef struct GaGdnVerifyParams {
  * optional left window and `sink_tokens` first tokens that stay visible beside it. Key j is visible to the query at
  * position p when j <= p and (window_left < 0 or j >= p - window_left or j < sink_tokens). Page-table entries of pages
  * without a visible key are never read (they may be released pages' or padding). A row without visible keys gets zeros
- * and an LSE of -inf; rows of q / out / lse past cu_seqlens_q[batch] are left alone. No counterpart in the reference
+ * and an LSE of -inf; rows of q / out / lse past cu_seqlens_q[batch] are left alone. Infinities and NaN of K and V reach
+ * the rows that see them and no others. No counterpart in the reference
  * (its kernels read e4m3 caches and have no first tokens). */
 typedef struct GaPagedParams {
   int32_t kv_type;          /* 0 bf16, 1 fp16, 2 e4m3 */
@@ -276,7 +277,7 @@ size_t ga_paged_workspace_bytes(int device, int max_batch);
 int ga_paged_attend(const GaPagedParams* p, void* stream);
 /* Scratch of a call with `n` entries. Indices are int32, or int64 where is64 is 1. */
 size_t ga_pages_scratch_bytes(const GaPagePool* p, int n);
-/* Page dst[i] becomes a copy of page src[i] in every tensor. Of entries with one dst the last counts; an entry whose src
+/* Page dst[i] becomes a copy of page src[i] in every tensor (onto itself: nothing). Of entries with one dst the last counts; an entry whose src
  * another entry writes is left out (10). */
 int ga_pages_copy(const GaPagePool* p, const void* src, const void* dst, int is64, int n, void* stream);
 /* Row children[i] (empty) becomes a copy of row parents[i]: full pages are shared, the tokens of a partial last page are
